@@ -563,6 +563,76 @@ int sln_conv2d_wgrad_f32(const uint16_t *gz_parts, int Cout, int Cout_pad, const
                          int OH, int OW, float *gw, const float *gz_scale, const float *x_scale,
                          void *workspace, size_t workspace_bytes, int gw_layout, sln_stream_t stream);
 
+/* ---------------------------------------------------------------------------
+ * Microscaled 4-bit operands (no reference counterpart: a fourth operand format for the row products of the heads,
+ * next to the 2 x fp16, 3 x bf16 and 1 x fp16 ones; csrc/mx4.hip has the format).
+ *
+ * A matrix [R][K] is held as codes (two e2m1 values per byte, the lower nibble first; row pitch Kp / 2 bytes, Kp =
+ * sln_mx4_row_values(K) = K rounded up to 256, the padding zero) and scales (one byte s + 127 per 32 values of a row: the
+ * block's values are code * 2^s; 255: all NaN; row pitch Kp / 32).  Codes start on 16-byte, scales on 8-byte boundaries.
+ * dtype: SLN_DTYPE_*.  K <= 2^22.
+ * ------------------------------------------------------------------------- */
+#define SLN_DTYPE_F32 0
+#define SLN_DTYPE_BF16 1
+#define SLN_DTYPE_F16 2
+int64_t sln_mx4_row_values(int64_t K);
+/* x [R][K], row stride `stride` elements -> codes, scales (fully written, padding included). */
+int sln_mx4_round(const void *x, int dtype, int64_t R, int64_t K, int64_t stride, uint8_t *codes, uint8_t *scales,
+                  sln_stream_t stream);
+/* The values that codes stand for -> out [R][K] (rounded to dtype; exact in f32 and bf16). */
+int sln_mx4_values(const uint8_t *codes, const uint8_t *scales, int64_t R, int64_t K, void *out, int dtype,
+                   sln_stream_t stream);
+/* y [M][N] = act((a b^T) * scale[n] + bias[n]), a [M][K] and b [N][K] rounded; scale / bias f32 [N] or NULL; relu: act =
+ * max(0, .) (a NaN stays).  Workspace: sln_mx4_product_workspace_bytes(M, N, K, 1) (0: none needed).  Bit-reproducible. */
+size_t sln_mx4_product_workspace_bytes(int64_t M, int64_t N, int64_t K, int rounded);
+int sln_mx4_product(const uint8_t *a_codes, const uint8_t *a_scales, const uint8_t *b_codes, const uint8_t *b_scales,
+                    int64_t M, int64_t N, int64_t K, const float *scale, const float *bias, int relu, void *y, int dtype,
+                    void *workspace, size_t workspace_bytes, sln_stream_t stream);
+/* The same for up to 16 rows of x that are rounded on the way (same values as sln_mx4_round + sln_mx4_product, another
+ * order of the sum).  Workspace: sln_mx4_product_workspace_bytes(M, N, K, 0). */
+int sln_mx4_rows_product(const void *x, int dtype, int64_t M, int64_t K, int64_t stride, const uint8_t *b_codes,
+                         const uint8_t *b_scales, int64_t N, const float *scale, const float *bias, int relu, void *y,
+                         void *workspace, size_t workspace_bytes, sln_stream_t stream);
+/* Straight-through gradients of y = act((x^ w^T) * scale + bias): gy [M][N] in dtype (row stride gy_stride), y [M][N] in
+ * dtype: the output, gy counts where it is > 0 (NULL: everywhere); gx [M][K] in dtype, gw [N][K] f32, gb [N] f32, each
+ * NULL if not wanted.  Workspace (256-byte boundary): sln_mx4_linear_bwd_workspace_bytes.  Bit-reproducible. */
+size_t sln_mx4_linear_bwd_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype, int want_gx, int want_gw,
+                                          int want_gb);
+int sln_mx4_linear_bwd(const void *gy, int dtype, int64_t gy_stride, const void *y, const float *scale,
+                       const uint8_t *x_codes, const uint8_t *x_scales, const uint8_t *w_codes, const uint8_t *w_scales,
+                       int64_t M, int64_t N, int64_t K, void *gx, float *gw, float *gb, void *workspace,
+                       size_t workspace_bytes, sln_stream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * Newton-Schulz orthogonalisation of n matrices, and the optimiser step built on it (csrc/ortho.hip has the iteration).
+ * `descs` is HOST memory (copied into the launches).  Matrices may have any shape (an empty one is skipped; the shorter
+ * side at most 65535, the longer 2^22); they are processed together, every launch covers all of them.
+ * Workspace (256-byte boundary): the function next to the entry point (0: nothing to do or a shape out of range).
+ * ------------------------------------------------------------------------- */
+typedef struct {
+    const void *g;                /* [rows][cols], row stride g_stride   */
+    void *out;                    /* [rows][cols], row stride out_stride */
+    int64_t g_stride, out_stride;
+    int32_t rows, cols;
+} sln_ortho_desc_t;
+size_t sln_orthogonalize_workspace_bytes(const sln_ortho_desc_t *descs, int n);
+int sln_orthogonalize(const sln_ortho_desc_t *descs, int n, int dtype, int steps, float eps, void *workspace,
+                      size_t workspace_bytes, sln_stream_t stream);
+/* One update of n weight matrices (dense [rows][cols] f32): with cf = min(1, max_norm / (sqrt(*sqnorm) + 1e-6)),
+ *   momentum <- mu momentum + cf grad;  u = nesterov ? cf grad + mu momentum : momentum;
+ *   param <- param * decay - lr * orthogonalised(u)
+ * Nothing is written if *sqnorm (device, from sln_grad_sqnorm_f32 over ALL gradients of the step) is not finite. */
+typedef struct {
+    float *param;
+    const float *grad;
+    float *momentum;
+    int32_t rows, cols;
+    float lr, decay;
+} sln_muon_desc_t;
+size_t sln_muon_step_workspace_bytes(const sln_muon_desc_t *descs, int n);
+int sln_muon_step_f32(const sln_muon_desc_t *descs, int n, int steps, float eps, const double *sqnorm, float max_norm,
+                      float mu, int nesterov, void *workspace, size_t workspace_bytes, sln_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

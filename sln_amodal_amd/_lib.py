@@ -14,6 +14,7 @@ _lib = None
 _p = C.c_void_p
 _i = C.c_int
 _f = C.c_float
+_l = C.c_int64
 
 # name -> (restype, argtypes); mirrors include/sln_amodal.h one to one.
 SIGNATURES = {
@@ -86,6 +87,18 @@ SIGNATURES = {
     "sln_wgrad_reduce_batch_f32": (_i, [_p, _i, _p]),
     "sln_conv2d_wgrad_f32": (_i, [_p, _i, _i, _p, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i,
                                   _i, _i, _i, _i, _p, _p, _p, _p, C.c_size_t, _i, _p]),
+    "sln_mx4_row_values": (_l, [_l]),
+    "sln_mx4_round": (_i, [_p, _i, _l, _l, _l, _p, _p, _p]),
+    "sln_mx4_values": (_i, [_p, _p, _l, _l, _p, _i, _p]),
+    "sln_mx4_product_workspace_bytes": (C.c_size_t, [_l, _l, _l, _i]),
+    "sln_mx4_product": (_i, [_p, _p, _p, _p, _l, _l, _l, _p, _p, _i, _p, _i, _p, C.c_size_t, _p]),
+    "sln_mx4_rows_product": (_i, [_p, _i, _l, _l, _l, _p, _p, _l, _p, _p, _i, _p, _p, C.c_size_t, _p]),
+    "sln_mx4_linear_bwd_workspace_bytes": (C.c_size_t, [_l, _l, _l, _i, _i, _i, _i]),
+    "sln_mx4_linear_bwd": (_i, [_p, _i, _l, _p, _p, _p, _p, _p, _p, _l, _l, _l, _p, _p, _p, _p, C.c_size_t, _p]),
+    "sln_orthogonalize_workspace_bytes": (C.c_size_t, [_p, _i]),
+    "sln_orthogonalize": (_i, [_p, _i, _i, _i, _f, _p, C.c_size_t, _p]),
+    "sln_muon_step_workspace_bytes": (C.c_size_t, [_p, _i]),
+    "sln_muon_step_f32": (_i, [_p, _i, _i, _f, _p, _f, _f, _i, _p, C.c_size_t, _p]),
 }
 
 

@@ -84,6 +84,14 @@ class Config(object):
     # convolutions (regular expression on the weight's name) that run in the strict 3 x bf16 operand format instead of
     # the default 2 x scaled fp16 (MaskRCNN.set_strict_layers)
     STRICT_LAYERS = os.environ.get("SLN_STRICT_LAYERS", "")
+    # layers of the classifier head (regular expression on the weight's name) whose products run on microscaled 4-bit
+    # operands, forward; backward straight through the rounding (MaskRCNN.set_mx4_layers)
+    MX4_LAYERS = os.environ.get("SLN_MX4_LAYERS", "")
+    # "sgd" (optim.ClippedSGD, the reference's rule) or "muon" (optim.ClippedMuon: orthogonalised momentum for the weight
+    # matrices at MUON_LR_RATIO times the learning rate, ClippedSGD's rule for the biases)
+    OPTIMIZER = os.environ.get("SLN_OPTIMIZER", "sgd")
+    MUON_LR_RATIO = 20.0
+    MUON_MOMENTUM = 0.95
 
     def __init__(self):
         self.IMAGE_SHAPE = np.array([self.IMAGE_MAX_DIM, self.IMAGE_MAX_DIM, 3])

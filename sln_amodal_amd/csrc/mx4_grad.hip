@@ -1,0 +1,291 @@
+// Straight-through gradients of the 4-bit layer y = act((x^ w^T) * scale + bias), x^ and w^ rounded (gfx950):
+//
+//   z = gy [y > 0],   gx = (z scale) w^,   gw = scale (z^T x^),   gb = sum over the rows of z
+//
+// The rounding passes its gradient through unchanged, saturated values included.  w^ and x^ are what the forward
+// multiplied: e2m1 values times powers of two have two significant bits, so ONE bf16 part holds them exactly, and a
+// float32 gradient is exactly the sum of three bf16 parts (8 bits of its significand each, cut, not rounded).
+// Three (two: 16-bit gradients) products on the bf16 matrix instructions into fp32 accumulators are therefore the
+// float32 products: nothing is rounded before the sum.  (Parts below bf16's smallest normal, 2^-126, may be lost.)
+// For 16-bit types z * scale is cut to 16 bits: gx has 8 or 11.
+//
+// Both products contract along rows (mfma_nt.h): gx over the outputs, so w^ is laid out [K][N]; gw over the rows of the
+// batch, so z is laid out [N][M] and x^ [K][M].
+#include "mx4.h"
+
+#define MG_PITCH 65
+
+__device__ __forceinline__ void mg_cut(float v, int parts, __bf16 *h) {
+    if (!(fabsf(v) < INFINITY)) {                  // one part carries it; inf - inf would make a NaN of an infinity
+        h[0] = (__bf16)v;
+        for (int p = 1; p < parts; ++p) h[p] = (__bf16)0.f;
+        return;
+    }
+    for (int p = 0; p < parts; ++p) {
+        const float c = __uint_as_float(__float_as_uint(v) & 0xffff0000u);
+        h[p] = (__bf16)c;
+        v -= c;
+    }
+}
+// values k ... k + 7 (k a multiple of 8) of parts row `row`
+template <int P>
+__device__ __forceinline__ void mg_store8(char *base, int64_t row, int64_t row_bytes, int k, const float *v) {
+    char *at = base + row * row_bytes + (k >> 5) * (64 * P) + (k & 31) * 2;
+    b16x8 h[P];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        __bf16 q[P];
+        mg_cut(v[e], P, q);
+#pragma unroll
+        for (int p = 0; p < P; ++p) h[p][e] = q[p];
+    }
+#pragma unroll
+    for (int p = 0; p < P; ++p) *(b16x8 *)(at + p * 64) = h[p];
+}
+__host__ __device__ __forceinline__ int64_t mg_row_bytes(int64_t k, int parts) { return (k + 31) / 32 * 64 * parts; }
+
+// Block = 64 x 64 of gy: parts of z * scale (rows M) and of z^T (rows N), one partial bias sum per column.
+template <typename T, int P>
+__global__ __launch_bounds__(256) void mx4_grad_split_kernel(const T *__restrict__ gy, int64_t stride,
+                                                             const T *__restrict__ y, const float *__restrict__ scale,
+                                                             int M, int N, char *__restrict__ rows,
+                                                             char *__restrict__ cols, float *__restrict__ bias_part) {
+    __shared__ float z[64 * MG_PITCH];
+    __shared__ float s_bias[4][64];
+    const int t = threadIdx.x, m0 = blockIdx.y * 64, n0 = blockIdx.x * 64;
+    float sum = 0.f;
+    for (int i = t >> 6; i < 64; i += 4) {
+        const int m = m0 + i, n = n0 + (t & 63);
+        float v = 0.f;
+        if (m < M && n < N) {
+            v = (float)gy[(int64_t)m * stride + n];
+            if (y && !((float)y[(int64_t)m * N + n] > 0.f)) v = 0.f;
+        }
+        z[i * MG_PITCH + (t & 63)] = v;
+        sum += v;
+    }
+    s_bias[t >> 6][t & 63] = sum;
+    __syncthreads();
+    if (bias_part && t < 64 && n0 + t < N)
+        bias_part[(int64_t)blockIdx.y * N + n0 + t] = (s_bias[0][t] + s_bias[1][t]) + (s_bias[2][t] + s_bias[3][t]);
+    if (rows) {
+        const int64_t rb = mg_row_bytes(N, P);
+        const int npad = (N + 31) & ~31;
+        for (int e = t; e < 512; e += 256) {
+            const int i = e >> 3, k = (e & 7) * 8;
+            if (m0 + i >= M || n0 + k >= npad) continue;
+            float v[8];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                v[q] = z[i * MG_PITCH + k + q];
+                if (scale && n0 + k + q < N) v[q] *= scale[n0 + k + q];
+            }
+            mg_store8<P>(rows, m0 + i, rb, n0 + k, v);
+        }
+    }
+    if (cols) {
+        const int64_t rb = mg_row_bytes(M, P);
+        const int mpad = (M + 31) & ~31;
+        for (int e = t; e < 512; e += 256) {
+            const int j = e >> 3, k = (e & 7) * 8;
+            if (n0 + j >= N || m0 + k >= mpad) continue;
+            float v[8];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) v[q] = z[(k + q) * MG_PITCH + j];
+            mg_store8<P>(cols, n0 + j, rb, m0 + k, v);
+        }
+    }
+}
+
+// Partial bias sums, added in order in double.
+__global__ __launch_bounds__(64) void mx4_grad_bias_kernel(const float *__restrict__ part, int blocks, int N,
+                                                           float *__restrict__ gb) {
+    const int n = blockIdx.x * 64 + threadIdx.x;
+    if (n >= N) return;
+    double s = 0.0;
+    for (int b = 0; b < blocks; ++b) s += part[(int64_t)b * N + n];
+    gb[n] = (float)s;
+}
+
+// Codes [R][K] -> bf16 values as parts rows [K][R].  Block = 64 x 64.
+__global__ __launch_bounds__(256) void mx4_grad_turn_kernel(const unsigned *__restrict__ codes,
+                                                            const uint8_t *__restrict__ scales, int R, int K, int64_t kp,
+                                                            char *__restrict__ out) {
+    __shared__ float z[64 * MG_PITCH];
+    const int t = threadIdx.x, r0 = blockIdx.y * 64, k0 = blockIdx.x * 64;
+    for (int e = t; e < 512; e += 256) {
+        const int i = e >> 3, k = k0 + (e & 7) * 8;
+        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (r0 + i < R && k < kp) {
+            const int64_t at = (int64_t)(r0 + i) * (kp / 8) + k / 8;
+            mx_values8(codes[at], scales[at >> 2], v);
+        }
+#pragma unroll
+        for (int q = 0; q < 8; ++q) z[i * MG_PITCH + (e & 7) * 8 + q] = v[q];
+    }
+    __syncthreads();
+    const int64_t rb = mg_row_bytes(R, 1);
+    const int rpad = (R + 31) & ~31;
+    for (int e = t; e < 512; e += 256) {
+        const int j = e >> 3, i = (e & 7) * 8;
+        if (k0 + j >= K || r0 + i >= rpad) continue;
+        float v[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] = z[(i + q) * MG_PITCH + j];
+        mg_store8<1>(out, k0 + j, rb, r0 + i, v);
+    }
+}
+
+struct MgProduct {
+    const char *a, *b;            // parts rows: a [RA] of P parts, b [RB] of one
+    int RA, RB, groups, nsplit;
+    const float *row_scale;       // per row of the result, or NULL
+    void *c;                      // [RA][RB]
+    float *slab;
+};
+
+template <typename T>
+__device__ __forceinline__ void mg_finish(const MgProduct &p, int i, int64_t at, float v) {
+    ((T *)p.c)[at] = (T)(p.row_scale ? v * p.row_scale[i] : v);
+}
+
+template <typename T, int P>
+__global__ __launch_bounds__(256, 2) void mx4_grad_product_kernel(const MgProduct p, int tiles) {
+    __shared__ __attribute__((aligned(128))) char smem[2 * NtShape<P, 1>::STAGE];
+    const int at = nt_xcd_order(blockIdx.x, tiles);
+    const int ta = (p.RA + NT_TILE - 1) / NT_TILE;
+    const int split = at % p.nsplit, tile = at / p.nsplit;
+    const int i0 = tile % ta * NT_TILE, j0 = tile / ta * NT_TILE;
+    const int64_t ra = (int64_t)p.groups * 64 * P, rb = (int64_t)p.groups * 64;
+    const int g0 = (int)((int64_t)p.groups * split / p.nsplit), g1 = (int)((int64_t)p.groups * (split + 1) / p.nsplit);
+    f32x16 acc[2][2];
+    nt_tile<b16x8, P, 1, NT_EXACTB>(p.a + i0 * ra, ra, p.RA - i0, p.b + j0 * rb, rb, p.RB - j0, g0, g1, smem, acc);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int col = j0 + 64 * (wave & 1) + 32 * j + (lane & 31);
+            if (col >= p.RB) continue;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int row = i0 + 64 * (wave >> 1) + 32 * i + nt_acc_row(r, lane);
+                if (row >= p.RA) continue;
+                const int64_t e = (int64_t)row * p.RB + col;
+                if (p.nsplit > 1) p.slab[(int64_t)split * p.RA * p.RB + e] = acc[i][j][r];
+                else mg_finish<T>(p, row, e, acc[i][j][r]);
+            }
+        }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void mx4_grad_join_kernel(const MgProduct p) {
+    const int64_t total = (int64_t)p.RA * p.RB;
+    for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < total; e += (int64_t)gridDim.x * 256) {
+        float v = 0.f;
+        for (int k = 0; k < p.nsplit; ++k) v += p.slab[k * total + e];
+        mg_finish<T>(p, (int)(e / p.RB), e, v);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ host side
+struct MgPlan {
+    int64_t z_rows, z_cols, wt, xt, bias, slab, bytes;
+    int gx_cuts, gw_cuts;
+};
+static inline int64_t mg_align(int64_t v) { return (v + 255) & ~(int64_t)255; }
+static inline int mg_cuts(int64_t RA, int64_t RB, int64_t groups) {
+    const int64_t tiles = ((RA + NT_TILE - 1) / NT_TILE) * ((RB + NT_TILE - 1) / NT_TILE);
+    int64_t c = 512 / (tiles < 1 ? 1 : tiles);
+    if (c > groups / 8) c = groups / 8;
+    if (c > 32) c = 32;
+    return c < 1 ? 1 : (int)c;
+}
+static void mg_plan(int64_t M, int64_t N, int64_t K, int parts, bool gx, bool gw, bool gb, MgPlan &p) {
+    int64_t at = 0;
+    p.gx_cuts = mg_cuts(M, K, (N + 31) / 32);
+    p.gw_cuts = mg_cuts(N, K, (M + 31) / 32);
+    p.z_rows = at; at += gx ? mg_align(M * mg_row_bytes(N, parts)) : 0;
+    p.z_cols = at; at += gw ? mg_align(N * mg_row_bytes(M, parts)) : 0;
+    p.wt = at; at += gx ? mg_align(K * mg_row_bytes(N, 1)) : 0;
+    p.xt = at; at += gw ? mg_align(K * mg_row_bytes(M, 1)) : 0;
+    p.bias = at; at += gb ? mg_align((M + 63) / 64 * N * 4) : 0;
+    int64_t slab = 0;
+    if (gx && p.gx_cuts > 1) slab = p.gx_cuts * M * K * 4;
+    if (gw && p.gw_cuts > 1 && p.gw_cuts * N * K * 4 > slab) slab = p.gw_cuts * N * K * 4;
+    p.slab = at; at += mg_align(slab);
+    p.bytes = at;
+}
+static inline int mg_parts(int dtype) { return dtype == SLN_DTYPE_F32 ? 3 : 2; }
+
+extern "C" size_t sln_mx4_linear_bwd_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype, int want_gx, int want_gw,
+                                                     int want_gb) {
+    if (M < 1 || N < 1 || K < 1) return 0;
+    MgPlan p;
+    mg_plan(M, N, K, mg_parts(dtype), want_gx, want_gw, want_gb, p);
+    return (size_t)p.bytes;
+}
+
+template <typename T, int P>
+static void mg_product(const char *a, int64_t RA, const char *b, int64_t RB, int64_t k, int cuts, const float *row_scale,
+                       void *c, float *slab, hipStream_t st) {
+    const MgProduct p = {a, b, (int)RA, (int)RB, (int)((k + 31) / 32), cuts, row_scale, c, slab};
+    const int64_t tiles = ((RA + NT_TILE - 1) / NT_TILE) * ((RB + NT_TILE - 1) / NT_TILE) * cuts;
+    hipLaunchKernelGGL((mx4_grad_product_kernel<T, P>), dim3((unsigned)tiles), dim3(256), 0, st, p, (int)tiles);
+    if (cuts > 1) {
+        const int64_t blocks = (RA * RB + 255) / 256;
+        hipLaunchKernelGGL((mx4_grad_join_kernel<T>), dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, p);
+    }
+}
+
+template <typename T, int P>
+static void mg_run(const void *gy, int64_t stride, const void *y, const float *scale, const uint8_t *xc, const uint8_t *xs,
+                   const uint8_t *wc, const uint8_t *wsc, int64_t M, int64_t N, int64_t K, void *gx, float *gw, float *gb,
+                   char *ws, hipStream_t st) {
+    MgPlan pl;
+    mg_plan(M, N, K, P, gx, gw, gb, pl);
+    const int64_t kp = sln_mx4_row_values(K);
+    const dim3 gn((unsigned)((N + 63) / 64), (unsigned)((M + 63) / 64));
+    hipLaunchKernelGGL((mx4_grad_split_kernel<T, P>), gn, dim3(256), 0, st, (const T *)gy, stride, (const T *)y, scale,
+                       (int)M, (int)N, gx ? ws + pl.z_rows : nullptr, gw ? ws + pl.z_cols : nullptr,
+                       gb ? (float *)(ws + pl.bias) : nullptr);
+    if (gb)
+        hipLaunchKernelGGL(mx4_grad_bias_kernel, dim3((unsigned)((N + 63) / 64)), dim3(64), 0, st,
+                           (const float *)(ws + pl.bias), (int)((M + 63) / 64), (int)N, gb);
+    if (gx) {
+        hipLaunchKernelGGL(mx4_grad_turn_kernel, dim3((unsigned)((K + 63) / 64), (unsigned)((N + 63) / 64)), dim3(256), 0,
+                           st, (const unsigned *)wc, wsc, (int)N, (int)K, kp, ws + pl.wt);
+        mg_product<T, P>(ws + pl.z_rows, M, ws + pl.wt, K, N, pl.gx_cuts, nullptr, gx, (float *)(ws + pl.slab), st);
+    }
+    if (gw) {
+        hipLaunchKernelGGL(mx4_grad_turn_kernel, dim3((unsigned)((K + 63) / 64), (unsigned)((M + 63) / 64)), dim3(256), 0,
+                           st, (const unsigned *)xc, xs, (int)M, (int)K, kp, ws + pl.xt);
+        mg_product<float, P>(ws + pl.z_cols, N, ws + pl.xt, K, M, pl.gw_cuts, scale, gw, (float *)(ws + pl.slab), st);
+    }
+}
+
+extern "C" int sln_mx4_linear_bwd(const void *gy, int dtype, int64_t gy_stride, const void *y, const float *scale,
+                                  const uint8_t *x_codes, const uint8_t *x_scales, const uint8_t *w_codes,
+                                  const uint8_t *w_scales, int64_t M, int64_t N, int64_t K, void *gx, float *gw, float *gb,
+                                  void *workspace, size_t workspace_bytes, sln_stream_t stream) {
+    if ((dtype != SLN_DTYPE_F32 && dtype != SLN_DTYPE_BF16 && dtype != SLN_DTYPE_F16) || M < 1 || N < 1 || K < 1 ||
+        gy_stride < N || !gy)
+        return SLN_ERR_INVALID_ARG;
+    if (M > (1 << 21) || N > (1 << 21) || K > MX_MAX_K) return SLN_ERR_UNSUPPORTED;   // grid.y, 128 rows below 2^32 B
+    if ((gx && (!w_codes || !w_scales)) || (gw && (!x_codes || !x_scales))) return SLN_ERR_INVALID_ARG;
+    MgPlan pl;
+    mg_plan(M, N, K, mg_parts(dtype), gx, gw, gb, pl);
+    if (pl.bytes && (!workspace || ((uintptr_t)workspace & 255))) return SLN_ERR_INVALID_ARG;
+    if (workspace_bytes < (size_t)pl.bytes) return SLN_ERR_WORKSPACE;
+    if (!gx && !gw && !gb) return SLN_OK;
+    sln_enter();
+    char *ws = (char *)workspace;
+    hipStream_t st = (hipStream_t)stream;
+    if (dtype == SLN_DTYPE_F32)
+        mg_run<float, 3>(gy, gy_stride, y, scale, x_codes, x_scales, w_codes, w_scales, M, N, K, gx, gw, gb, ws, st);
+    else if (dtype == SLN_DTYPE_BF16)
+        mg_run<__bf16, 2>(gy, gy_stride, y, scale, x_codes, x_scales, w_codes, w_scales, M, N, K, gx, gw, gb, ws, st);
+    else
+        mg_run<_Float16, 2>(gy, gy_stride, y, scale, x_codes, x_scales, w_codes, w_scales, M, N, K, gx, gw, gb, ws, st);
+    return sln_launch_status();
+}

@@ -120,6 +120,25 @@ class MaskRCNN(nn.Module):
         # (_training_heads; opt-in, bench.py reports it as a second number).
         self.mask_train_slots = None
         self.set_strict_layers(getattr(config, "STRICT_LAYERS", ""))
+        self.set_mx4_layers(getattr(config, "MX4_LAYERS", ""))
+
+    def set_mx4_layers(self, pattern):
+        """Layers of the classifier head whose weight's name matches the regular expression `pattern` (fullmatch, like
+        set_trainable) multiply microscaled 4-bit operands (mx4.mx4_linear): their inputs and weights are rounded to
+        4.25 bits per value, sums are float32, and training passes the gradient straight through the rounding.  For
+        instance r"classifier\\.(conv1|conv2)\\.weight".  In evaluation a weight is rounded once per change of the
+        weight.  Config.MX4_LAYERS is the default ("" = none).  Raises ValueError if the pattern matches a weight whose
+        layer is not a product of rows (anything outside the classifier head).  Returns the number of tagged weights."""
+        heads = {"classifier.%s.weight" % n for n in ("conv1", "conv2", "linear_class", "linear_bbox")}
+        hit = {name: p for name, p in self.named_parameters()
+               if p.dim() >= 2 and pattern and re.fullmatch(pattern, name)}
+        if set(hit) - heads:
+            raise ValueError("no 4-bit form for %s: only the classifier head's layers are products of rows" %
+                             ", ".join(sorted(set(hit) - heads)[:3]))
+        for name, p in self.named_parameters():
+            p._sln_mx4 = name in hit
+        self.mx4_layers = pattern
+        return len(hit)
 
     def set_strict_layers(self, pattern):
         """Convolutions whose weight's name matches the regular expression `pattern` (fullmatch, like set_trainable)
@@ -196,6 +215,7 @@ class MaskRCNN(nn.Module):
         if glm:
             self.GLM_modual = DeepLabV2_ResNet101_MSC(cfg.GLM_CLASSES)
         self.set_strict_layers(getattr(self, "strict_layers", ""))     # (the replaced layers are new Parameters)
+        self.set_mx4_layers(getattr(self, "mx4_layers", ""))
         return self
 
     def set_trainable(self, layer_regex, model=None, indent=0, verbose=1, exclusive_off=True):
@@ -517,7 +537,22 @@ class MaskRCNN(nn.Module):
 
     def make_optimizer(self, learning_rate):
         """SGD, momentum, weight decay on everything but 'bn' parameters
-        (model.py:352-358)."""
+        (model.py:352-358).  Config.OPTIMIZER = "muon": weights of two or more axes take orthogonalised momentum at
+        MUON_LR_RATIO times the learning rate (optim.ClippedMuon), the rest as before."""
+        kind = getattr(self.config, "OPTIMIZER", "sgd")
+        if kind not in ("sgd", "muon"):
+            raise ValueError("Config.OPTIMIZER must be 'sgd' or 'muon', got %r" % (kind,))
+        if kind == "muon":
+            from .optim import ClippedMuon
+            named = [(n, p) for n, p in self.named_parameters() if p.requires_grad]
+            mats = [p for n, p in named if p.dim() >= 2 and "bn" not in n]
+            wd = [p for n, p in named if p.dim() < 2 and "bn" not in n]
+            no_wd = [p for n, p in named if "bn" in n]
+            decay, mu = self.config.WEIGHT_DECAY, self.config.LEARNING_MOMENTUM
+            return ClippedMuon([{"params": mats, "weight_decay": decay, "orthogonal": True,
+                                 "lr": learning_rate * self.config.MUON_LR_RATIO, "momentum": self.config.MUON_MOMENTUM},
+                                {"params": wd, "weight_decay": decay, "momentum": mu}, {"params": no_wd, "momentum": mu}],
+                               lr=learning_rate)
         wd = [p for n, p in self.named_parameters() if p.requires_grad and "bn" not in n]
         no_wd = [p for n, p in self.named_parameters() if p.requires_grad and "bn" in n]
         groups = [{"params": wd, "weight_decay": self.config.WEIGHT_DECAY}, {"params": no_wd}]

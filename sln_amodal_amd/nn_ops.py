@@ -70,6 +70,48 @@ def bn_affine(bn):
     return scale, shift
 
 
+def _mx4_rows(x, weight, w2, bias, scale, relu):
+    """act((x w2^T) * scale + bias) on microscaled 4-bit operands; w2() makes the [N, K] rows of `weight`.  In evaluation
+    the weight's codes are kept on the parameter until its version counter moves (edits through `.data` do not move it:
+    delete `weight._sln_mx4_codes` after one) or the stream changes; a captured graph rounds the weight itself, so that
+    its replays follow the weight and read no memory that is given back when the weight changes."""
+    from . import mx4
+    if not x.is_cuda:
+        raise RuntimeError("4-bit layers run on the GPU only (no CPU fallback in sln_amodal_amd)")
+    if torch.is_grad_enabled() and weight.requires_grad:
+        return mx4.mx4_linear(x, w2(), bias, scale=scale, relu=relu)
+    if torch.cuda.is_current_stream_capturing():
+        with torch.no_grad():
+            codes = mx4.mx4_quantize(w2())
+        return mx4.mx4_linear(x, codes, bias, scale=scale, relu=relu)
+    key = (weight._version, weight.data_ptr(), torch.cuda.current_stream(x.device).cuda_stream)
+    hit = getattr(weight, "_sln_mx4_codes", None)
+    if hit is None or hit[0] != key:
+        with torch.no_grad():
+            hit = weight._sln_mx4_codes = (key, mx4.mx4_quantize(w2()))
+    return mx4.mx4_linear(x, hit[1], bias, scale=scale, relu=relu)
+
+
+def _mx4_conv(x, conv, bn, relu):
+    """A tagged convolution that is one product of rows: a window as large as its input, or 1x1 with stride 1."""
+    kh, kw = conv.kernel_size
+    N, Cc, H, W = x.shape
+    whole = (kh, kw) == (H, W)
+    if conv.groups != 1 or not (whole or ((kh, kw) == (1, 1) and tuple(conv.stride) == (1, 1))) or \
+            tuple(conv.padding) != (0, 0):
+        raise RuntimeError("conv %s -> %s k%s on a %dx%d map is no product of rows: no 4-bit form" %
+                           (conv.in_channels, conv.out_channels, (kh, kw), H, W))
+    scale = shift = None
+    bias = conv.bias
+    if bn is not None:
+        scale, shift = bn_affine(bn)
+        bias = shift if bias is None else bias * scale + shift
+    rows = x.permute(0, 2, 3, 1).reshape(-1, kh * kw * Cc)
+    w2 = lambda: conv.weight.permute(0, 2, 3, 1).reshape(conv.out_channels, kh * kw * Cc)
+    y = _mx4_rows(rows, conv.weight, w2, bias, scale, relu)
+    return y.view((N, 1, 1, -1) if whole else (N, H, W, -1)).permute(0, 3, 1, 2)
+
+
 def conv_bn_act(x, conv, bn=None, relu=False, residual=None, same=False, link=None, chain_in=None,
                 chain_out=None, parts_only=False, pair=None, grad_inbox=None, pool_handoff=None):
     """x [B,C,H,W] (any memory format; channels-last preferred).
@@ -106,6 +148,10 @@ def conv_bn_act(x, conv, bn=None, relu=False, residual=None, same=False, link=No
         if residual is not None:
             y = y + residual
         return F.relu(y) if relu else y
+    if getattr(conv.weight, "_sln_mx4", False):
+        if residual is not None or same or not torch.is_tensor(x) or getattr(x, "_sln_po", None) is not None:
+            raise RuntimeError("a 4-bit layer takes a plain tensor, no shortcut, no padding")
+        return _mx4_conv(x, conv, bn, relu)
     stride, dilation = conv.stride, conv.dilation
     kh, kw = conv.kernel_size
     if same:   # (never with a MultiScale: the GLM uses symmetric padding)
@@ -411,6 +457,8 @@ def deconv2x2_relu_conv1x1(x, deconv, conv):
 
 def linear(x, lin):
     """nn.Linear on [R, C] rows through the same GEMM kernel (a 1x1 conv on R 1x1 'images')."""
+    if getattr(lin.weight, "_sln_mx4", False):
+        return _mx4_rows(x, lin.weight, lambda: lin.weight, lin.bias, None, False)
     hip = _hip_conv() if BACKEND in ("auto", "hip") else None
     if BACKEND != "torch" and x.is_cuda and (hip is None or x.shape[1] % 8):
         raise RuntimeError("linear with %d input features has no HIP path" % x.shape[1])

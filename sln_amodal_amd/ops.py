@@ -9,6 +9,7 @@ import ctypes as C
 import torch
 
 from . import _lib
+from .mx4 import Mx4Tensor, mx4_linear, mx4_quantize  # noqa: F401  (4-bit row products)
 
 LAYOUT_NCHW, LAYOUT_NHWC = 0, 1
 
@@ -365,3 +366,70 @@ def rle_encode(masks, max_runs):
     _lib.check(_lib.lib().sln_rle_encode_u8(_ptr(masks), N, a, int(max_runs), _ptr(counts), _ptr(num),
                                             _stream()), "sln_rle_encode_u8")
     return counts, num
+
+
+# ------------------------------------------------------------------ orthogonalised updates
+class _OrthoDesc(C.Structure):
+    _fields_ = [("g", C.c_void_p), ("out", C.c_void_p), ("g_stride", C.c_int64), ("out_stride", C.c_int64),
+                ("rows", C.c_int32), ("cols", C.c_int32)]
+
+
+_FLOATS = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def orthogonalize(x, steps=5, eps=1e-7):
+    """The nearly orthogonal factor of every matrix by Newton-Schulz products (csrc/ortho.hip): with X = x / (|x|_F + eps),
+    on the transpose where x is taller than wide, `steps` times X <- (a I + b A + c A^2) X, A = X X^T, (a, b, c) =
+    (3.4445, -4.7750, 2.0315).
+
+    x: a tensor [..., rows, cols] (a matrix or a stack of them) or a list / tuple of matrices of any shapes; float32,
+    bfloat16 or float16, one type and device for all.  Returns the same structure, the same types; a matrix of zeros stays
+    zero, one with an infinity or a NaN becomes NaN.  All matrices share every launch.  Products are float32-accurate
+    whatever the type, rounded once at the end.  No gradient."""
+    many = isinstance(x, (list, tuple))
+    mats = list(x) if many else [x]
+    for t in mats:
+        if not torch.is_tensor(t):
+            raise TypeError("orthogonalize takes tensors")
+        if not t.is_cuda:
+            raise RuntimeError("x must live on the GPU (no CPU fallback in sln_amodal_amd)")
+        if t.dtype not in _FLOATS:
+            raise TypeError("x must be float32, bfloat16 or float16, got %s" % t.dtype)
+        if t.dim() < 2 or (many and t.dim() != 2):
+            raise ValueError("orthogonalize takes matrices [rows, cols] (or one stack [..., rows, cols]), got %s" %
+                             (tuple(t.shape),))
+        if t.dtype != mats[0].dtype or t.device != mats[0].device:
+            raise ValueError("the matrices of one call share a type and a device")
+        if t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("orthogonalize has no gradient: detach x or call it under torch.no_grad()")
+        if min(t.shape[-2:]) > 65535 or max(t.shape[-2:]) > 1 << 22:
+            raise ValueError("orthogonalize: at most 65535 x 2^22, got %s" % (tuple(t.shape),))
+    if not 1 <= int(steps) <= 64 or not float(eps) >= 1e-30:
+        raise ValueError("orthogonalize: 1 <= steps <= 64 and eps >= 1e-30 (got %r, %r)" % (steps, eps))
+    outs, flat, keep = [], [], []
+    for t in mats:
+        o = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+        outs.append(o)
+        if t.numel() == 0:
+            continue
+        r, c = t.shape[-2:]
+        src = t.detach()
+        if src.dim() != 2:
+            src = src.reshape(-1, r, c)
+        if (c > 1 and src.stride(-1) != 1) or (r > 1 and src.stride(-2) < c):
+            src = src.contiguous()
+        keep.append(src)
+        gs = src.stride(-2) if r > 1 else c
+        es = t.element_size()
+        base, step = src.data_ptr(), (src.stride(0) * es if src.dim() == 3 else 0)
+        for b in range(src.shape[0] if src.dim() == 3 else 1):
+            flat.append((base + b * step, o.data_ptr() + b * r * c * es, gs, c, r, c))
+    if flat:
+        descs = (_OrthoDesc * len(flat))(*flat)
+        L = _lib.lib()
+        with torch.cuda.device(mats[0].device):
+            nbytes = L.sln_orthogonalize_workspace_bytes(descs, len(flat))
+            ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=mats[0].device)
+            _lib.check(L.sln_orthogonalize(descs, len(flat), _FLOATS[mats[0].dtype], int(steps), float(eps), _ptr(ws), nbytes,
+                                           _stream()), "sln_orthogonalize")
+    return type(x)(outs) if many else outs[0]

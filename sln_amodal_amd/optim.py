@@ -140,11 +140,36 @@ class ClippedSGD(object):
         dev = act[0][0].device
         if dev.type != "cuda":
             raise RuntimeError("ClippedSGD runs on the GPU only (no CPU fallback in sln_amodal_amd)")
+        ps, gs, bs = self._buffers(act)
+        ct, co, numel, partial, wd = self._chunks([p.numel() for p in ps], [w for _, w in act], dev)
+        tab = self._upload(ps, gs, bs, dev)
+        sq = torch.empty(1, dtype=torch.float64, device=dev)
+        if self.skipped is None:
+            self.skipped = torch.zeros(1, dtype=torch.int32, device=dev)
+        lr, momentum = self._hyper()
+        st = C.c_void_p(torch.cuda.current_stream().cuda_stream)
+        L = _lib.lib()
+        vp = lambda t: C.c_void_p(t.data_ptr())
+        nch = ct.numel() if sum(p.numel() for p in ps) else 0
+        _lib.check(L.sln_grad_sqnorm_f32(vp(tab[1]), vp(numel), vp(ct), vp(co), nch, CHUNK, vp(partial), vp(sq),
+                                         st), "sln_grad_sqnorm_f32")
+        sq_guard = self._guard(sq, veto)
+        _lib.check(L.sln_sgd_clip_step_f32(vp(tab[0]), vp(tab[1]), vp(tab[2]), vp(numel), vp(wd), vp(ct), vp(co),
+                                           nch, CHUNK, vp(sq_guard), float(max_norm), lr, momentum, vp(self.skipped),
+                                           st), "sln_sgd_clip_step_f32")
+        # caches keyed by the weights' version counters (split weight parts) must see the update
+        torch._C._autograd._unsafe_set_version_counter(ps, [p._version + 1 for p in ps])
+        self._keep = (tab, gs, sq_guard)      # alive until the next step: the launches above are asynchronous
+        self.last_norm = sq.sqrt().to(torch.float32)[0]
+        return self.last_norm
+
+    def _buffers(self, act):
+        """Parameters, gradients (element i of the gradient is element i of the weight) and momentum buffers."""
         ps, gs, bs = [], [], []
         for p, _ in act:
             g = p.grad
             if p.dtype != torch.float32 or g.dtype != torch.float32:
-                raise TypeError("ClippedSGD needs float32 parameters and gradients")
+                raise TypeError("%s needs float32 parameters and gradients" % type(self).__name__)
             if not (p.is_contiguous() or (p.dim() == 4 and p.is_contiguous(memory_format=torch.channels_last))):
                 raise ValueError("parameters must be dense")
             if g.stride() != p.stride():       # element i of the gradient must be element i of the weight
@@ -153,12 +178,14 @@ class ClippedSGD(object):
             if b is None:
                 b = self.state[p] = torch.zeros_like(p, memory_format=torch.preserve_format)
             ps.append(p); gs.append(g); bs.append(b)
+        return ps, gs, bs
+
+    def _upload(self, ps, gs, bs, dev):
+        """Pointer tables [3, n] (weights, gradients, momentum) on the device: gradients are fresh allocations every
+        step, so the tables are re-sent each time -- from pinned staging buffers and asynchronously, so the host never
+        waits for the GPU here (a pageable copy would drain the stream once per step).  A staging buffer is reused only
+        after the copy that read it has completed (4 in flight)."""
         n = len(ps)
-        ct, co, numel, partial, wd = self._chunks([p.numel() for p in ps], [w for _, w in act], dev)
-        # Pointer tables: gradients are fresh allocations every step, so the tables are re-sent each
-        # time -- from pinned staging buffers and asynchronously, so the host never waits for the GPU
-        # here (a pageable copy would drain the stream once per step).  A staging buffer is reused
-        # only after the copy that read it has completed (4 in flight).
         if not self._ring or self._ring[0][0].shape[1] != n:
             self._ring = [[torch.empty((3, n), dtype=torch.int64, pin_memory=True), None] for _ in range(4)]
         stage = self._ring[self._turn % len(self._ring)]
@@ -174,30 +201,130 @@ class ClippedSGD(object):
         if not self.capturing:
             stage[1] = torch.cuda.Event()
             stage[1].record()
-        sq = torch.empty(1, dtype=torch.float64, device=dev)
-        if self.skipped is None:
-            self.skipped = torch.zeros(1, dtype=torch.int32, device=dev)
+        return tab
+
+    def _guard(self, sq, veto):
+        """The guard's input: +inf instead of the squared norm when the step is vetoed (two 5-us elementwise ops)."""
+        if veto is None:
+            return sq
+        if self.skipped_clamped is None:
+            self.skipped_clamped = torch.zeros(1, dtype=torch.int32, device=sq.device)
+        hit = veto.reshape(1) > 0
+        # (a step that is non-finite anyway is counted as that, not as clamped)
+        self.skipped_clamped += (hit & torch.isfinite(sq)).to(torch.int32)
+        return torch.where(hit, torch.full_like(sq, float("inf")), sq)
+
+
+class _MuonDesc(C.Structure):
+    _fields_ = [("param", C.c_void_p), ("grad", C.c_void_p), ("momentum", C.c_void_p), ("rows", C.c_int32),
+                ("cols", C.c_int32), ("lr", C.c_float), ("decay", C.c_float)]
+
+
+class ClippedMuon(ClippedSGD):
+    """Clip + orthogonalised momentum for the weight matrices, ClippedSGD's rule for everything else, in one step over
+    all tensors (csrc/ortho.hip).  A group with "orthogonal": True holds parameters of two or more axes, each read as
+    the matrix [first axis][all the others] (in memory order: a permutation of the columns permutes the result's); with
+    g clipped by the global norm over ALL parameters,
+
+        b <- momentum b + g;  u = g + momentum b (nesterov) or b
+        p <- p (1 - lr weight_decay) - lr sqrt(max(1, rows / cols)) orthogonalize(u, steps, eps)
+
+    Orthogonal groups have an lr, momentum, weight_decay of their own (one momentum for all of them); the other groups
+    agree on one lr and momentum, like ClippedSGD's.  The same guard: a step with a non-finite gradient norm or a veto
+    writes nothing and is counted.  Hyper-parameters are read when step() is called; a captured step keeps them."""
+
+    def __init__(self, param_groups, lr, momentum=0.95, nesterov=True, steps=5, eps=1e-7):
+        super(ClippedMuon, self).__init__(param_groups, lr, momentum)
+        self.nesterov, self.steps, self.eps = bool(nesterov), int(steps), float(eps)
+        if not 1 <= self.steps <= 64 or not self.eps >= 1e-30:
+            raise ValueError("ClippedMuon: 1 <= steps <= 64 and eps >= 1e-30 (got %r, %r)" % (steps, eps))
+        seen = set()
+        for g in self.param_groups:
+            g["orthogonal"] = bool(g.get("orthogonal", False))
+            for p in g["params"]:
+                if id(p) in seen:
+                    raise ValueError("a parameter appears twice in the parameter groups")
+                seen.add(id(p))
+                if g["orthogonal"] and (p.dim() < 2 or min(p.shape[0], p[0].numel() if p.shape[0] else 0) > 65535):
+                    raise ValueError("an orthogonal group takes matrices (two or more axes, the shorter side at most "
+                                     "65535), got %s" % (tuple(p.shape),))
+
+    def _split(self):
+        rest = [g for g in self.param_groups if not g["orthogonal"]]
+        return rest, [g for g in self.param_groups if g["orthogonal"]]
+
+    def _hyper(self):
+        """lr / momentum of the groups that are not orthogonal (of the orthogonal ones where there are no others)."""
+        rest, ortho = self._split()
+        groups = [g for g in (rest if any(g["params"] for g in rest) else ortho) if g["params"]]
+        lrs, moms = {float(g["lr"]) for g in groups}, {float(g["momentum"]) for g in groups}
+        if rest and any(g["params"] for g in rest) and (len(lrs) > 1 or len(moms) > 1):
+            raise ValueError("ClippedMuon applies one lr / momentum to its non-orthogonal groups (got lr %s, "
+                             "momentum %s)" % (sorted(lrs), sorted(moms)))
+        return (min(lrs) if lrs else 0.0), (min(moms) if moms else 0.0)
+
+    def load_state_dict(self, sd):
+        if len(sd["param_groups"]) == len(self.param_groups):
+            for g, d in zip(self.param_groups, sd["param_groups"]):
+                if bool(d.get("orthogonal", g["orthogonal"])) != g["orthogonal"]:
+                    raise ValueError("loaded state dict marks other parameter groups as orthogonal")
+        super(ClippedMuon, self).load_state_dict(sd)
+
+    @torch.no_grad()
+    def step(self, max_norm, veto=None):
+        """See ClippedSGD.step: the same arguments, guard and counters."""
+        rest_groups, ortho_groups = self._split()
+        rest = [(p, float(g["weight_decay"])) for g in rest_groups for p in g["params"] if p.grad is not None]
+        mats = [(p, g) for g in ortho_groups for p in g["params"] if p.grad is not None]
+        act = rest + [(p, 0.0) for p, _ in mats]
+        if not act:
+            return None
+        dev = act[0][0].device
+        if dev.type != "cuda":
+            raise RuntimeError("ClippedMuon runs on the GPU only (no CPU fallback in sln_amodal_amd)")
+        if any(p.device != dev or p.grad.device != dev for p, _ in act):
+            raise ValueError("ClippedMuon: the parameters and gradients of one step share a device")
+        moms = {float(g["momentum"]) for _, g in mats}
+        if len(moms) > 1:
+            raise ValueError("ClippedMuon applies one momentum to its orthogonal groups (got %s)" % sorted(moms))
         lr, momentum = self._hyper()
-        st = C.c_void_p(torch.cuda.current_stream().cuda_stream)
-        L = _lib.lib()
-        vp = lambda t: C.c_void_p(t.data_ptr())
-        nch = ct.numel() if sum(p.numel() for p in ps) else 0
-        _lib.check(L.sln_grad_sqnorm_f32(vp(tab[1]), vp(numel), vp(ct), vp(co), nch, CHUNK, vp(partial), vp(sq),
-                                         st), "sln_grad_sqnorm_f32")
-        sq_guard = sq
-        if veto is not None:
-            # the guard's input: +inf instead of the squared norm when the step is vetoed (two 5-us elementwise ops)
-            if self.skipped_clamped is None:
-                self.skipped_clamped = torch.zeros(1, dtype=torch.int32, device=dev)
-            hit = veto.reshape(1) > 0
-            sq_guard = torch.where(hit, torch.full_like(sq, float("inf")), sq)
-            # (a step that is non-finite anyway is counted as that, not as clamped)
-            self.skipped_clamped += (hit & torch.isfinite(sq)).to(torch.int32)
-        _lib.check(L.sln_sgd_clip_step_f32(vp(tab[0]), vp(tab[1]), vp(tab[2]), vp(numel), vp(wd), vp(ct), vp(co),
-                                           nch, CHUNK, vp(sq_guard), float(max_norm), lr, momentum, vp(self.skipped),
-                                           st), "sln_sgd_clip_step_f32")
-        # caches keyed by the weights' version counters (split weight parts) must see the update
-        torch._C._autograd._unsafe_set_version_counter(ps, [p._version + 1 for p in ps])
-        self._keep = (tab, gs, sq_guard)      # alive until the next step: the launches above are asynchronous
-        self.last_norm = sq.sqrt().to(torch.float32)[0]
+        with torch.cuda.device(dev):
+            ps, gs, bs = self._buffers(act)
+            ct, co, numel, partial, wd = self._chunks([p.numel() for p in ps], [w for _, w in act], dev)
+            tab = self._upload(ps, gs, bs, dev)
+            sq = torch.empty(1, dtype=torch.float64, device=dev)
+            if self.skipped is None:
+                self.skipped = torch.zeros(1, dtype=torch.int32, device=dev)
+            st = C.c_void_p(torch.cuda.current_stream().cuda_stream)
+            L = _lib.lib()
+            vp = lambda t: C.c_void_p(t.data_ptr())
+            nch = ct.numel() if sum(p.numel() for p in ps) else 0
+            _lib.check(L.sln_grad_sqnorm_f32(vp(tab[1]), vp(numel), vp(ct), vp(co), nch, CHUNK, vp(partial), vp(sq), st),
+                       "sln_grad_sqnorm_f32")
+            guard = self._guard(sq, veto)
+            # the vectors come first in the tables: their chunks are a prefix of the chunk list.  (The SGD kernel also
+            # counts a skipped step; without vectors that is done here.)
+            nrest = sum(-(-p.numel() // CHUNK) for p, _ in rest)
+            if nrest:
+                _lib.check(L.sln_sgd_clip_step_f32(vp(tab[0]), vp(tab[1]), vp(tab[2]), vp(numel), vp(wd), vp(ct), vp(co),
+                                                   nrest, CHUNK, vp(guard), float(max_norm), lr, momentum,
+                                                   vp(self.skipped), st), "sln_sgd_clip_step_f32")
+            else:
+                self.skipped += (~torch.isfinite(guard)).to(torch.int32)
+            if mats:
+                k, flat = len(rest), []
+                for i, (p, g) in enumerate(mats):
+                    rows = p.shape[0]
+                    cols = p.numel() // rows if rows else 0
+                    glr = float(g["lr"])
+                    flat.append((p.data_ptr(), gs[k + i].data_ptr(), bs[k + i].data_ptr(), rows, cols,
+                                 glr * max(1.0, rows / cols) ** 0.5 if cols else 0.0, 1.0 - glr * float(g["weight_decay"])))
+                descs = (_MuonDesc * len(flat))(*flat)
+                nbytes = L.sln_muon_step_workspace_bytes(descs, len(flat))
+                ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=dev)
+                _lib.check(L.sln_muon_step_f32(descs, len(flat), self.steps, self.eps, vp(guard), float(max_norm),
+                                               moms.pop(), int(self.nesterov), vp(ws), nbytes, st), "sln_muon_step_f32")
+            torch._C._autograd._unsafe_set_version_counter(ps, [p._version + 1 for p in ps])
+            self._keep = (tab, gs, guard)
+            self.last_norm = sq.sqrt().to(torch.float32)[0]
         return self.last_norm
