@@ -593,6 +593,13 @@ int sln_mx4_product(const uint8_t *a_codes, const uint8_t *a_scales, const uint8
 int sln_mx4_rows_product(const void *x, int dtype, int64_t M, int64_t K, int64_t stride, const uint8_t *b_codes,
                          const uint8_t *b_scales, int64_t N, const float *scale, const float *bias, int relu, void *y,
                          void *workspace, size_t workspace_bytes, sln_stream_t stream);
+/* A layer's whole forward: w [N][K] (f32, row stride w_stride; NULL: w_codes / w_scales hold it already) and x are rounded
+ * into the given codes (kept by the caller for the backward), then multiplied.  x_codes NULL: up to 16 rows of x are
+ * rounded on the way.  Workspace: sln_mx4_product_workspace_bytes(M, N, K, x_codes != NULL). */
+int sln_mx4_linear_fwd(const void *x, int dtype, int64_t M, int64_t K, int64_t stride, uint8_t *x_codes,
+                       uint8_t *x_scales, const float *w, int64_t w_stride, uint8_t *w_codes, uint8_t *w_scales, int64_t N,
+                       const float *scale, const float *bias, int relu, void *y, void *workspace, size_t workspace_bytes,
+                       sln_stream_t stream);
 /* Straight-through gradients of y = act((x^ w^T) * scale + bias): gy [M][N] in dtype (row stride gy_stride), y [M][N] in
  * dtype: the output, gy counts where it is > 0 (NULL: everywhere); gx [M][K] in dtype, gw [N][K] f32, gb [N] f32, each
  * NULL if not wanted.  Workspace (256-byte boundary): sln_mx4_linear_bwd_workspace_bytes.  Bit-reproducible. */

@@ -93,6 +93,7 @@ SIGNATURES = {
     "sln_mx4_product_workspace_bytes": (C.c_size_t, [_l, _l, _l, _i]),
     "sln_mx4_product": (_i, [_p, _p, _p, _p, _l, _l, _l, _p, _p, _i, _p, _i, _p, C.c_size_t, _p]),
     "sln_mx4_rows_product": (_i, [_p, _i, _l, _l, _l, _p, _p, _l, _p, _p, _i, _p, _p, C.c_size_t, _p]),
+    "sln_mx4_linear_fwd": (_i, [_p, _i, _l, _l, _l, _p, _p, _p, _l, _p, _p, _l, _p, _p, _i, _p, _p, C.c_size_t, _p]),
     "sln_mx4_linear_bwd_workspace_bytes": (C.c_size_t, [_l, _l, _l, _i, _i, _i, _i]),
     "sln_mx4_linear_bwd": (_i, [_p, _i, _l, _p, _p, _p, _p, _p, _p, _l, _l, _l, _p, _p, _p, _p, C.c_size_t, _p]),
     "sln_orthogonalize_workspace_bytes": (C.c_size_t, [_p, _i]),

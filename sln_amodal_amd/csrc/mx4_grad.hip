@@ -44,31 +44,42 @@ __device__ __forceinline__ void mg_store8(char *base, int64_t row, int64_t row_b
 }
 __host__ __device__ __forceinline__ int64_t mg_row_bytes(int64_t k, int parts) { return (k + 31) / 32 * 64 * parts; }
 
-// Block = 64 x 64 of gy: parts of z * scale (rows M) and of z^T (rows N), one partial bias sum per column.
+// What has to be laid out, in one launch: blocks [0, split) cut 64 x 64 tiles of gy, [split, split + turn_w) turn tiles
+// of the weight's codes, the rest tiles of x's.
+struct MgPrep {
+    const void *gy, *y;
+    const float *scale;
+    int64_t stride;
+    int M, N, K;
+    char *rows, *cols;                   // parts of z * scale (rows M) and of z^T (rows N), or NULL
+    float *bias_part;                    // one sum per 64 rows and column, or NULL
+    const unsigned *w_codes, *x_codes;
+    const uint8_t *w_scales, *x_scales;
+    char *wt, *xt;                       // [K][N], [K][M]
+    unsigned split, turn_w;
+};
+
 template <typename T, int P>
-__global__ __launch_bounds__(256) void mx4_grad_split_kernel(const T *__restrict__ gy, int64_t stride,
-                                                             const T *__restrict__ y, const float *__restrict__ scale,
-                                                             int M, int N, char *__restrict__ rows,
-                                                             char *__restrict__ cols, float *__restrict__ bias_part) {
-    __shared__ float z[64 * MG_PITCH];
-    __shared__ float s_bias[4][64];
-    const int t = threadIdx.x, m0 = blockIdx.y * 64, n0 = blockIdx.x * 64;
+__device__ __forceinline__ void mg_split(const MgPrep &p, unsigned b, float *z, float (*s_bias)[64]) {
+    const unsigned tn = (unsigned)(p.N + 63) / 64;
+    const int t = threadIdx.x, m0 = (int)(b / tn) * 64, n0 = (int)(b % tn) * 64;
+    const int M = p.M, N = p.N;
     float sum = 0.f;
     for (int i = t >> 6; i < 64; i += 4) {
         const int m = m0 + i, n = n0 + (t & 63);
         float v = 0.f;
         if (m < M && n < N) {
-            v = (float)gy[(int64_t)m * stride + n];
-            if (y && !((float)y[(int64_t)m * N + n] > 0.f)) v = 0.f;
+            v = (float)((const T *)p.gy)[(int64_t)m * p.stride + n];
+            if (p.y && !((float)((const T *)p.y)[(int64_t)m * N + n] > 0.f)) v = 0.f;
         }
         z[i * MG_PITCH + (t & 63)] = v;
         sum += v;
     }
     s_bias[t >> 6][t & 63] = sum;
     __syncthreads();
-    if (bias_part && t < 64 && n0 + t < N)
-        bias_part[(int64_t)blockIdx.y * N + n0 + t] = (s_bias[0][t] + s_bias[1][t]) + (s_bias[2][t] + s_bias[3][t]);
-    if (rows) {
+    if (p.bias_part && t < 64 && n0 + t < N)
+        p.bias_part[(int64_t)(m0 / 64) * N + n0 + t] = (s_bias[0][t] + s_bias[1][t]) + (s_bias[2][t] + s_bias[3][t]);
+    if (p.rows) {
         const int64_t rb = mg_row_bytes(N, P);
         const int npad = (N + 31) & ~31;
         for (int e = t; e < 512; e += 256) {
@@ -78,12 +89,12 @@ __global__ __launch_bounds__(256) void mx4_grad_split_kernel(const T *__restrict
 #pragma unroll
             for (int q = 0; q < 8; ++q) {
                 v[q] = z[i * MG_PITCH + k + q];
-                if (scale && n0 + k + q < N) v[q] *= scale[n0 + k + q];
+                if (p.scale && n0 + k + q < N) v[q] *= p.scale[n0 + k + q];
             }
-            mg_store8<P>(rows, m0 + i, rb, n0 + k, v);
+            mg_store8<P>(p.rows, m0 + i, rb, n0 + k, v);
         }
     }
-    if (cols) {
+    if (p.cols) {
         const int64_t rb = mg_row_bytes(M, P);
         const int mpad = (M + 31) & ~31;
         for (int e = t; e < 512; e += 256) {
@@ -92,31 +103,21 @@ __global__ __launch_bounds__(256) void mx4_grad_split_kernel(const T *__restrict
             float v[8];
 #pragma unroll
             for (int q = 0; q < 8; ++q) v[q] = z[(k + q) * MG_PITCH + j];
-            mg_store8<P>(cols, n0 + j, rb, m0 + k, v);
+            mg_store8<P>(p.cols, n0 + j, rb, m0 + k, v);
         }
     }
 }
 
-// Partial bias sums, added in order in double.
-__global__ __launch_bounds__(64) void mx4_grad_bias_kernel(const float *__restrict__ part, int blocks, int N,
-                                                           float *__restrict__ gb) {
-    const int n = blockIdx.x * 64 + threadIdx.x;
-    if (n >= N) return;
-    double s = 0.0;
-    for (int b = 0; b < blocks; ++b) s += part[(int64_t)b * N + n];
-    gb[n] = (float)s;
-}
-
-// Codes [R][K] -> bf16 values as parts rows [K][R].  Block = 64 x 64.
-__global__ __launch_bounds__(256) void mx4_grad_turn_kernel(const unsigned *__restrict__ codes,
-                                                            const uint8_t *__restrict__ scales, int R, int K, int64_t kp,
-                                                            char *__restrict__ out) {
-    __shared__ float z[64 * MG_PITCH];
-    const int t = threadIdx.x, r0 = blockIdx.y * 64, k0 = blockIdx.x * 64;
+// Codes [R][K] -> bf16 values as parts rows [K][R].  A block turns 64 x 64.
+__device__ __forceinline__ void mg_turn(const unsigned *codes, const uint8_t *scales, int R, int K, char *out, unsigned b,
+                                        float *z) {
+    const unsigned tk = (unsigned)(K + 63) / 64;
+    const int t = threadIdx.x, r0 = (int)(b / tk) * 64, k0 = (int)(b % tk) * 64;
+    const int64_t kp = (int64_t)(K + MX_STEP - 1) / MX_STEP * MX_STEP;
     for (int e = t; e < 512; e += 256) {
         const int i = e >> 3, k = k0 + (e & 7) * 8;
         float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (r0 + i < R && k < kp) {
+        if (r0 + i < R) {                      // (k < kp: the padded row holds whole tiles of 64)
             const int64_t at = (int64_t)(r0 + i) * (kp / 8) + k / 8;
             mx_values8(codes[at], scales[at >> 2], v);
         }
@@ -136,12 +137,22 @@ __global__ __launch_bounds__(256) void mx4_grad_turn_kernel(const unsigned *__re
     }
 }
 
+template <typename T, int P>
+__global__ __launch_bounds__(256) void mx4_grad_prep_kernel(const MgPrep p) {
+    __shared__ float z[64 * MG_PITCH];
+    __shared__ float s_bias[4][64];
+    if (blockIdx.x < p.split) mg_split<T, P>(p, blockIdx.x, z, s_bias);
+    else if (blockIdx.x < p.split + p.turn_w) mg_turn(p.w_codes, p.w_scales, p.N, p.K, p.wt, blockIdx.x - p.split, z);
+    else mg_turn(p.x_codes, p.x_scales, p.M, p.K, p.xt, blockIdx.x - p.split - p.turn_w, z);
+}
+
 struct MgProduct {
     const char *a, *b;            // parts rows: a [RA] of P parts, b [RB] of one
     int RA, RB, groups, nsplit;
+    unsigned tiles;               // of the launch, cuts included
     const float *row_scale;       // per row of the result, or NULL
     void *c;                      // [RA][RB]
-    float *slab;
+    float *slab;                  // nsplit > 1: [nsplit][RA][RB]
 };
 
 template <typename T>
@@ -150,9 +161,7 @@ __device__ __forceinline__ void mg_finish(const MgProduct &p, int i, int64_t at,
 }
 
 template <typename T, int P>
-__global__ __launch_bounds__(256, 2) void mx4_grad_product_kernel(const MgProduct p, int tiles) {
-    __shared__ __attribute__((aligned(128))) char smem[2 * NtShape<P, 1>::STAGE];
-    const int at = nt_xcd_order(blockIdx.x, tiles);
+__device__ __forceinline__ void mg_product(const MgProduct &p, int at, char *smem) {
     const int ta = (p.RA + NT_TILE - 1) / NT_TILE;
     const int split = at % p.nsplit, tile = at / p.nsplit;
     const int i0 = tile % ta * NT_TILE, j0 = tile / ta * NT_TILE;
@@ -178,19 +187,43 @@ __global__ __launch_bounds__(256, 2) void mx4_grad_product_kernel(const MgProduc
         }
 }
 
+// Both products and the bias sums in one launch (x: gx, w: gw; tiles = 0: not wanted).
+template <typename T, int P>
+__global__ __launch_bounds__(256, 2) void mx4_grad_product_kernel(const MgProduct x, const MgProduct w,
+                                                                  const float *__restrict__ bias_part, int bias_blocks,
+                                                                  int N, float *__restrict__ gb) {
+    __shared__ __attribute__((aligned(128))) char smem[2 * NtShape<P, 1>::STAGE];
+    if (blockIdx.x < x.tiles) {
+        mg_product<T, P>(x, nt_xcd_order(blockIdx.x, x.tiles), smem);
+    } else if (blockIdx.x < x.tiles + w.tiles) {
+        mg_product<float, P>(w, nt_xcd_order(blockIdx.x - x.tiles, w.tiles), smem);
+    } else {                                       // partial bias sums, added in order in double
+        const int n = (blockIdx.x - x.tiles - w.tiles) * 256 + threadIdx.x;
+        if (n >= N) return;
+        double s = 0.0;
+        for (int b = 0; b < bias_blocks; ++b) s += bias_part[(int64_t)b * N + n];
+        gb[n] = (float)s;
+    }
+}
+
 template <typename T>
-__global__ __launch_bounds__(256) void mx4_grad_join_kernel(const MgProduct p) {
+__device__ __forceinline__ void mg_join(const MgProduct &p, int64_t first, int64_t step) {
     const int64_t total = (int64_t)p.RA * p.RB;
-    for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < total; e += (int64_t)gridDim.x * 256) {
+    for (int64_t e = first; e < total; e += step) {
         float v = 0.f;
         for (int k = 0; k < p.nsplit; ++k) v += p.slab[k * total + e];
         mg_finish<T>(p, (int)(e / p.RB), e, v);
     }
 }
+template <typename T>
+__global__ __launch_bounds__(256) void mx4_grad_join_kernel(const MgProduct x, const MgProduct w, unsigned blocks_x) {
+    if (blockIdx.x < blocks_x) mg_join<T>(x, (int64_t)blockIdx.x * 256 + threadIdx.x, (int64_t)blocks_x * 256);
+    else mg_join<float>(w, (int64_t)(blockIdx.x - blocks_x) * 256 + threadIdx.x, (int64_t)(gridDim.x - blocks_x) * 256);
+}
 
 // ------------------------------------------------------------------------------------------------ host side
 struct MgPlan {
-    int64_t z_rows, z_cols, wt, xt, bias, slab, bytes;
+    int64_t z_rows, z_cols, wt, xt, bias, slab_x, slab_w, bytes;
     int gx_cuts, gw_cuts;
 };
 static inline int64_t mg_align(int64_t v) { return (v + 255) & ~(int64_t)255; }
@@ -210,10 +243,8 @@ static void mg_plan(int64_t M, int64_t N, int64_t K, int parts, bool gx, bool gw
     p.wt = at; at += gx ? mg_align(K * mg_row_bytes(N, 1)) : 0;
     p.xt = at; at += gw ? mg_align(K * mg_row_bytes(M, 1)) : 0;
     p.bias = at; at += gb ? mg_align((M + 63) / 64 * N * 4) : 0;
-    int64_t slab = 0;
-    if (gx && p.gx_cuts > 1) slab = p.gx_cuts * M * K * 4;
-    if (gw && p.gw_cuts > 1 && p.gw_cuts * N * K * 4 > slab) slab = p.gw_cuts * N * K * 4;
-    p.slab = at; at += mg_align(slab);
+    p.slab_x = at; at += gx && p.gx_cuts > 1 ? mg_align(p.gx_cuts * M * K * 4) : 0;
+    p.slab_w = at; at += gw && p.gw_cuts > 1 ? mg_align(p.gw_cuts * N * K * 4) : 0;
     p.bytes = at;
 }
 static inline int mg_parts(int dtype) { return dtype == SLN_DTYPE_F32 ? 3 : 2; }
@@ -226,42 +257,45 @@ extern "C" size_t sln_mx4_linear_bwd_workspace_bytes(int64_t M, int64_t N, int64
     return (size_t)p.bytes;
 }
 
-template <typename T, int P>
-static void mg_product(const char *a, int64_t RA, const char *b, int64_t RB, int64_t k, int cuts, const float *row_scale,
-                       void *c, float *slab, hipStream_t st) {
-    const MgProduct p = {a, b, (int)RA, (int)RB, (int)((k + 31) / 32), cuts, row_scale, c, slab};
-    const int64_t tiles = ((RA + NT_TILE - 1) / NT_TILE) * ((RB + NT_TILE - 1) / NT_TILE) * cuts;
-    hipLaunchKernelGGL((mx4_grad_product_kernel<T, P>), dim3((unsigned)tiles), dim3(256), 0, st, p, (int)tiles);
-    if (cuts > 1) {
-        const int64_t blocks = (RA * RB + 255) / 256;
-        hipLaunchKernelGGL((mx4_grad_join_kernel<T>), dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, p);
-    }
+static MgProduct mg_job(const char *a, int64_t RA, const char *b, int64_t RB, int64_t k, int cuts, const float *row_scale,
+                        void *c, char *slab) {
+    MgProduct p = {};
+    if (!c) return p;
+    p.a = a; p.b = b; p.RA = (int)RA; p.RB = (int)RB;
+    p.groups = (int)((k + 31) / 32); p.nsplit = cuts;
+    p.tiles = (unsigned)(((RA + NT_TILE - 1) / NT_TILE) * ((RB + NT_TILE - 1) / NT_TILE) * cuts);
+    p.row_scale = row_scale; p.c = c; p.slab = (float *)slab;
+    return p;
+}
+static inline unsigned mg_join_blocks(const MgProduct &p) {
+    if (p.tiles == 0 || p.nsplit == 1) return 0;
+    const int64_t blocks = ((int64_t)p.RA * p.RB + 255) / 256;
+    return (unsigned)(blocks < 4096 ? blocks : 4096);
 }
 
 template <typename T, int P>
 static void mg_run(const void *gy, int64_t stride, const void *y, const float *scale, const uint8_t *xc, const uint8_t *xs,
                    const uint8_t *wc, const uint8_t *wsc, int64_t M, int64_t N, int64_t K, void *gx, float *gw, float *gb,
-                   char *ws, hipStream_t st) {
-    MgPlan pl;
-    mg_plan(M, N, K, P, gx, gw, gb, pl);
-    const int64_t kp = sln_mx4_row_values(K);
-    const dim3 gn((unsigned)((N + 63) / 64), (unsigned)((M + 63) / 64));
-    hipLaunchKernelGGL((mx4_grad_split_kernel<T, P>), gn, dim3(256), 0, st, (const T *)gy, stride, (const T *)y, scale,
-                       (int)M, (int)N, gx ? ws + pl.z_rows : nullptr, gw ? ws + pl.z_cols : nullptr,
-                       gb ? (float *)(ws + pl.bias) : nullptr);
-    if (gb)
-        hipLaunchKernelGGL(mx4_grad_bias_kernel, dim3((unsigned)((N + 63) / 64)), dim3(64), 0, st,
-                           (const float *)(ws + pl.bias), (int)((M + 63) / 64), (int)N, gb);
-    if (gx) {
-        hipLaunchKernelGGL(mx4_grad_turn_kernel, dim3((unsigned)((K + 63) / 64), (unsigned)((N + 63) / 64)), dim3(256), 0,
-                           st, (const unsigned *)wc, wsc, (int)N, (int)K, kp, ws + pl.wt);
-        mg_product<T, P>(ws + pl.z_rows, M, ws + pl.wt, K, N, pl.gx_cuts, nullptr, gx, (float *)(ws + pl.slab), st);
-    }
-    if (gw) {
-        hipLaunchKernelGGL(mx4_grad_turn_kernel, dim3((unsigned)((K + 63) / 64), (unsigned)((M + 63) / 64)), dim3(256), 0,
-                           st, (const unsigned *)xc, xs, (int)M, (int)K, kp, ws + pl.xt);
-        mg_product<float, P>(ws + pl.z_cols, N, ws + pl.xt, K, M, pl.gw_cuts, scale, gw, (float *)(ws + pl.slab), st);
-    }
+                   const MgPlan &pl, char *ws, hipStream_t st) {
+    MgPrep p = {};
+    p.gy = gy; p.y = y; p.scale = scale; p.stride = stride;
+    p.M = (int)M; p.N = (int)N; p.K = (int)K;
+    p.rows = gx ? ws + pl.z_rows : nullptr;
+    p.cols = gw ? ws + pl.z_cols : nullptr;
+    p.bias_part = gb ? (float *)(ws + pl.bias) : nullptr;
+    p.w_codes = (const unsigned *)wc; p.w_scales = wsc; p.wt = ws + pl.wt;
+    p.x_codes = (const unsigned *)xc; p.x_scales = xs; p.xt = ws + pl.xt;
+    const int64_t tm = (M + 63) / 64, tn = (N + 63) / 64, tk = (K + 63) / 64;
+    p.split = (unsigned)(tm * tn);
+    p.turn_w = gx ? (unsigned)(tk * tn) : 0u;
+    hipLaunchKernelGGL((mx4_grad_prep_kernel<T, P>), dim3(p.split + p.turn_w + (gw ? (unsigned)(tk * tm) : 0u)), dim3(256),
+                       0, st, p);
+    const MgProduct jx = mg_job(ws + pl.z_rows, M, ws + pl.wt, K, N, pl.gx_cuts, nullptr, gx, ws + pl.slab_x);
+    const MgProduct jw = mg_job(ws + pl.z_cols, N, ws + pl.xt, K, M, pl.gw_cuts, scale, gw, ws + pl.slab_w);
+    hipLaunchKernelGGL((mx4_grad_product_kernel<T, P>), dim3(jx.tiles + jw.tiles + (gb ? (unsigned)((N + 255) / 256) : 0u)),
+                       dim3(256), 0, st, jx, jw, p.bias_part, (int)tm, (int)N, gb);
+    const unsigned bx = mg_join_blocks(jx), bw = mg_join_blocks(jw);
+    if (bx + bw) hipLaunchKernelGGL((mx4_grad_join_kernel<T>), dim3(bx + bw), dim3(256), 0, st, jx, jw, bx);
 }
 
 extern "C" int sln_mx4_linear_bwd(const void *gy, int dtype, int64_t gy_stride, const void *y, const float *scale,
@@ -271,7 +305,10 @@ extern "C" int sln_mx4_linear_bwd(const void *gy, int dtype, int64_t gy_stride, 
     if ((dtype != SLN_DTYPE_F32 && dtype != SLN_DTYPE_BF16 && dtype != SLN_DTYPE_F16) || M < 1 || N < 1 || K < 1 ||
         gy_stride < N || !gy)
         return SLN_ERR_INVALID_ARG;
-    if (M > (1 << 21) || N > (1 << 21) || K > MX_MAX_K) return SLN_ERR_UNSUPPORTED;   // grid.y, 128 rows below 2^32 B
+    // 128 rows below 2^32 B, and every launch below 2^31 blocks
+    if (M > (1 << 21) || N > (1 << 21) || K > MX_MAX_K || (M + 63) / 64 * ((N + 63) / 64) > (1 << 28) ||
+        (K + 63) / 64 * ((M + 63) / 64) > (1 << 28) || (K + 63) / 64 * ((N + 63) / 64) > (1 << 28))
+        return SLN_ERR_UNSUPPORTED;
     if ((gx && (!w_codes || !w_scales)) || (gw && (!x_codes || !x_scales))) return SLN_ERR_INVALID_ARG;
     MgPlan pl;
     mg_plan(M, N, K, mg_parts(dtype), gx, gw, gb, pl);
@@ -282,10 +319,10 @@ extern "C" int sln_mx4_linear_bwd(const void *gy, int dtype, int64_t gy_stride, 
     char *ws = (char *)workspace;
     hipStream_t st = (hipStream_t)stream;
     if (dtype == SLN_DTYPE_F32)
-        mg_run<float, 3>(gy, gy_stride, y, scale, x_codes, x_scales, w_codes, w_scales, M, N, K, gx, gw, gb, ws, st);
+        mg_run<float, 3>(gy, gy_stride, y, scale, x_codes, x_scales, w_codes, w_scales, M, N, K, gx, gw, gb, pl, ws, st);
     else if (dtype == SLN_DTYPE_BF16)
-        mg_run<__bf16, 2>(gy, gy_stride, y, scale, x_codes, x_scales, w_codes, w_scales, M, N, K, gx, gw, gb, ws, st);
+        mg_run<__bf16, 2>(gy, gy_stride, y, scale, x_codes, x_scales, w_codes, w_scales, M, N, K, gx, gw, gb, pl, ws, st);
     else
-        mg_run<_Float16, 2>(gy, gy_stride, y, scale, x_codes, x_scales, w_codes, w_scales, M, N, K, gx, gw, gb, ws, st);
+        mg_run<_Float16, 2>(gy, gy_stride, y, scale, x_codes, x_scales, w_codes, w_scales, M, N, K, gx, gw, gb, pl, ws, st);
     return sln_launch_status();
 }

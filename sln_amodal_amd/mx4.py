@@ -4,8 +4,6 @@
 their negatives): 4.25 bits per value.  `mx4_quantize` rounds a matrix, `mx4_linear` multiplies rounded rows with a rounded
 weight -- forward on the scaled 4-bit matrix instructions, backward straight through the rounding with the products in
 float32 accuracy.  `ops` re-exports both; `MaskRCNN.set_mx4_layers` runs the classifier head's layers this way."""
-import ctypes as C
-
 import torch
 from torch.autograd.function import once_differentiable
 
@@ -16,12 +14,24 @@ FEW_ROWS = 16          # rows that sln_mx4_rows_product takes: rounded inside th
 MAX_K = 1 << 22
 
 
-def _ptr(t):
-    return C.c_void_p(t.data_ptr()) if t is not None else C.c_void_p(0)
+def _stream(dev):
+    return torch._C._cuda_getCurrentRawStream(dev.index)
 
 
-def _stream(t):
-    return C.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+class _On(object):
+    """Launches go to the tensors' device; nothing is switched where that is the current one already."""
+    __slots__ = ("guard",)
+
+    def __init__(self, dev):
+        self.guard = None if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
 
 
 def _need_float(t, name):
@@ -35,46 +45,72 @@ def _need_float(t, name):
 
 
 def _rows(t, name):
-    """t [..., K] -> [R, K] whose rows lie anywhere with values side by side (a copy only where they do not)."""
-    if t.dim() < 1 or not 1 <= t.shape[-1] <= MAX_K:
-        raise ValueError("%s must be [..., K] with 1 <= K <= 2^22, got %s" % (name, tuple(t.shape)))
-    t = t.detach()
-    t = t.reshape(-1, t.shape[-1]) if t.dim() != 2 else t
-    if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
-        t = t.contiguous()
-    return t
-
-
-def _pitch(t):
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    """t [..., K] -> (a [R, K] whose rows lie anywhere with values side by side -- a copy only where they do not --, R, K,
+    row stride)."""
+    shape = t.shape
+    if len(shape) < 1 or not 1 <= shape[-1] <= MAX_K:
+        raise ValueError("%s must be [..., K] with 1 <= K <= 2^22, got %s" % (name, tuple(shape)))
+    if len(shape) != 2:
+        t = t.detach().reshape(-1, shape[-1])
+        shape = t.shape
+    R, K = shape
+    s0, s1 = t.stride()
+    if (K > 1 and s1 != 1) or (R > 1 and s0 < K):
+        t = t.detach().contiguous()
+        s0 = K
+    return t, R, K, (s0 if R > 1 else K)
 
 
 class Mx4Tensor(object):
-    """A matrix held in 4 bits: codes uint8 [R, Kp / 2] (Kp = K rounded up to 256), scales uint8 [R, Kp / 32], the
-    `shape` and `dtype` of what it was made from.  Its rows are the last axis' vectors."""
-    __slots__ = ("codes", "scales", "shape", "dtype")
+    """A matrix held in 4 bits: `codes` uint8 [R, Kp / 2] (Kp = K rounded up to 256) and `scales` uint8 [R, Kp / 32], both
+    views of one buffer; the `shape` and `dtype` of what it was made from.  Its rows are the last axis' vectors."""
+    __slots__ = ("data", "rows", "shape", "dtype")
 
-    def __init__(self, codes, scales, shape, dtype):
-        self.codes, self.scales, self.shape, self.dtype = codes, scales, torch.Size(shape), dtype
+    def __init__(self, data, rows, shape, dtype):
+        self.data, self.rows, self.shape, self.dtype = data, rows, torch.Size(shape), dtype
 
     @property
     def device(self):
-        return self.codes.device
+        return self.data.device
+
+    @property
+    def codes(self):
+        kp = _padded(self.shape[-1])
+        return self.data[:self.rows * (kp // 2)].view(self.rows, kp // 2)
+
+    @property
+    def scales(self):
+        kp = _padded(self.shape[-1])
+        return self.data[self.rows * (kp // 2):].view(self.rows, kp // 32)
 
     def dequantize(self, dtype=None):
         """The values that the codes stand for, in `dtype` (default: the source's; exact in float32 and bfloat16)."""
         dtype = self.dtype if dtype is None else dtype
         if dtype not in _DTYPES:
             raise TypeError("dtype must be float32, bfloat16 or float16, got %s" % dtype)
-        out = torch.empty(self.shape, dtype=dtype, device=self.device)
-        with torch.cuda.device(self.device):
-            _lib.check(_lib.lib().sln_mx4_values(_ptr(self.codes), _ptr(self.scales), self.codes.shape[0],
-                                                 self.shape[-1], _ptr(out), _DTYPES[dtype], _stream(out)),
-                       "sln_mx4_values")
+        dev = self.data.device
+        out = torch.empty(self.shape, dtype=dtype, device=dev)
+        codes, scales = _pointers(self.data, self.rows, self.shape[-1])
+        with _On(dev):
+            _lib.check(_lib.lib().sln_mx4_values(codes, scales, self.rows, self.shape[-1], out.data_ptr(),
+                                                 _DTYPES[dtype], _stream(dev)), "sln_mx4_values")
         return out
 
     def __repr__(self):
         return "Mx4Tensor(%s, %s, %s)" % (tuple(self.shape), self.dtype, self.device)
+
+
+def _padded(K):
+    return -(-K // 256) * 256
+
+
+def _buffer(R, K, dev):
+    return torch.empty(R * (_padded(K) // 32) * 17, dtype=torch.uint8, device=dev)
+
+
+def _pointers(data, R, K):
+    p = data.data_ptr()
+    return p, p + R * (_padded(K) // 2)
 
 
 def mx4_quantize(x):
@@ -82,38 +118,41 @@ def mx4_quantize(x):
     times the block's scale 2^(floor(log2 max|x|) - 2); a block with an infinity or a NaN becomes all NaN.  Rows may be
     strided.  No gradient (mx4_linear has one)."""
     _need_float(x, "x")
-    rows = _rows(x, "x")
-    R, K = rows.shape
-    kp = -(-K // 256) * 256
-    codes = torch.empty((R, kp // 2), dtype=torch.uint8, device=x.device)
-    scales = torch.empty((R, kp // 32), dtype=torch.uint8, device=x.device)
-    with torch.cuda.device(x.device):
-        _lib.check(_lib.lib().sln_mx4_round(_ptr(rows), _DTYPES[x.dtype], R, K, _pitch(rows), _ptr(codes), _ptr(scales),
-                                            _stream(x)), "sln_mx4_round")
-    return Mx4Tensor(codes, scales, x.shape, x.dtype)
+    src, R, K, pitch = _rows(x, "x")
+    dev = x.device
+    data = _buffer(R, K, dev)
+    codes, scales = _pointers(data, R, K)
+    with _On(dev):
+        _lib.check(_lib.lib().sln_mx4_round(src.data_ptr(), _DTYPES[x.dtype], R, K, pitch, codes, scales, _stream(dev)),
+                   "sln_mx4_round")
+    return Mx4Tensor(data, R, x.shape, x.dtype)
 
 
-def _forward(rows, xq, wq, scale, bias, relu, dtype):
-    """rows [M,K] (few rows, not rounded) or xq (their codes) times wq -> [M, N]."""
-    M, K = rows.shape
-    N = wq.codes.shape[0]
-    dev = wq.device
-    y = torch.empty((M, N), dtype=dtype, device=dev)
-    if M == 0 or N == 0:
-        return y
+def _forward(x, weight, wq, bias, scale, relu, keep):
+    """-> y [M, N] and, where the backward needs them (`keep`) or the rows are many, the codes of x; the weight's codes."""
+    src, M, K, pitch = _rows(x, "x")
+    dev = x.device
     L = _lib.lib()
-    nbytes = L.sln_mx4_product_workspace_bytes(M, N, K, 0 if xq is None else 1)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    with torch.cuda.device(dev):
-        if xq is None:
-            _lib.check(L.sln_mx4_rows_product(_ptr(rows), _DTYPES[dtype], M, K, _pitch(rows), _ptr(wq.codes),
-                                              _ptr(wq.scales), N, _ptr(scale), _ptr(bias), int(relu), _ptr(y), _ptr(ws),
-                                              nbytes, _stream(y)), "sln_mx4_rows_product")
-        else:
-            _lib.check(L.sln_mx4_product(_ptr(xq.codes), _ptr(xq.scales), _ptr(wq.codes), _ptr(wq.scales), M, N, K,
-                                         _ptr(scale), _ptr(bias), int(relu), _ptr(y), _DTYPES[dtype], _ptr(ws), nbytes,
-                                         _stream(y)), "sln_mx4_product")
-    return y
+    w = w_pitch = 0
+    if wq is None:
+        wsrc, N, _, w_pitch = _rows(weight, "weight")
+        w, wdata = wsrc.data_ptr(), _buffer(N, K, dev)
+    else:
+        wdata, N = wq.data, wq.rows
+    y = torch.empty((M, N), dtype=x.dtype, device=dev)
+    xdata = _buffer(M, K, dev) if keep or M > FEW_ROWS else None
+    if M == 0 or N == 0:
+        return y, M, K, N, xdata, wdata
+    xc, xs = _pointers(xdata, M, K) if xdata is not None else (0, 0)
+    wc, ws = _pointers(wdata, N, K)
+    nbytes = L.sln_mx4_product_workspace_bytes(M, N, K, xdata is not None)
+    work = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    with _On(dev):
+        _lib.check(L.sln_mx4_linear_fwd(src.data_ptr(), _DTYPES[x.dtype], M, K, pitch, xc, xs, w, w_pitch, wc, ws, N,
+                                        scale.data_ptr() if scale is not None else 0,
+                                        bias.data_ptr() if bias is not None else 0, relu, y.data_ptr(),
+                                        work.data_ptr() if nbytes else 0, nbytes, _stream(dev)), "sln_mx4_linear_fwd")
+    return y, M, K, N, xdata, wdata
 
 
 class _Mx4LinearFn(torch.autograd.Function):
@@ -121,25 +160,20 @@ class _Mx4LinearFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, scale, relu, wq):
-        rows = _rows(x, "x")
-        if wq is None:
-            wq = mx4_quantize(weight)
         need_w = weight is not None and ctx.needs_input_grad[1]
-        xq = mx4_quantize(rows) if need_w or rows.shape[0] > FEW_ROWS else None
-        y = _forward(rows, xq, wq, scale, bias, relu, x.dtype)
-        ctx.cfg = (tuple(x.shape), tuple(rows.shape), wq.codes.shape[0], x.dtype)
-        ctx.save_for_backward(xq.codes if need_w else None, xq.scales if need_w else None, wq.codes, wq.scales, scale,
-                              y if relu else None)
-        return y if x.dim() == 2 else y.view(x.shape[:-1] + (y.shape[1],))
+        y, M, K, N, xdata, wdata = _forward(x, weight, wq, bias, scale, relu, need_w)
+        ctx.cfg = (x.shape, M, K, N, x.dtype)
+        ctx.save_for_backward(xdata if need_w else None, wdata, scale, y if relu else None)
+        return y if x.dim() == 2 else y.view(x.shape[:-1] + (N,))
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gy):
-        xc, xs, wc, wsc, scale, y = ctx.saved_tensors
-        shape, (M, K), N, dtype = ctx.cfg
-        dev = wc.device
+        xdata, wdata, scale, y = ctx.saved_tensors
+        shape, M, K, N, dtype = ctx.cfg
+        dev = wdata.device
         want_x, want_w, want_b = ctx.needs_input_grad[:3]
-        gx = torch.empty((M, K), dtype=dtype, device=dev) if want_x else None
+        gx = torch.empty(shape, dtype=dtype, device=dev) if want_x else None
         gw = torch.empty((N, K), dtype=torch.float32, device=dev) if want_w else None
         gb = torch.empty((N,), dtype=torch.float32, device=dev) if want_b else None
         if M == 0 or N == 0:
@@ -147,17 +181,20 @@ class _Mx4LinearFn(torch.autograd.Function):
                 if t is not None:
                     t.zero_()
         elif want_x or want_w or want_b:
-            g = gy.reshape(M, N)
-            if (N > 1 and g.stride(1) != 1) or (M > 1 and g.stride(0) < N):
-                g = g.contiguous()
+            g = gy if gy.dim() == 2 else gy.reshape(M, N)
+            g, _, _, pitch = _rows(g, "gradient")
             L = _lib.lib()
-            nbytes = L.sln_mx4_linear_bwd_workspace_bytes(M, N, K, _DTYPES[dtype], want_x, want_w, want_b)
-            ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=dev)
-            with torch.cuda.device(dev):
-                _lib.check(L.sln_mx4_linear_bwd(_ptr(g), _DTYPES[dtype], _pitch(g), _ptr(y), _ptr(scale), _ptr(xc),
-                                                _ptr(xs), _ptr(wc), _ptr(wsc), M, N, K, _ptr(gx), _ptr(gw), _ptr(gb),
-                                                _ptr(ws), nbytes, _stream(g)), "sln_mx4_linear_bwd")
-        return gx.view(shape) if want_x else None, gw, gb, None, None, None
+            kind = _DTYPES[dtype]
+            nbytes = L.sln_mx4_linear_bwd_workspace_bytes(M, N, K, kind, want_x, want_w, want_b)
+            work = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            xc, xs = _pointers(xdata, M, K) if want_w else (0, 0)
+            wc, ws = _pointers(wdata, N, K)
+            at = lambda t: t.data_ptr() if t is not None else 0
+            with _On(dev):
+                _lib.check(L.sln_mx4_linear_bwd(g.data_ptr(), kind, pitch, at(y), at(scale), xc, xs, wc, ws, M, N, K,
+                                                at(gx), at(gw), at(gb), work.data_ptr(), nbytes, _stream(dev)),
+                           "sln_mx4_linear_bwd")
+        return gx, gw, gb, None, None, None
 
 
 def mx4_linear(x, weight, bias=None, scale=None, relu=False):
@@ -174,21 +211,29 @@ def mx4_linear(x, weight, bias=None, scale=None, relu=False):
         _need_float(weight, "weight")
         if weight.dtype != torch.float32:
             raise TypeError("weight must be float32 or an Mx4Tensor, got %s" % weight.dtype)
-    if len(weight.shape) != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] or weight.shape[1] < 1:
-        raise ValueError("mx4_linear: x %s does not fit a weight %s" % (tuple(x.shape), tuple(weight.shape)))
-    N = weight.shape[0]
+    wshape, dev = weight.shape, x.device
+    if len(wshape) != 2 or x.dim() < 1 or x.shape[-1] != wshape[1] or wshape[1] < 1:
+        raise ValueError("mx4_linear: x %s does not fit a weight %s" % (tuple(x.shape), tuple(wshape)))
+    N = wshape[0]
+    if weight.device != dev:
+        raise ValueError("weight is on %s, x on %s" % (weight.device, dev))
     for t, name in ((bias, "bias"), (scale, "scale")):
         if t is None:
             continue
         if not torch.is_tensor(t) or t.dtype != torch.float32:
             raise TypeError("%s must be a float32 tensor" % name)
-        if tuple(t.shape) != (N,):
+        if t.dim() != 1 or t.shape[0] != N:
             raise ValueError("%s must be [%d], got %s" % (name, N, tuple(t.shape)))
-    for t, name in ((weight, "weight"), (bias, "bias"), (scale, "scale")):
-        if t is not None and t.device != x.device:
-            raise ValueError("%s is on %s, x on %s" % (name, t.device, x.device))
-    if scale is not None and scale.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError("mx4_linear: scale gets no gradient (a frozen normalisation's factor); detach it")
-    bias = bias.contiguous() if bias is not None else None
-    scale = scale.detach().contiguous() if scale is not None else None
-    return _Mx4LinearFn.apply(x, None if wq is not None else weight, bias, scale, bool(relu), wq)
+        if t.device != dev:
+            raise ValueError("%s is on %s, x on %s" % (name, t.device, dev))
+    grad = torch.is_grad_enabled()
+    if scale is not None:
+        if grad and scale.requires_grad:
+            raise RuntimeError("mx4_linear: scale gets no gradient (a frozen normalisation's factor); detach it")
+        scale = scale.detach().contiguous() if scale.requires_grad or not scale.is_contiguous() else scale
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.contiguous()
+    if grad and (x.requires_grad or (wq is None and weight.requires_grad) or (bias is not None and bias.requires_grad)):
+        return _Mx4LinearFn.apply(x, None if wq is not None else weight, bias, scale, bool(relu), wq)
+    y = _forward(x, weight, wq, bias, scale, bool(relu), False)[0]
+    return y if x.dim() == 2 else y.view(x.shape[:-1] + (N,))
