@@ -104,12 +104,14 @@ struct MxGemm {
     int relu;
 };
 
+// One rounding for scale, one for bias (no fused multiply-add), so that every kernel of this file ends alike.
+__device__ __forceinline__ float mx_act(float v, float scale, float bias, int relu) {
+    v = __fadd_rn(__fmul_rn(v, scale), bias);
+    return relu && v < 0.f ? 0.f : v;              // (a NaN stays)
+}
 template <typename T>
 __device__ __forceinline__ void mx_finish(const MxGemm &p, int m, int n, float v) {
-    if (p.scale) v *= p.scale[n];
-    if (p.bias) v += p.bias[n];
-    if (p.relu) v = v < 0.f ? 0.f : v;             // (a NaN stays)
-    ((T *)p.y)[(int64_t)m * p.N + n] = (T)v;
+    ((T *)p.y)[(int64_t)m * p.N + n] = (T)mx_act(v, p.scale ? p.scale[n] : 1.f, p.bias ? p.bias[n] : 0.f, p.relu);
 }
 
 __device__ __forceinline__ i32x8 mx_frag(const char *at) {
@@ -134,7 +136,7 @@ __global__ __launch_bounds__(256, 2) void mx4_product_kernel(const MxGemm p, int
     unsigned aoff[4], boff[4];
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-        const int slot = (q * 4 + wave) * 64 + lane, row = slot >> 3, c = (slot & 7) ^ (row & 7);
+        const int slot = (q * 4 + wave) * 64 + lane, row = slot >> 3, c = (slot & 7) ^ ((row >> 1) & 7);
         aoff[q] = (unsigned)(min(row, p.M - 1 - m0) * p.a_pitch + c * 16);
         boff[q] = (unsigned)(min(row, p.N - 1 - n0) * p.b_pitch + c * 16);
     }
@@ -185,8 +187,8 @@ __global__ __launch_bounds__(256, 2) void mx4_product_kernel(const MxGemm p, int
             i32x8 fa[2], fb[2];                                                                              \
             _Pragma("unroll") for (int i = 0; i < 2; ++i) {                                                  \
                 const int ra = 64 * wr + 32 * i + frow, rb = 64 * wc + 32 * i + frow;                        \
-                fa[i] = mx_frag(la + ra * 128 + (((4 * half + Q) ^ (ra & 7)) << 4));                         \
-                fb[i] = mx_frag(lb + rb * 128 + (((4 * half + Q) ^ (rb & 7)) << 4));                         \
+                fa[i] = mx_frag(la + ra * 128 + (((4 * half + Q) ^ ((ra >> 1) & 7)) << 4));                         \
+                fb[i] = mx_frag(lb + rb * 128 + (((4 * half + Q) ^ ((rb >> 1) & 7)) << 4));                         \
             }                                                                                                \
             _Pragma("unroll") for (int i = 0; i < 2; ++i) _Pragma("unroll") for (int j = 0; j < 2; ++j)      \
                 acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fa[i], fb[j], acc[i][j], 4, 4,   \
@@ -198,20 +200,24 @@ __global__ __launch_bounds__(256, 2) void mx4_product_kernel(const MxGemm p, int
         MX_QUARTER(3)
 #undef MX_QUARTER
     }
+    const int row0 = m0 + 64 * wr, col0 = n0 + 64 * wc + frow;
+    const bool inside = row0 + 64 <= p.M && col0 - frow + 64 <= p.N;              // (uniform: no test per element)
+    float *slab = p.nsplit > 1 ? p.slab + (int64_t)split * p.M * p.N : nullptr;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int j = 0; j < 2; ++j) {
+        const int n = col0 + 32 * j;
+        const float cs = p.scale ? p.scale[min(n, p.N - 1)] : 1.f, cb = p.bias ? p.bias[min(n, p.N - 1)] : 0.f;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int n = n0 + 64 * wc + 32 * j + frow;
-            if (n >= p.N) continue;
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const int m = m0 + 64 * wr + 32 * i + nt_acc_row(r, lane);
-                if (m >= p.M) continue;
-                if (p.nsplit > 1) p.slab[((int64_t)split * p.M + m) * p.N + n] = acc[i][j][r];
-                else mx_finish<T>(p, m, n, acc[i][j][r]);
+                const int m = row0 + 32 * i + nt_acc_row(r, lane);
+                if (!inside && (m >= p.M || n >= p.N)) continue;
+                const int64_t e = (int64_t)m * p.N + n;
+                if (slab) slab[e] = acc[i][j][r];
+                else ((T *)p.y)[e] = (T)mx_act(acc[i][j][r], cs, cb, p.relu);
             }
-        }
+    }
 }
 
 // The cuts of the contraction, added in order, and the epilogue.

@@ -146,6 +146,11 @@ __global__ __launch_bounds__(256) void mx4_grad_prep_kernel(const MgPrep p) {
     else mg_turn(p.x_codes, p.x_scales, p.M, p.K, p.xt, blockIdx.x - p.split - p.turn_w, z);
 }
 
+// 128 x 128 tiles, two workgroups per CU
+template <int P>
+struct MgShape : NtShape<P, 1, 128, 128, 2, 2, 2> {};
+#define MG_TILE 128
+
 struct MgProduct {
     const char *a, *b;            // parts rows: a [RA] of P parts, b [RB] of one
     int RA, RB, groups, nsplit;
@@ -162,29 +167,36 @@ __device__ __forceinline__ void mg_finish(const MgProduct &p, int i, int64_t at,
 
 template <typename T, int P>
 __device__ __forceinline__ void mg_product(const MgProduct &p, int at, char *smem) {
-    const int ta = (p.RA + NT_TILE - 1) / NT_TILE;
+    const int ta = (p.RA + MG_TILE - 1) / MG_TILE;
     const int split = at % p.nsplit, tile = at / p.nsplit;
-    const int i0 = tile % ta * NT_TILE, j0 = tile / ta * NT_TILE;
+    const int i0 = tile % ta * MG_TILE, j0 = tile / ta * MG_TILE;
     const int64_t ra = (int64_t)p.groups * 64 * P, rb = (int64_t)p.groups * 64;
     const int g0 = (int)((int64_t)p.groups * split / p.nsplit), g1 = (int)((int64_t)p.groups * (split + 1) / p.nsplit);
     f32x16 acc[2][2];
-    nt_tile<b16x8, P, 1, NT_EXACTB>(p.a + i0 * ra, ra, p.RA - i0, p.b + j0 * rb, rb, p.RB - j0, g0, g1, smem, acc);
+    nt_tile<MgShape<P>, b16x8, NT_EXACTB, false>(p.a + i0 * ra, ra, p.RA - i0, 0, p.b + j0 * rb, rb, p.RB - j0, g0, g1, smem, acc);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int row0 = i0 + 64 * (wave >> 1), col0 = j0 + 64 * (wave & 1) + (lane & 31);
+    const bool inside = row0 + 64 <= p.RA && col0 - (lane & 31) + 64 <= p.RB;     // (uniform: no test per element)
+    float *slab = p.nsplit > 1 ? p.slab + (int64_t)split * p.RA * p.RB : nullptr;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < 2; ++i) {
+        float rs[16];                              // (loads ahead of the stores, which the compiler may not pass)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+            rs[r] = p.row_scale && !slab ? p.row_scale[min(row0 + 32 * i + nt_acc_row(r, lane), p.RA - 1)] : 1.f;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            const int col = j0 + 64 * (wave & 1) + 32 * j + (lane & 31);
-            if (col >= p.RB) continue;
+            const int col = col0 + 32 * j;
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const int row = i0 + 64 * (wave >> 1) + 32 * i + nt_acc_row(r, lane);
-                if (row >= p.RA) continue;
+                const int row = row0 + 32 * i + nt_acc_row(r, lane);
+                if (!inside && (row >= p.RA || col >= p.RB)) continue;
                 const int64_t e = (int64_t)row * p.RB + col;
-                if (p.nsplit > 1) p.slab[(int64_t)split * p.RA * p.RB + e] = acc[i][j][r];
-                else mg_finish<T>(p, row, e, acc[i][j][r]);
+                if (slab) slab[e] = acc[i][j][r];
+                else ((T *)p.c)[e] = (T)(acc[i][j][r] * rs[r]);
             }
         }
+    }
 }
 
 // Both products and the bias sums in one launch (x: gx, w: gw; tiles = 0: not wanted).
@@ -192,7 +204,7 @@ template <typename T, int P>
 __global__ __launch_bounds__(256, 2) void mx4_grad_product_kernel(const MgProduct x, const MgProduct w,
                                                                   const float *__restrict__ bias_part, int bias_blocks,
                                                                   int N, float *__restrict__ gb) {
-    __shared__ __attribute__((aligned(128))) char smem[2 * NtShape<P, 1>::STAGE];
+    __shared__ __attribute__((aligned(128))) char smem[MgShape<P>::LDS];
     if (blockIdx.x < x.tiles) {
         mg_product<T, P>(x, nt_xcd_order(blockIdx.x, x.tiles), smem);
     } else if (blockIdx.x < x.tiles + w.tiles) {
@@ -228,7 +240,7 @@ struct MgPlan {
 };
 static inline int64_t mg_align(int64_t v) { return (v + 255) & ~(int64_t)255; }
 static inline int mg_cuts(int64_t RA, int64_t RB, int64_t groups) {
-    const int64_t tiles = ((RA + NT_TILE - 1) / NT_TILE) * ((RB + NT_TILE - 1) / NT_TILE);
+    const int64_t tiles = ((RA + MG_TILE - 1) / MG_TILE) * ((RB + MG_TILE - 1) / MG_TILE);
     int64_t c = 512 / (tiles < 1 ? 1 : tiles);
     if (c > groups / 8) c = groups / 8;
     if (c > 32) c = 32;
@@ -263,7 +275,7 @@ static MgProduct mg_job(const char *a, int64_t RA, const char *b, int64_t RB, in
     if (!c) return p;
     p.a = a; p.b = b; p.RA = (int)RA; p.RB = (int)RB;
     p.groups = (int)((k + 31) / 32); p.nsplit = cuts;
-    p.tiles = (unsigned)(((RA + NT_TILE - 1) / NT_TILE) * ((RB + NT_TILE - 1) / NT_TILE) * cuts);
+    p.tiles = (unsigned)(((RA + MG_TILE - 1) / MG_TILE) * ((RB + MG_TILE - 1) / MG_TILE) * cuts);
     p.row_scale = row_scale; p.c = c; p.slab = (float *)slab;
     return p;
 }

@@ -11,28 +11,36 @@
 // Where eps outweighs |G| (|X|_F = r << 1) the operand holds X 2^h instead, h = floor(-log2 r) in the first step and two
 // less in each later one (|X| grows by at most 3.45 < 4 a step): then A is held times 4^h.
 //
-// Launches (all matrices of a call in each of them; a work list in the workspace, made by the first launch):
+// Launches (all matrices of a call in each of them; work lists in the workspace, made by the first launch):
 //   ortho_norm_kernel    partial sums of squares in double (the optimiser: also the momentum update), the work lists
-//   ortho_split_kernel   u = G / (|G| + eps) -> parts of X [m][n] and of X^T [n][m]
-//   per step: ortho_gram_kernel    A's tiles on and above the diagonal (A is symmetric), the contraction over n cut so that
-//                                  the launch fills the chip; one cut: parts of A are written (both triangles), several:
-//                                  fp32 partial tiles, added in order by ortho_join_kernel
+//   ortho_split_kernel   u = G / (|G| + eps) -> parts of X [m][n]
+//   per step: ortho_gram_kernel    A's 128 x 128 tiles on and above the diagonal (A is symmetric), the contraction over n
+//                                  cut so that one round of workgroups fills the chip; one cut: parts of A are written
+//                                  (both triangles), several: fp32 partial tiles, added in order by ortho_join_kernel
 //             ortho_poly_kernel    P's tiles on and above the diagonal from A A^T, parts of both triangles
-//             ortho_apply_kernel   X <- P X from P's rows and X^T's rows: parts of X (next step's Gram matrix) and of X^T
-//                                  (next step's product); the last step writes the result, or updates the weights.
-// Every contraction runs along rows of both operands: that is why X is kept both ways.
+//             ortho_apply_kernel   X <- P X; the last step writes the result, or updates the weights.
+// X is kept one way only, rows of n.  The Gram matrix contracts along its rows; P X contracts across them and computes
+// (P X)^T with X as the first operand, read through LDS's transposing loads: the 16 accumulator values of a lane are then
+// neighbours along n, and parts go straight from registers to X's rows, 16 bytes a store.
+// A call whose matrices all fit one CU's LDS (ortho_small) is ONE launch instead, ortho_small_kernel: a workgroup per
+// matrix runs all the steps on chip.
 #include "mfma_nt.h"
 
-#define ORTHO_BATCH 32                     // matrices per ortho_norm_kernel launch (descriptors travel by value)
+#define ORTHO_BATCH 32                     // matrices per launch that takes descriptors by value
 #define ORTHO_CHUNK 16384                  // elements per partial sum of squares
 #define ORTHO_SCALE 16384.0f               // 2^14
 #define ORTHO_UNSCALE 6.103515625e-05f     // 2^-14
-#define ORTHO_PITCH 133                    // floats per row of the 64-row epilogue slab: odd, 8 * 133 = 40 mod 64
-#define ORTHO_LDS (2 * NtShape<2, 2>::STAGE)
+#define ORTHO_A 3.4445f
+#define ORTHO_B -4.7750f
+#define ORTHO_C 2.0315f
+#define GRAM_TILE 128
 
-static_assert(64 * ORTHO_PITCH * 4 <= ORTHO_LDS, "epilogue slab must fit the operand stages");
+typedef NtShape<2, 2, 128, 128, 2, 2, 2> OrthoGram;        // and the polynomial's large tile
+typedef NtShape<2, 2, 64, 64, 2, 2, 4> OrthoPolySmall;
+typedef NtShape<2, 2, 128, 128, 2, 2, 2> OrthoApplySmall;
+typedef NtShape<2, 2, 256, 256, 2, 4, 2> OrthoApplyLarge;
 
-// What one launch of ortho_norm_kernel is told about a matrix (by value), and the entry it leaves in the table.
+// What the launches are told about a matrix: by value to the first, a table in the workspace for the others.
 struct OrthoProb {
     const void *g;         // rows x cols, row stride gs
     void *out;             // rows x cols, row stride os (the optimiser: the weights)
@@ -40,98 +48,146 @@ struct OrthoProb {
     int64_t gs, os, off;   // off: byte offset of this matrix's operands in the workspace
     int32_t rows, cols;
     int32_t part0, nparts; // its partial sums of squares
-    int32_t sym0, gram0, apply0, nsplit;   // first entries in the work lists, cuts of the Gram contraction
+    int32_t split0, sym0, gram0, poly0, apply0, nsplit;    // first entries in the work lists, cuts of the contraction
     float lr, decay;       // update: p = p * decay - lr * X
     int32_t shift;         // h of the first step (ortho_split_kernel)
 };
 
-struct OrthoTile { int32_t prob, ij, first, split; };   // ij = row tile << 16 | column tile; first: gram entry of cut 0
+struct OrthoTile { int32_t prob, ij, first, cut; };        // ij = row tile << 16 | column tile; first: gram entry of cut 0
 
 struct OrthoTable {
     OrthoProb *prob;
-    OrthoTile *sym, *gram, *apply;
+    OrthoTile *split, *sym, *gram, *poly, *apply;
     double *part;
     char *ws;
-    float *slab;           // partial Gram tiles, NT_TILE^2 floats per gram entry
+    float *slab;           // partial Gram tiles, GRAM_TILE^2 floats per gram entry
+    int poly_tile, apply_tile;
 };
 
 struct OrthoBatch { OrthoProb p[ORTHO_BATCH]; };
+struct OrthoRule {         // the optimiser's side of a call
+    const double *sqnorm;
+    float max_norm, momentum;
+    int nesterov;
+};
 
 __host__ __device__ __forceinline__ int ortho_m(const OrthoProb &p) { return p.rows < p.cols ? p.rows : p.cols; }
 __host__ __device__ __forceinline__ int ortho_n(const OrthoProb &p) { return p.rows < p.cols ? p.cols : p.rows; }
 __host__ __device__ __forceinline__ int64_t ortho_row_bytes(int k) { return (int64_t)((k + 31) / 32) * 128; }
+__host__ __device__ __forceinline__ int ortho_tiles(int v, int tile) { return (v + tile - 1) / tile; }
 
-// operands of a matrix inside the workspace: X, X^T (two, in turn), A, P
-struct OrthoOperands { char *x, *xt[2], *a, *p; };
-__device__ __forceinline__ OrthoOperands ortho_operands(const OrthoProb &p, char *ws) {
+// operands of a matrix inside the workspace: X (two, in turn), A, P
+struct OrthoOperands {
+    char *x, *next, *a, *p;                        // this step's X, the next one's
+};
+__device__ __forceinline__ OrthoOperands ortho_operands(const OrthoProb &p, char *ws, int step) {
     const int m = ortho_m(p), n = ortho_n(p);
-    const int64_t bx = m * ortho_row_bytes(n), bt = n * ortho_row_bytes(m), bs = m * ortho_row_bytes(m);
+    const int64_t bx = m * ortho_row_bytes(n);
     OrthoOperands o;
-    o.x = ws + p.off;
-    o.xt[0] = o.x + bx;
-    o.xt[1] = o.xt[0] + bt;
-    o.a = o.xt[1] + bt;
-    o.p = o.a + bs;
+    o.x = ws + p.off + (step & 1) * bx;
+    o.next = ws + p.off + ((step & 1) ^ 1) * bx;
+    o.a = ws + p.off + 2 * bx;
+    o.p = o.a + m * ortho_row_bytes(m);
     return o;
 }
 static int64_t ortho_operand_bytes(const OrthoProb &p) {
     const int m = ortho_m(p), n = ortho_n(p);
-    return m * ortho_row_bytes(n) + 2 * n * ortho_row_bytes(m) + 2 * m * ortho_row_bytes(m);
+    return 2 * m * ortho_row_bytes(n) + 2 * m * ortho_row_bytes(m);
 }
 
 // 2^(sign h) for step `step`
-__device__ __forceinline__ float ortho_shift(const OrthoProb &p, int step, int sign) {
-    return ldexpf(1.f, sign * max(0, p.shift - 2 * step));
+__device__ __forceinline__ float ortho_shift(int shift, int step, int sign) {
+    return ldexpf(1.f, sign * max(0, shift - 2 * step));
+}
+// 1 / (norm + eps) and h
+__device__ __forceinline__ float ortho_inverse(double sum, float eps, int &shift) {
+    const double norm = sqrt(sum), r = norm / (norm + (double)eps);
+    shift = 0;
+    if (r > 0.0 && r < 1.0) {
+        frexp(r, &shift);                          // r < 2^shift
+        shift = min(max(-shift, 0), 126);
+    }
+    return (float)(1.0 / (norm + (double)eps));
 }
 
 template <typename T>
 __device__ __forceinline__ float ortho_load(const void *p, int64_t i) { return (float)((const T *)p)[i]; }
 
 // The clip coefficient and the verdict of the optimiser's guard (a non-finite norm: the step is not applied).
-__device__ __forceinline__ bool ortho_clip(const double *sqnorm, float max_norm, float &cf) {
-    const double sq = sqnorm[0];
-    const double coef = (double)max_norm / (sqrt(sq) + 1e-6);
+__device__ __forceinline__ bool ortho_clip(const OrthoRule &rule, float &cf) {
+    const double sq = rule.sqnorm[0];
+    const double coef = (double)rule.max_norm / (sqrt(sq) + 1e-6);
     cf = coef < 1.0 ? (float)coef : 1.0f;
     return sq >= 0.0 && sq < INFINITY;
 }
+// One element of the momentum update (b is written if `apply`) and what is orthogonalised.
+__device__ __forceinline__ float ortho_momentum(const OrthoRule &rule, float g, float cf, float &b) {
+    const float gc = g * cf;
+    b = rule.momentum * b + gc;
+    return rule.nesterov ? gc + rule.momentum * b : b;
+}
+// The same from the momentum that is already updated.
+__device__ __forceinline__ float ortho_update(const OrthoRule &rule, float g, float cf, float b) {
+    return rule.nesterov ? g * cf + rule.momentum * b : b;
+}
+
+__device__ __forceinline__ double ortho_block_sum(double acc, double *s_red) {      // any whole number of waves
+    for (int o = 32; o > 0; o >>= 1) acc += __shfl_xor(acc, o);
+    if ((threadIdx.x & 63) == 0) s_red[threadIdx.x >> 6] = acc;
+    __syncthreads();
+    double s = 0.0;
+    for (int w = 0; w < (int)blockDim.x / 64; ++w) s += s_red[w];
+    return s;
+}
 
 // ------------------------------------------------------------------------------------------------ norms and lists
+__device__ __forceinline__ void ortho_lists(const OrthoProb &p, int prob, const OrthoTable &tab) {
+    const int t = threadIdx.x, m = ortho_m(p), n = ortho_n(p);
+    if (t == 0) tab.prob[prob] = p;
+    const int si = ortho_tiles(m, 64), sj = ortho_tiles(n, 128);
+    for (int e = t; e < si * sj; e += 256) {
+        const OrthoTile w = {prob, (e / sj) << 16 | (e % sj), 0, 0};
+        tab.split[p.split0 + e] = w;
+    }
+    const int tm = ortho_tiles(m, GRAM_TILE), nsym = tm * (tm + 1) / 2;
+    for (int e = t; e < tm * tm; e += 256) {
+        const int i = e / tm, j = e - i * tm;
+        if (j < i) continue;
+        const int s = i * tm - i * (i - 1) / 2 + (j - i);
+        OrthoTile w = {prob, i << 16 | j, p.gram0 + s, 0};
+        tab.sym[p.sym0 + s] = w;
+        for (int k = 0; k < p.nsplit; ++k) {
+            w.cut = k;
+            tab.gram[p.gram0 + k * nsym + s] = w;
+        }
+    }
+    const int tp = ortho_tiles(m, tab.poly_tile);
+    for (int e = t; e < tp * tp; e += 256) {
+        const int i = e / tp, j = e - i * tp;
+        if (j < i) continue;
+        const OrthoTile w = {prob, i << 16 | j, 0, 0};
+        tab.poly[p.poly0 + i * tp - i * (i - 1) / 2 + (j - i)] = w;
+    }
+    const int ti = ortho_tiles(m, tab.apply_tile), tj = ortho_tiles(n, tab.apply_tile);
+    for (int e = t; e < ti * tj; e += 256) {       // the m tiles of one column of X run side by side
+        const OrthoTile w = {prob, (e % ti) << 16 | (e / ti), 0, 0};
+        tab.apply[p.apply0 + e] = w;
+    }
+}
+
 // Block (c, i): elements [c, c + 1) * ORTHO_CHUNK of matrix i (row-major order) -> one partial sum of squares, added in a
 // fixed order.  The optimiser (buf != NULL): b <- momentum b + cf g is written on the way and the sum is that of
 // u = cf g + momentum b (nesterov) or u = b.  Memory-bound: 4 B read (optimiser: 8 read + 4 written) per element.
 template <typename T>
-__global__ __launch_bounds__(256) void ortho_norm_kernel(OrthoBatch batch, int prob0, OrthoTable tab,
-                                                         const double *__restrict__ sqnorm, float max_norm,
-                                                         float momentum, int nesterov) {
+__global__ __launch_bounds__(256) void ortho_norm_kernel(OrthoBatch batch, int prob0, OrthoTable tab, OrthoRule rule) {
     __shared__ double s_red[4];
     const OrthoProb &p = batch.p[blockIdx.y];
     const int t = threadIdx.x, chunk = blockIdx.x;
-    const int m = ortho_m(p), n = ortho_n(p);
-    const int tm = (m + NT_TILE - 1) / NT_TILE, tn = (n + NT_TILE - 1) / NT_TILE;
-    if (chunk == 0) {
-        if (t == 0) tab.prob[prob0 + blockIdx.y] = p;
-        const int prob = prob0 + blockIdx.y, nsym = tm * (tm + 1) / 2;
-        for (int e = t; e < tm * tm; e += 256) {
-            const int i = e / tm, j = e - i * tm;
-            if (j < i) continue;
-            const int s = i * tm - i * (i - 1) / 2 + (j - i);
-            const OrthoTile tile = {prob, i << 16 | j, p.gram0 + s, p.nsplit};
-            tab.sym[p.sym0 + s] = tile;
-            for (int k = 0; k < p.nsplit; ++k) {
-                const OrthoTile cut = {prob, i << 16 | j, p.gram0 + s, k};
-                tab.gram[p.gram0 + k * nsym + s] = cut;
-            }
-        }
-        for (int e = t; e < tm * tn; e += 256) {
-            const int j = e / tm, i = e - j * tm;
-            const OrthoTile tile = {prob, i << 16 | j, 0, 0};
-            tab.apply[p.apply0 + e] = tile;
-        }
-    }
+    if (chunk == 0) ortho_lists(p, prob0 + blockIdx.y, tab);
     if (chunk >= p.nparts) return;
     float cf = 1.f;
     bool apply = true;
-    if (p.buf) apply = ortho_clip(sqnorm, max_norm, cf);
+    if (p.buf) apply = ortho_clip(rule, cf);
     const int64_t total = (int64_t)p.rows * p.cols, e0 = (int64_t)chunk * ORTHO_CHUNK;
     const int64_t e1 = min(total, e0 + ORTHO_CHUNK);
     double acc = 0.0;
@@ -139,9 +195,9 @@ __global__ __launch_bounds__(256) void ortho_norm_kernel(OrthoBatch batch, int p
     auto one = [&](float g, float *b) {
         float u = g;
         if (p.buf) {
-            const float gc = g * cf, nb = momentum * *b + gc;
+            float nb = *b;
+            u = ortho_momentum(rule, g, cf, nb);
             if (apply) *b = nb;
-            u = nesterov ? gc + momentum * nb : nb;
         }
         acc += (double)u * u;
     };
@@ -171,10 +227,8 @@ __global__ __launch_bounds__(256) void ortho_norm_kernel(OrthoBatch batch, int p
             one(ortho_load<T>(p.g, ge), p.buf ? p.buf + e : nullptr);
         }
     }
-    for (int o = 32; o > 0; o >>= 1) acc += __shfl_xor(acc, o);
-    if ((t & 63) == 0) s_red[t >> 6] = acc;
-    __syncthreads();
-    if (t == 0) tab.part[p.part0 + chunk] = (s_red[0] + s_red[1]) + (s_red[2] + s_red[3]);
+    acc = ortho_block_sum(acc, s_red);
+    if (t == 0) tab.part[p.part0 + chunk] = acc;
 }
 
 // ------------------------------------------------------------------------------------------------ parts
@@ -197,241 +251,270 @@ __device__ __forceinline__ void ortho_store8(char *at, const float *v) {
     *(f16x8 *)(at + 64) = h1;
 }
 
-// A 64 x 128 slab (rows i0 ..., columns j0 ... of an R x C matrix) from LDS to parts of the matrix (`dst`: R rows of
-// C values) and of its transpose (`dst_t`: C rows of R values); either may be NULL.  Values behind the last column (row)
-// are the zeros that pad the contraction: `keep` of a lane's values says so.
-__device__ __forceinline__ void ortho_store_slab(const float *slab, int i0, int j0, int R, int C, char *dst, char *dst_t) {
-    const int t = threadIdx.x;
-    if (dst) {
-        const int64_t rb = ortho_row_bytes(C);
-        const int cpad = (C + 31) & ~31;
-        for (int e = t; e < 64 * 16; e += 256) {
-            const int r = e >> 4, k = j0 + (e & 15) * 8;
-            if (i0 + r >= R || k >= cpad) continue;
-            float v[8];
-#pragma unroll
-            for (int q = 0; q < 8; ++q) v[q] = k + q < C ? slab[r * ORTHO_PITCH + (e & 15) * 8 + q] : 0.f;
-            ortho_store8(ortho_at(dst, rb, i0 + r, k), v);
-        }
-    }
-    if (dst_t) {
-        const int64_t rb = ortho_row_bytes(R);
-        const int rpad = (R + 31) & ~31;
-        for (int e = t; e < 128 * 8; e += 256) {
-            const int c = e >> 3, k = i0 + (e & 7) * 8;
-            if (j0 + c >= C || k >= rpad) continue;
-            float v[8];
-#pragma unroll
-            for (int q = 0; q < 8; ++q) v[q] = k + q < R ? slab[((e & 7) * 8 + q) * ORTHO_PITCH + c] : 0.f;
-            ortho_store8(ortho_at(dst_t, rb, j0 + c, k), v);
-        }
-    }
-}
-
-// Accumulators of slab h (the two waves that hold rows 64 h ... 64 h + 63) to LDS, in units of the values.
-__device__ __forceinline__ void ortho_slab_from_acc(float *slab, const f32x16 (&acc)[2][2], int h, float unscale) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    if ((wave >> 1) != h) return;
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-                slab[(32 * i + nt_acc_row(r, lane)) * ORTHO_PITCH + 64 * (wave & 1) + 32 * j + (lane & 31)] =
-                    acc[i][j][r] * unscale;
-}
-
-// ------------------------------------------------------------------------------------------------ G -> X, X^T
-// Block = one 128 x 128 tile of X in two 64-row slabs.  Reads 4 B (optimiser: 8, u is made again from g and the new
-// momentum), writes 8 B per element.
+// ------------------------------------------------------------------------------------------------ G -> X
+// Block = 64 x 128 of X.  Reads 4 B (optimiser: 8, u is made again from g and the new momentum), writes 4 B per element.
 template <typename T>
-__global__ __launch_bounds__(256) void ortho_split_kernel(OrthoTable tab, const double *__restrict__ sqnorm,
-                                                          float max_norm, float momentum, int nesterov, float eps) {
-    __shared__ float slab[64 * ORTHO_PITCH];
+__global__ __launch_bounds__(256) void ortho_split_kernel(OrthoTable tab, OrthoRule rule, float eps) {
+    __shared__ float slab[64 * 129];
     __shared__ double s_red[4];
-    const OrthoTile w = tab.apply[blockIdx.x];
+    const OrthoTile w = tab.split[blockIdx.x];
     const OrthoProb p = tab.prob[w.prob];
     const int t = threadIdx.x, m = ortho_m(p), n = ortho_n(p);
     double acc = 0.0;
     for (int i = t; i < p.nparts; i += 256) acc += tab.part[p.part0 + i];
-    for (int o = 32; o > 0; o >>= 1) acc += __shfl_xor(acc, o);
-    if ((t & 63) == 0) s_red[t >> 6] = acc;
-    __syncthreads();
-    const double norm = sqrt((s_red[0] + s_red[1]) + (s_red[2] + s_red[3]));
-    const float inv = (float)(1.0 / (norm + (double)eps));
-    const double r = norm / (norm + (double)eps);
-    int shift = 0;
-    if (r > 0.0 && r < 1.0) {
-        frexp(r, &shift);                          // r < 2^shift
-        shift = min(max(-shift, 0), 126);
-    }
+    int shift;
+    const float inv = ortho_inverse(ortho_block_sum(acc, s_red), eps, shift);
     if (w.ij == 0 && t == 0) tab.prob[w.prob].shift = shift;
     const float up = ldexpf(1.f, shift);           // |g| up <= norm + eps
     float cf = 1.f;
-    if (p.buf) ortho_clip(sqnorm, max_norm, cf);
+    if (p.buf) ortho_clip(rule, cf);
     const bool tall = p.rows > p.cols;
-    const OrthoOperands o = ortho_operands(p, tab.ws);
-    const int i0 = (w.ij >> 16) * NT_TILE, j0 = (w.ij & 0xffff) * NT_TILE;
-    auto value = [&](int r, int c) {               // of G, original orientation
-        const float g = ortho_load<T>(p.g, (int64_t)r * p.gs + c);
-        if (!p.buf) return g * up * inv;
-        const float b = p.buf[(int64_t)r * p.cols + c];
-        return (nesterov ? g * cf + momentum * b : b) * up * inv;
-    };
-    for (int h = 0; h < 2; ++h) {
-        const int r0 = i0 + 64 * h;
-        if (r0 >= m) break;
-        __syncthreads();
+    char *x = ortho_operands(p, tab.ws, 0).x;
+    const int64_t rb = ortho_row_bytes(n);
+    const int i0 = (w.ij >> 16) * 64, j0 = (w.ij & 0xffff) * 128, npad = (n + 31) & ~31;
+    if (tall) {                                    // X = G^T: lanes along G's rows, turned in LDS
         for (int e = t; e < 64 * 128; e += 256) {
-            int i, j;                               // of the slab; the faster one runs along G's rows
-            if (tall) { i = e & 63; j = e >> 6; } else { j = e & 127; i = e >> 7; }
-            const bool in = r0 + i < m && j0 + j < n;
-            slab[i * ORTHO_PITCH + j] = in ? (tall ? value(j0 + j, r0 + i) : value(r0 + i, j0 + j)) : 0.f;
+            const int i = e & 63, j = e >> 6;
+            float v = 0.f;
+            if (i0 + i < m && j0 + j < n) {
+                v = ortho_load<T>(p.g, (int64_t)(j0 + j) * p.gs + i0 + i);
+                if (p.buf) v = ortho_update(rule, v, cf, p.buf[(int64_t)(j0 + j) * p.cols + i0 + i]);
+            }
+            slab[i * 129 + j] = v * up * inv;
         }
         __syncthreads();
-        ortho_store_slab(slab, r0, j0, m, n, o.x, o.xt[0]);
+    }
+    for (int e = t; e < 64 * 16; e += 256) {
+        const int i = e >> 4, k = j0 + (e & 15) * 8;
+        if (i0 + i >= m || k >= npad) continue;
+        float v[8];
+        if (tall) {
+#pragma unroll
+            for (int q = 0; q < 8; ++q) v[q] = slab[i * 129 + (e & 15) * 8 + q];
+        } else {
+            const int64_t at = (int64_t)(i0 + i) * p.gs + k, bt = (int64_t)(i0 + i) * p.cols + k;
+            float g[8], b[8];
+            const bool wide = sizeof(T) == 4 && k + 8 <= n && !(((uintptr_t)((const float *)p.g + at)) & 15) &&
+                              !(p.buf && ((uintptr_t)(p.buf + bt) & 15));
+            if (wide) {
+                *(float4 *)g = *(const float4 *)((const float *)p.g + at);
+                *(float4 *)(g + 4) = *(const float4 *)((const float *)p.g + at + 4);
+                if (p.buf) {
+                    *(float4 *)b = *(const float4 *)(p.buf + bt);
+                    *(float4 *)(b + 4) = *(const float4 *)(p.buf + bt + 4);
+                }
+            } else {
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {
+                    g[q] = k + q < n ? ortho_load<T>(p.g, at + q) : 0.f;
+                    b[q] = p.buf && k + q < n ? p.buf[bt + q] : 0.f;
+                }
+            }
+#pragma unroll
+            for (int q = 0; q < 8; ++q) v[q] = (p.buf ? ortho_update(rule, g[q], cf, b[q]) : g[q]) * up * inv;
+        }
+        ortho_store8(ortho_at(x, rb, i0 + i, k), v);
     }
 }
 
+// ------------------------------------------------------------------------------------------------ symmetric tiles
+// A R x TILE slab (rows i0 ..., columns j0 ... of an m x m matrix) from LDS to parts of the matrix and, where `mirror`, of
+// its transpose.  Values behind the last column (row) are the zeros that pad the contraction.  The pitch TILE + 5 is odd
+// and 8 pitches are 40 mod 64: neither way of reading meets more than two lanes on a bank.
+template <int R, int TILE>
+__device__ __forceinline__ void ortho_store_sym(const float *slab, int i0, int j0, int m, char *dst, bool mirror) {
+    const int t = threadIdx.x, mpad = (m + 31) & ~31;
+    const int64_t rb = ortho_row_bytes(m);
+    for (int e = t; e < R * (TILE / 8); e += 256) {
+        const int r = e / (TILE / 8), c8 = e % (TILE / 8) * 8, k = j0 + c8;
+        if (i0 + r >= m || k >= mpad) continue;
+        float v[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] = k + q < m ? slab[r * (TILE + 5) + c8 + q] : 0.f;
+        ortho_store8(ortho_at(dst, rb, i0 + r, k), v);
+    }
+    if (!mirror) return;
+    for (int e = t; e < TILE * (R / 8); e += 256) {
+        const int c = e / (R / 8), r8 = e % (R / 8) * 8, k = i0 + r8;
+        if (j0 + c >= m || k >= mpad) continue;
+        float v[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] = k + q < m ? slab[(r8 + q) * (TILE + 5) + c] : 0.f;
+        ortho_store8(ortho_at(dst, rb, j0 + c, k), v);
+    }
+}
+
+// Accumulators of slab h (the waves that hold rows TILE / 2 h ...) to LDS, in units of the values.
+template <typename S>
+__device__ __forceinline__ void ortho_slab_from_acc(float *slab, const f32x16 (&acc)[S::FA][S::FB], int h, float unscale) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if (wave / S::WC != h) return;
+#pragma unroll
+    for (int i = 0; i < S::FA; ++i)
+#pragma unroll
+        for (int j = 0; j < S::FB; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                slab[(32 * i + nt_acc_row(r, lane)) * (S::TB + 5) + S::TB / S::WC * (wave % S::WC) + 32 * j + (lane & 31)] =
+                    acc[i][j][r] * unscale;
+}
+
 // ------------------------------------------------------------------------------------------------ A = X X^T
-__global__ __launch_bounds__(256, 2) void ortho_gram_kernel(OrthoTable tab, int ntiles) {
-    __shared__ __attribute__((aligned(128))) char smem[ORTHO_LDS];
-    const int at = nt_xcd_order(blockIdx.x, ntiles);
+__global__ __launch_bounds__(256, 2) void ortho_gram_kernel(OrthoTable tab, int step, int ntiles) {
+    typedef OrthoGram S;
+    __shared__ __attribute__((aligned(128))) char smem[S::LDS];
+    static_assert(64 * (S::TB + 5) * 4 <= S::LDS, "epilogue slab must fit the operand stages");
+    const int at = nt_xcd_runs(blockIdx.x, ntiles);
     const OrthoTile w = tab.gram[at];
     const OrthoProb p = tab.prob[w.prob];
-    const OrthoOperands o = ortho_operands(p, tab.ws);
+    const OrthoOperands o = ortho_operands(p, tab.ws, step);
     const int m = ortho_m(p), n = ortho_n(p);
-    const int i0 = (w.ij >> 16) * NT_TILE, j0 = (w.ij & 0xffff) * NT_TILE;
+    const int i0 = (w.ij >> 16) * GRAM_TILE, j0 = (w.ij & 0xffff) * GRAM_TILE;
     const int64_t rb = ortho_row_bytes(n);
     const int groups = (n + 31) / 32;
-    const int g0 = (int)((int64_t)groups * w.split / p.nsplit), g1 = (int)((int64_t)groups * (w.split + 1) / p.nsplit);
-    f32x16 acc[2][2];
-    nt_tile<f16x8, 2, 2, NT_SPLIT2>(o.x + i0 * rb, rb, m - i0, o.x + j0 * rb, rb, m - j0, g0, g1, smem, acc);
+    const int g0 = (int)((int64_t)groups * w.cut / p.nsplit), g1 = (int)((int64_t)groups * (w.cut + 1) / p.nsplit);
+    f32x16 acc[S::FA][S::FB];
+    nt_tile<S, f16x8, NT_SPLIT2, false>(o.x + i0 * rb, rb, m - i0, 0, o.x + j0 * rb, rb, m - j0, g0, g1, smem, acc);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     if (p.nsplit > 1) {
-        float *slab = tab.slab + (int64_t)at * NT_TILE * NT_TILE;
+        float *slab = tab.slab + (int64_t)at * GRAM_TILE * GRAM_TILE;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < S::FA; ++i)
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+            for (int j = 0; j < S::FB; ++j)
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
-                    slab[(64 * (wave >> 1) + 32 * i + nt_acc_row(r, lane)) * NT_TILE + 64 * (wave & 1) + 32 * j +
+                    slab[(64 * (wave >> 1) + 32 * i + nt_acc_row(r, lane)) * GRAM_TILE + 64 * (wave & 1) + 32 * j +
                          (lane & 31)] = acc[i][j][r];
         return;
     }
     for (int h = 0; h < 2; ++h) {
         if (i0 + 64 * h >= m) break;
         __syncthreads();
-        ortho_slab_from_acc((float *)smem, acc, h, ORTHO_UNSCALE * ORTHO_UNSCALE);
+        ortho_slab_from_acc<S>((float *)smem, acc, h, ORTHO_UNSCALE * ORTHO_UNSCALE);
         __syncthreads();
-        ortho_store_slab((const float *)smem, i0 + 64 * h, j0, m, m, o.a, i0 == j0 ? nullptr : o.a);
+        ortho_store_sym<64, GRAM_TILE>((const float *)smem, i0 + 64 * h, j0, m, o.a, i0 != j0);
     }
 }
 
-// The cuts of a Gram tile, added in order.  Block = 64 rows of one tile.
+// The cuts of a Gram tile, added in order.  Block = 32 rows of one tile.
 __global__ __launch_bounds__(256) void ortho_join_kernel(OrthoTable tab) {
-    __shared__ float slab[64 * ORTHO_PITCH];
-    const OrthoTile w = tab.sym[blockIdx.x >> 1];
-    const int h = blockIdx.x & 1;
+    __shared__ float slab[32 * (GRAM_TILE + 5)];
+    const OrthoTile w = tab.sym[blockIdx.x >> 2];
+    const int h = blockIdx.x & 3;
     const OrthoProb p = tab.prob[w.prob];
-    const int m = ortho_m(p), tm = (m + NT_TILE - 1) / NT_TILE, nsym = tm * (tm + 1) / 2;
-    const int i0 = (w.ij >> 16) * NT_TILE + 64 * h, j0 = (w.ij & 0xffff) * NT_TILE;
+    const int m = ortho_m(p), tm = ortho_tiles(m, GRAM_TILE), nsym = tm * (tm + 1) / 2;
+    const int i0 = (w.ij >> 16) * GRAM_TILE + 32 * h, j0 = (w.ij & 0xffff) * GRAM_TILE;
     if (p.nsplit == 1 || i0 >= m) return;
-    const OrthoOperands o = ortho_operands(p, tab.ws);
-    const float4 *src = (const float4 *)(tab.slab + (int64_t)w.first * NT_TILE * NT_TILE + 64 * h * NT_TILE);
-    for (int e = threadIdx.x; e < 64 * 32; e += 256) {
+    const float4 *src = (const float4 *)(tab.slab + (int64_t)w.first * GRAM_TILE * GRAM_TILE + 32 * h * GRAM_TILE);
+    const int64_t next = (int64_t)nsym * (GRAM_TILE * GRAM_TILE / 4);
+#pragma unroll
+    for (int e4 = 0; e4 < 4; ++e4) {
+        const int e = e4 * 256 + threadIdx.x;
         float4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
         for (int k = 0; k < p.nsplit; ++k) {
-            const float4 v = src[(int64_t)k * nsym * (NT_TILE * NT_TILE / 4) + e];
+            const float4 v = src[k * next + e];
             s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
         }
-        float *d = slab + (e >> 5) * ORTHO_PITCH + (e & 31) * 4;
+        float *d = slab + (e >> 5) * (GRAM_TILE + 5) + (e & 31) * 4;
         const float u = ORTHO_UNSCALE * ORTHO_UNSCALE;
         d[0] = s.x * u; d[1] = s.y * u; d[2] = s.z * u; d[3] = s.w * u;
     }
     __syncthreads();
-    ortho_store_slab(slab, i0, j0, m, m, o.a, (w.ij >> 16) == (w.ij & 0xffff) ? nullptr : o.a);
+    ortho_store_sym<32, GRAM_TILE>(slab, i0, j0, m, ortho_operands(p, tab.ws, 0).a, (w.ij >> 16) != (w.ij & 0xffff));
 }
 
 // ------------------------------------------------------------------------------------------------ P = a I + b A + c A^2
-__global__ __launch_bounds__(256, 2) void ortho_poly_kernel(OrthoTable tab, int ntiles, int step, float ca, float cb,
-                                                            float cc) {
-    __shared__ __attribute__((aligned(128))) char smem[ORTHO_LDS];
-    const OrthoTile w = tab.sym[nt_xcd_order(blockIdx.x, ntiles)];
+template <typename S>
+__global__ __launch_bounds__(256, 2) void ortho_poly_kernel(OrthoTable tab, int ntiles, int step) {
+    constexpr int TILE = S::TA, R = TILE / 2;
+    __shared__ __attribute__((aligned(128))) char smem[S::LDS];
+    static_assert(R * (TILE + 5) * 4 <= S::LDS, "epilogue slab must fit the operand stages");
+    const OrthoTile w = tab.poly[nt_xcd_runs(blockIdx.x, ntiles)];
     const OrthoProb p = tab.prob[w.prob];
-    const OrthoOperands o = ortho_operands(p, tab.ws);
+    const OrthoOperands o = ortho_operands(p, tab.ws, step);
     const int m = ortho_m(p);
-    const int i0 = (w.ij >> 16) * NT_TILE, j0 = (w.ij & 0xffff) * NT_TILE;
+    const int i0 = (w.ij >> 16) * TILE, j0 = (w.ij & 0xffff) * TILE;
     const int64_t rb = ortho_row_bytes(m);
-    f32x16 acc[2][2];
-    nt_tile<f16x8, 2, 2, NT_SPLIT2>(o.a + i0 * rb, rb, m - i0, o.a + j0 * rb, rb, m - j0, 0, (m + 31) / 32, smem, acc);
+    f32x16 acc[S::FA][S::FB];
+    nt_tile<S, f16x8, NT_SPLIT2, false>(o.a + i0 * rb, rb, m - i0, 0, o.a + j0 * rb, rb, m - j0, 0, (m + 31) / 32, smem, acc);
     const int t = threadIdx.x;
     float *slab = (float *)smem;
-    const float down = ortho_shift(p, step, -1), down2 = down * down;
+    const float down = ortho_shift(p.shift, step, -1), down2 = down * down;
     for (int h = 0; h < 2; ++h) {
-        const int r0 = i0 + 64 * h;
+        const int r0 = i0 + R * h;
         if (r0 >= m) break;
         __syncthreads();
-        ortho_slab_from_acc(slab, acc, h, cc * (down2 * down2) * (ORTHO_UNSCALE * ORTHO_UNSCALE));
+        ortho_slab_from_acc<S>(slab, acc, h, ORTHO_C * (down2 * down2) * (ORTHO_UNSCALE * ORTHO_UNSCALE));
         __syncthreads();
-        for (int e = t; e < 64 * 16; e += 256) {     // + b A + a I, in place
-            const int r = e >> 4, k = j0 + (e & 15) * 8;
+        for (int e = t; e < R * (TILE / 8); e += 256) {     // + b A + a I, in place
+            const int r = e / (TILE / 8), c8 = e % (TILE / 8) * 8, k = j0 + c8;
             if (r0 + r >= m || k >= m) continue;
             const char *at = ortho_at(o.a, rb, r0 + r, k);
             const f16x8 h0 = *(const f16x8 *)at, h1 = *(const f16x8 *)(at + 64);
-            float *d = slab + r * ORTHO_PITCH + (e & 15) * 8;
+            float *d = slab + r * (TILE + 5) + c8;
 #pragma unroll
             for (int q = 0; q < 8; ++q) {
                 const float av = ((float)h0[q] + (float)h1[q]) * (ORTHO_UNSCALE * down2);
-                d[q] += cb * av + (r0 + r == k + q ? ca : 0.f);
+                d[q] += ORTHO_B * av + (r0 + r == k + q ? ORTHO_A : 0.f);
             }
         }
         __syncthreads();
-        ortho_store_slab(slab, r0, j0, m, m, o.p, i0 == j0 ? nullptr : o.p);
+        ortho_store_sym<R, TILE>(slab, r0, j0, m, o.p, i0 != j0);
     }
 }
 
 // ------------------------------------------------------------------------------------------------ X <- P X
-// LAST: write the result in T (or update the weights: buf != NULL) instead of the next step's operands.
-template <typename T, bool LAST>
-__global__ __launch_bounds__(256, 2) void ortho_apply_kernel(OrthoTable tab, int ntiles, int step,
-                                                             const double *__restrict__ sqnorm) {
-    __shared__ __attribute__((aligned(128))) char smem[ORTHO_LDS];
-    const OrthoTile w = tab.apply[nt_xcd_order(blockIdx.x, ntiles)];
-    const OrthoProb p = tab.prob[w.prob];
-    const OrthoOperands o = ortho_operands(p, tab.ws);
-    const int m = ortho_m(p), n = ortho_n(p);
-    const int i0 = (w.ij >> 16) * NT_TILE, j0 = (w.ij & 0xffff) * NT_TILE;
-    const int64_t rb = ortho_row_bytes(m);
-    f32x16 acc[2][2];
-    nt_tile<f16x8, 2, 2, NT_SPLIT2>(o.p + i0 * rb, rb, m - i0, o.xt[step & 1] + j0 * rb, rb, n - j0, 0, (m + 31) / 32,
-                                    smem, acc);
-    const int t = threadIdx.x;
-    const float *slab = (const float *)smem;
-    const float unscale = ORTHO_UNSCALE * ORTHO_UNSCALE * ortho_shift(p, step, -1) * (LAST ? 1.f : ortho_shift(p, step + 1, 1));
-    if (LAST && p.buf) {
-        const double sq = sqnorm[0];
-        if (!(sq >= 0.0 && sq < INFINITY)) return;
-    }
-    for (int h = 0; h < 2; ++h) {
-        const int r0 = i0 + 64 * h;
-        if (r0 >= m) break;
-        __syncthreads();
-        ortho_slab_from_acc((float *)smem, acc, h, unscale);
-        __syncthreads();
-        if (!LAST) {
-            ortho_store_slab(slab, r0, j0, m, n, o.x, o.xt[(step & 1) ^ 1]);
-            continue;
+// Eight neighbours along n (columns k ... k + 7, of which n - k exist) of row `row` of the result.
+template <typename T>
+__device__ __forceinline__ void ortho_result8(const OrthoProb &p, int row, int k, int n, const float *v) {
+    const int64_t at = (int64_t)row * p.os + k;
+    if (p.buf) {
+        float *d = (float *)p.out + at;
+        if (k + 8 <= n && !((uintptr_t)d & 15)) {
+            float4 a = *(float4 *)d, b = *(float4 *)(d + 4);
+            a.x = a.x * p.decay - p.lr * v[0]; a.y = a.y * p.decay - p.lr * v[1];
+            a.z = a.z * p.decay - p.lr * v[2]; a.w = a.w * p.decay - p.lr * v[3];
+            b.x = b.x * p.decay - p.lr * v[4]; b.y = b.y * p.decay - p.lr * v[5];
+            b.z = b.z * p.decay - p.lr * v[6]; b.w = b.w * p.decay - p.lr * v[7];
+            *(float4 *)d = a;
+            *(float4 *)(d + 4) = b;
+            return;
         }
-        const bool tall = p.rows > p.cols;
-        for (int e = t; e < 64 * 128; e += 256) {
-            int i, j;
-            if (tall) { i = e & 63; j = e >> 6; } else { j = e & 127; i = e >> 7; }
-            if (r0 + i >= m || j0 + j >= n) continue;
-            const int64_t at = tall ? (int64_t)(j0 + j) * p.os + r0 + i : (int64_t)(r0 + i) * p.os + j0 + j;
-            const float v = slab[i * ORTHO_PITCH + j];
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+            if (k + q < n) d[q] = d[q] * p.decay - p.lr * v[q];
+        return;
+    }
+    T *d = (T *)p.out + at;
+    typedef T t4 __attribute__((ext_vector_type(4)));
+    if (k + 8 <= n && !((uintptr_t)d & (4 * sizeof(T) - 1))) {
+        t4 a, b;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) { a[q] = (T)v[q]; b[q] = (T)v[4 + q]; }
+        *(t4 *)d = a;
+        *(t4 *)(d + 4) = b;
+        return;
+    }
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+        if (k + q < n) d[q] = (T)v[q];
+}
+
+// One 32 (n, from k0) x 32 (m, from r0) block of (P X)^T held by a wave: the result in T (or the weights' update).
+template <typename T>
+__device__ __forceinline__ void ortho_result_block(const OrthoProb &p, const f32x16 &acc, int k0, int r0, int m, int n,
+                                                   float unscale) {
+    const int lane = threadIdx.x & 63, row = r0 + (lane & 31);
+    if (p.rows > p.cols) {                         // out[n][m]: lanes along its rows
+        if (row >= m) return;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int k = k0 + nt_acc_row(r, lane);
+            if (k >= n) continue;
+            const int64_t at = (int64_t)k * p.os + row;
+            const float v = acc[r] * unscale;
             if (p.buf) {
                 float *d = (float *)p.out + at;
                 *d = *d * p.decay - p.lr * v;
@@ -439,144 +522,493 @@ __global__ __launch_bounds__(256, 2) void ortho_apply_kernel(OrthoTable tab, int
                 ((T *)p.out)[at] = (T)v;
             }
         }
+        return;
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        float v[8];
+        nt_acc_rows8(acc, h, v);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] *= unscale;
+        const int k = k0 + 16 * h + 8 * (lane >> 5);
+        if (row < m && k < n) ortho_result8<T>(p, row, k, n, v);
+    }
+}
+
+// LAST: the result instead of the next step's X.
+template <typename T, typename S, bool LAST>
+__global__ __launch_bounds__(S::THREADS, S::THREADS == 256 ? 2 : 1) void ortho_apply_kernel(OrthoTable tab, int ntiles,
+                                                                                            int step, OrthoRule rule) {
+    __shared__ __attribute__((aligned(128))) char smem[S::LDS];
+    const OrthoTile w = tab.apply[nt_xcd_runs(blockIdx.x, ntiles)];
+    const OrthoProb p = tab.prob[w.prob];
+    const OrthoOperands o = ortho_operands(p, tab.ws, step);
+    const int m = ortho_m(p), n = ortho_n(p);
+    const int i0 = (w.ij >> 16) * S::TB, j0 = (w.ij & 0xffff) * S::TA;
+    const int64_t rx = ortho_row_bytes(n), rp = ortho_row_bytes(m);
+    const int groups = (n + 31) / 32;
+    f32x16 acc[S::FA][S::FB];
+    nt_tile<S, f16x8, NT_SPLIT2, true>(o.x + (j0 / 32) * 128, rx, groups - j0 / 32, m, o.p + i0 * rp, rp, m - i0, 0,
+                                       (m + 31) / 32, smem, acc);
+    if (LAST && p.buf) {
+        const double sq = rule.sqnorm[0];
+        if (!(sq >= 0.0 && sq < INFINITY)) return;
+    }
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int k0 = j0 + S::TA / S::WR * (wave / S::WC), r0 = i0 + S::TB / S::WC * (wave % S::WC);
+    const float unscale = ORTHO_UNSCALE * ORTHO_UNSCALE * ortho_shift(p.shift, step, -1) *
+                          (LAST ? 1.f : ortho_shift(p.shift, step + 1, 1));
+#pragma unroll
+    for (int j = 0; j < S::FB; ++j)
+#pragma unroll
+        for (int i = 0; i < S::FA; ++i) {
+            if (LAST) {
+                ortho_result_block<T>(p, acc[i][j], k0 + 32 * i, r0 + 32 * j, m, n, unscale);
+                continue;
+            }
+            const int row = r0 + 32 * j + (lane & 31);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float v[8];
+                nt_acc_rows8(acc[i][j], h, v);
+#pragma unroll
+                for (int q = 0; q < 8; ++q) v[q] *= unscale;
+                const int k = k0 + 32 * i + 16 * h + 8 * (lane >> 5);
+                if (row < m && k < groups * 32) ortho_store8(ortho_at(o.next, rx, row, k), v);
+            }
+        }
+}
+
+// ------------------------------------------------------------------------------------------------ one launch
+// A matrix whose shorter side is at most 32 (MB = 1) or 64 (MB = 2) and whose parts of X fit 144 KB of LDS, by one
+// workgroup of eight waves.  X rows of G groups of 128 B; S: 16 KB for the joined sums of the Gram matrix, then A, then P
+// (rows of MB groups).  16-byte chunks are XORed with bits of the row (f) so that both ways of reading -- sixteen rows of
+// one chunk, four rows of four chunks -- meet at most two lanes on a bank.
+//   Gram: wave (block, part of the contraction); the parts meet in S; the block's sums stay in registers for b A.
+//   Apply: a wave takes a group of 32 columns, reads all of its X, and writes P X in its place.
+#define SMALL_X 147456
+#define SMALL_S 16384
+__host__ __device__ static inline bool ortho_small(int m, int n) {
+    return m <= 64 && (int64_t)(m <= 32 ? 32 : 64) * ortho_row_bytes(n) <= SMALL_X;
+}
+__device__ __forceinline__ int small_swizzle(int row, int c) { return c ^ (((row & 1) << 2) | ((row >> 1) & 3)); }
+// byte of chunk c (0 ... 7; part 1 from 4 on) of group g of row `row`
+__device__ __forceinline__ int small_at(int row, int pitch, int g, int c) {
+    return row * pitch + g * 128 + small_swizzle(row, c) * 16;
+}
+__device__ __forceinline__ f32x16 small_products(const f16x8 *a, const f16x8 *b, f32x16 acc) {
+    acc = nt_mfma<f16x8>(a[1], b[0], acc);
+    acc = nt_mfma<f16x8>(a[0], b[1], acc);
+    return nt_mfma<f16x8>(a[0], b[0], acc);
+}
+
+template <typename T, int MB>
+__global__ __launch_bounds__(512) void ortho_small_kernel(OrthoBatch batch, OrthoRule rule, int steps, float eps) {
+    __shared__ __attribute__((aligned(128))) char smem[SMALL_X + SMALL_S];
+    constexpr int MP = 32 * MB, CUTS = MB == 2 ? 2 : 4, SP = MB * 128;      // contraction cuts, pitch of S
+    char *lx = smem, *ls = smem + SMALL_X;
+    const OrthoProb p = batch.p[blockIdx.x];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const int m = ortho_m(p), n = ortho_n(p), groups = (n + 31) / 32, pitch = groups * 128;
+    const bool tall = p.rows > p.cols;
+    float cf = 1.f;
+    bool apply = true;
+    if (p.buf) apply = ortho_clip(rule, cf);
+    // ---- u (and the momentum) and its norm: a thread holds up to nine runs of eight neighbours along n
+    constexpr int RUNS = SMALL_X / 4 / 8 / 512;
+    float u[RUNS][8];
+    double sum = 0.0;
+    auto place = [&](int e, int &i, int &k8) {     // lanes run along G's rows
+        if (tall) { i = e % MP; k8 = e / MP; } else { k8 = e % (groups * 4); i = e / (groups * 4); }
+    };
+#pragma unroll
+    for (int s = 0; s < RUNS; ++s) {
+        int i, k8;
+        place(t + 512 * s, i, k8);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+            const int k = k8 * 8 + q;
+            u[s][q] = i < m && k < n ? ortho_load<T>(p.g, tall ? (int64_t)k * p.gs + i : (int64_t)i * p.gs + k) : 0.f;
+        }
+    }
+    if (p.buf) {
+#pragma unroll
+        for (int s = 0; s < RUNS; ++s) {
+            int i, k8;
+            place(t + 512 * s, i, k8);
+            float b[8];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                const int k = k8 * 8 + q;
+                b[q] = i < m && k < n ? p.buf[tall ? (int64_t)k * p.cols + i : (int64_t)i * p.cols + k] : 0.f;
+            }
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                const int k = k8 * 8 + q;
+                u[s][q] = ortho_momentum(rule, u[s][q], cf, b[q]);
+                if (apply && i < m && k < n) p.buf[tall ? (int64_t)k * p.cols + i : (int64_t)i * p.cols + k] = b[q];
+            }
+        }
+    }
+#pragma unroll
+    for (int s = 0; s < RUNS; ++s)
+#pragma unroll
+        for (int q = 0; q < 8; ++q) sum += (double)u[s][q] * u[s][q];
+    int shift;
+    const float inv = ortho_inverse(ortho_block_sum(sum, (double *)ls), eps, shift);
+    const float up = ldexpf(1.f, shift);
+    // ---- X
+#pragma unroll
+    for (int s = 0; s < RUNS; ++s) {
+        int i, k8;
+        place(t + 512 * s, i, k8);
+        if (t + 512 * s >= MP * groups * 4) continue;
+        float v[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] = u[s][q] * up * inv;
+        f16x8 h0, h1;
+        ortho_parts8(v, h0, h1);
+        *(f16x8 *)(lx + small_at(i, pitch, k8 >> 2, k8 & 3)) = h0;
+        *(f16x8 *)(lx + small_at(i, pitch, k8 >> 2, 4 + (k8 & 3))) = h1;
+    }
+    __syncthreads();
+    const int frow = lane & 31, fhalf = lane >> 5;
+    const int blk = wave % (MB * MB), cut = wave / (MB * MB), bi = blk / MB, bj = blk % MB;
+    const float un2 = ORTHO_UNSCALE * ORTHO_UNSCALE;
+    for (int step = 0; step < steps; ++step) {
+        // ---- A = X X^T: block (bi, bj), groups of this cut
+        f32x16 ga, gb;                             // (two sums: a product waits for the one before it in its own only)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) ga[r] = gb[r] = 0.f;
+        if (cut < CUTS) {
+            for (int g = groups * cut / CUTS; g < groups * (cut + 1) / CUTS; ++g)
+#pragma unroll
+                for (int kk = 0; kk < 2; ++kk) {
+                    f16x8 fa[2], fb[2];
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        fa[q] = *(const f16x8 *)(lx + small_at(32 * bi + frow, pitch, g, 4 * q + 2 * kk + fhalf));
+                        fb[q] = *(const f16x8 *)(lx + small_at(32 * bj + frow, pitch, g, 4 * q + 2 * kk + fhalf));
+                    }
+                    if (kk == 0) ga = small_products(fa, fb, ga);
+                    else gb = small_products(fa, fb, gb);
+                }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) ga[r] += gb[r];
+            if (cut > 0) {
+                float *d = (float *)ls + ((cut - 1) * MB * MB + blk) * 1024 + lane;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) d[r * 64] = ga[r];
+            }
+        }
+        __syncthreads();
+        if (cut == 0) {
+#pragma unroll
+            for (int c = 1; c < CUTS; ++c) {
+                const float *s = (const float *)ls + ((c - 1) * MB * MB + blk) * 1024 + lane;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) ga[r] += s[r * 64];
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) ga[r] *= un2;      // A 4^h
+        }
+        __syncthreads();
+        // a block is symmetric to its mirror image: eight neighbours of column lane & 31 are eight neighbours of that row
+        auto store_block = [&](const f32x16 &b) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float v[8];
+                nt_acc_rows8(b, h, v);
+                f16x8 h0, h1;
+                ortho_parts8(v, h0, h1);
+                const int row = 32 * bj + frow, c = 2 * h + fhalf;
+                *(f16x8 *)(ls + small_at(row, SP, bi, c)) = h0;
+                *(f16x8 *)(ls + small_at(row, SP, bi, 4 + c)) = h1;
+            }
+        };
+        if (cut == 0) store_block(ga);
+        __syncthreads();
+        // ---- P = a I + b A + c A^2
+        const float down = ortho_shift(shift, step, -1), down2 = down * down;
+        f32x16 pa;
+        if (cut == 0) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) pa[r] = 0.f;
+#pragma unroll
+            for (int g = 0; g < MB; ++g)
+#pragma unroll
+                for (int kk = 0; kk < 2; ++kk) {
+                    f16x8 fa[2], fb[2];
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        fa[q] = *(const f16x8 *)(ls + small_at(32 * bi + frow, SP, g, 4 * q + 2 * kk + fhalf));
+                        fb[q] = *(const f16x8 *)(ls + small_at(32 * bj + frow, SP, g, 4 * q + 2 * kk + fhalf));
+                    }
+                    pa = small_products(fa, fb, pa);
+                }
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                pa[r] = ORTHO_C * (down2 * down2) * un2 * pa[r] + ORTHO_B * down2 * ga[r] +
+                        (32 * bi + nt_acc_row(r, lane) == 32 * bj + frow ? ORTHO_A : 0.f);
+        }
+        __syncthreads();
+        if (cut == 0) store_block(pa);
+        __syncthreads();
+        // ---- X <- P X, as (P X)^T: rows n of group g, columns m
+        const bool last = step + 1 == steps;
+        const float unscale = un2 * down * (last ? 1.f : ortho_shift(shift, step + 1, 1));
+        f16x8 fp[MB][MB][2][2];                    // P's rows: [block of m][k group][kk][part]
+#pragma unroll
+        for (int b = 0; b < MB; ++b)
+#pragma unroll
+            for (int kg = 0; kg < MB; ++kg)
+#pragma unroll
+                for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+                    for (int q = 0; q < 2; ++q)
+                        fp[b][kg][kk][q] = *(const f16x8 *)(ls + small_at(32 * b + frow, SP, kg, 4 * q + 2 * kk + fhalf));
+        for (int g = wave; g < groups; g += 8) {
+            f16x8 fx[MB][2][2];                    // [k group][kk][part]
+#pragma unroll
+            for (int kg = 0; kg < MB; ++kg)
+#pragma unroll
+                for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        union { s16x4 h[2]; f16x8 v; } u;
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const int k = 32 * kg + 16 * kk + 8 * fhalf + 4 * e + ((lane >> 2) & 3);
+                            const char *at2 = lx + small_at(k, pitch, g, 4 * q + 2 * (frow >> 4) + ((lane & 3) >> 1)) +
+                                              (lane & 1) * 8;
+                            u.h[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)at2);
+                        }
+                        fx[kg][kk][q] = u.v;
+                    }
+            f32x16 y[MB];
+#pragma unroll
+            for (int b = 0; b < MB; ++b) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) y[b][r] = 0.f;
+#pragma unroll
+                for (int kg = 0; kg < MB; ++kg)
+#pragma unroll
+                    for (int kk = 0; kk < 2; ++kk) y[b] = small_products(fx[kg][kk], fp[b][kg][kk], y[b]);
+            }
+            if (last) {
+                if (apply)
+#pragma unroll
+                    for (int b = 0; b < MB; ++b) ortho_result_block<T>(p, y[b], 32 * g, 32 * b, m, n, unscale);
+                continue;
+            }
+#pragma unroll
+            for (int b = 0; b < MB; ++b)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float v[8];
+                    nt_acc_rows8(y[b], h, v);
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) v[q] *= unscale;
+                    f16x8 h0, h1;
+                    ortho_parts8(v, h0, h1);
+                    const int row = 32 * b + frow, c = 2 * h + fhalf;
+                    *(f16x8 *)(lx + small_at(row, pitch, g, c)) = h0;
+                    *(f16x8 *)(lx + small_at(row, pitch, g, 4 + c)) = h1;
+                }
+        }
+        __syncthreads();
     }
 }
 
 // ------------------------------------------------------------------------------------------------ host side
-// Positions of everything in the workspace: a pure function of the shapes.
+// Everything about a call that follows from its shapes.
 struct OrthoPlan {
-    int64_t prob, sym, gram, apply, part, slab, operands, bytes;
-    int nsym, ngram, napply, nparts, max_parts, joined;
+    int64_t prob, split, sym, gram, poly, apply, part, slab, operands, bytes;
+    int nsplit, nsym, ngram, npoly, napply, nparts, cut, poly_tile, apply_tile, empty;
+    bool joined, small;
 };
 
 static inline int64_t ortho_align(int64_t v) { return (v + 255) & ~(int64_t)255; }
 
-// Cuts of the Gram contraction: enough work items that a launch over all matrices gives every CU its two workgroups, but
-// no cut shorter than 8 k-steps (below that its partial tile costs more to write and add than it saves).
-static inline int ortho_cut_groups(int64_t tile_groups) {
-    const int64_t g = (tile_groups + 511) / 512;
-    return g < 8 ? 8 : (g > (1 << 20) ? 1 << 20 : (int)g);
+template <typename D>
+static void ortho_sides(const D &d, int64_t &m, int64_t &n) {
+    m = d.rows < d.cols ? d.rows : d.cols;
+    n = d.rows < d.cols ? d.cols : d.rows;
+}
+
+// Cuts of the Gram contraction.  With W k-steps in all and two workgroups per CU the launch takes about
+// (W + 8 items) / 512 + cut / 2 k-steps: an item costs about eight more (its epilogue, or its partial tile and the join),
+// and the last ones end half a cut apart.  The power of two times 8 or 12 that makes this least.
+template <typename D>
+static int64_t ortho_gram_cut(const D *d, int n) {
+    int64_t best = 8, least = INT64_MAX;
+    for (int64_t c = 8; c <= (1 << 18); c += (c & (c - 1)) ? c / 3 : c / 2) {
+        int64_t steps = 0, items = 0, longest = 0;
+        for (int i = 0; i < n; ++i) {
+            int64_t m, k;
+            ortho_sides(d[i], m, k);
+            const int64_t t = (m + GRAM_TILE - 1) / GRAM_TILE, tiles = t * (t + 1) / 2, g = (k + 31) / 32;
+            steps += tiles * g;
+            items += tiles * ((g + c - 1) / c);
+            if (g > longest) longest = g;
+        }
+        const int64_t cost = (steps + 8 * items) + 256 * (c < longest ? c : longest);
+        if (cost < least) { least = cost; best = c; }
+        if (c >= longest) break;
+    }
+    return best;
 }
 
 template <typename D>
 static int ortho_plan(const D *d, int n, OrthoPlan &pl) {
-    int64_t tile_groups = 0;
+    pl = OrthoPlan();
+    pl.small = true;
+    int64_t poly128 = 0, apply256 = 0, live = 0;
     for (int i = 0; i < n; ++i) {
         if (d[i].rows < 0 || d[i].cols < 0 || d[i].rows > (1 << 22) || d[i].cols > (1 << 22)) return SLN_ERR_INVALID_ARG;
-        const int64_t m = d[i].rows < d[i].cols ? d[i].rows : d[i].cols, k = d[i].rows < d[i].cols ? d[i].cols : d[i].rows;
+        int64_t m, k;
+        ortho_sides(d[i], m, k);
         if (m > 65535) return SLN_ERR_UNSUPPORTED;
-        const int64_t tm = (m + NT_TILE - 1) / NT_TILE;
-        tile_groups += tm * (tm + 1) / 2 * ((k + 31) / 32);
+        if (m == 0) continue;
+        ++live;
+        pl.small = pl.small && ortho_small((int)m, (int)k);
+        const int64_t t = (m + 127) / 128;
+        poly128 += t * (t + 1) / 2;
+        apply256 += ((m + 255) / 256) * ((k + 255) / 256);
     }
-    const int cut = ortho_cut_groups(tile_groups);
-    int64_t nsym = 0, ngram = 0, napply = 0, nparts = 0, max_parts = 0, operands = 0, nprob = 0;
-    bool joined = false;
+    pl.empty = live == 0;
+    if (pl.empty || pl.small) return SLN_OK;
+    pl.cut = (int)ortho_gram_cut(d, n);
+    // Tiles: large ones where they fill the chip, else smaller ones (the polynomial's product is short: what counts
+    // is how many CUs take part).
+    pl.poly_tile = poly128 >= 4096 ? 128 : 64;
+    pl.apply_tile = apply256 >= 192 ? 256 : 128;
+    int64_t nsplit = 0, nsym = 0, ngram = 0, npoly = 0, napply = 0, nparts = 0, operands = 0;
     for (int i = 0; i < n; ++i) {
         if (d[i].rows == 0 || d[i].cols == 0) continue;
         OrthoProb p = {};
         p.rows = d[i].rows; p.cols = d[i].cols;
         const int64_t m = ortho_m(p), k = ortho_n(p);
-        const int64_t tm = (m + NT_TILE - 1) / NT_TILE, tn = (k + NT_TILE - 1) / NT_TILE;
-        const int64_t groups = (k + 31) / 32, nsplit = (groups + cut - 1) / cut;
-        joined |= nsplit > 1;
-        ++nprob;
+        const int64_t tm = (m + GRAM_TILE - 1) / GRAM_TILE, cuts = ((k + 31) / 32 + pl.cut - 1) / pl.cut;
+        const int64_t tp = (m + pl.poly_tile - 1) / pl.poly_tile;
+        pl.joined |= cuts > 1;
+        nsplit += ((m + 63) / 64) * ((k + 127) / 128);
         nsym += tm * (tm + 1) / 2;
-        ngram += tm * (tm + 1) / 2 * nsplit;
-        napply += tm * tn;
-        const int64_t parts = ((int64_t)p.rows * p.cols + ORTHO_CHUNK - 1) / ORTHO_CHUNK;
-        nparts += parts;
-        if (parts > max_parts) max_parts = parts;
+        ngram += tm * (tm + 1) / 2 * cuts;
+        npoly += tp * (tp + 1) / 2;
+        napply += ((m + pl.apply_tile - 1) / pl.apply_tile) * ((k + pl.apply_tile - 1) / pl.apply_tile);
+        nparts += ((int64_t)p.rows * p.cols + ORTHO_CHUNK - 1) / ORTHO_CHUNK;
         operands += ortho_align(ortho_operand_bytes(p));
-        if (tn > 65535 || nsym > (1 << 28) || ngram > (1 << 28) || napply > (1 << 28) || nparts > (1 << 28) ||
-            max_parts > (1 << 24))
-            return SLN_ERR_UNSUPPORTED;
+        const int64_t most = 1 << 28;
+        if (nsplit > most || ngram > most || npoly > most || napply > most || nparts > most) return SLN_ERR_UNSUPPORTED;
     }
     int64_t at = 0;
-    pl.prob = at; at += ortho_align(nprob * (int64_t)sizeof(OrthoProb));
+    pl.prob = at; at += ortho_align(live * (int64_t)sizeof(OrthoProb));
+    pl.split = at; at += ortho_align(nsplit * (int64_t)sizeof(OrthoTile));
     pl.sym = at; at += ortho_align(nsym * (int64_t)sizeof(OrthoTile));
     pl.gram = at; at += ortho_align(ngram * (int64_t)sizeof(OrthoTile));
+    pl.poly = at; at += ortho_align(npoly * (int64_t)sizeof(OrthoTile));
     pl.apply = at; at += ortho_align(napply * (int64_t)sizeof(OrthoTile));
     pl.part = at; at += ortho_align(nparts * (int64_t)sizeof(double));
-    pl.slab = at; at += joined ? ortho_align(ngram * (int64_t)(NT_TILE * NT_TILE * 4)) : 0;
+    pl.slab = at; at += pl.joined ? ortho_align(ngram * (int64_t)(GRAM_TILE * GRAM_TILE * 4)) : 0;
     pl.operands = at; at += operands;
     pl.bytes = at;
-    pl.nsym = (int)nsym; pl.ngram = (int)ngram; pl.napply = (int)napply;
-    pl.nparts = (int)nparts; pl.max_parts = (int)max_parts; pl.joined = joined;
+    pl.nsplit = (int)nsplit; pl.nsym = (int)nsym; pl.ngram = (int)ngram; pl.npoly = (int)npoly; pl.napply = (int)napply;
+    pl.nparts = (int)nparts;
     return SLN_OK;
 }
 
-struct OrthoStep { const double *sqnorm; float max_norm, momentum; int nesterov; };
-
 static void ortho_desc(const sln_ortho_desc_t &d, OrthoProb &p) {
-    p.g = d.g; p.out = d.out; p.buf = nullptr;
+    p = OrthoProb();
+    p.g = d.g; p.out = d.out;
     p.gs = d.g_stride; p.os = d.out_stride;
-    p.lr = 0.f; p.decay = 1.f;
+    p.rows = d.rows; p.cols = d.cols;
+    p.decay = 1.f;
 }
 static void ortho_desc(const sln_muon_desc_t &d, OrthoProb &p) {
+    p = OrthoProb();
     p.g = d.grad; p.out = d.param; p.buf = d.momentum;
     p.gs = p.os = d.cols;
+    p.rows = d.rows; p.cols = d.cols;
     p.lr = d.lr; p.decay = d.decay;
 }
 
+template <typename T, typename D, int MB>
+static void ortho_run_small(const D *d, int n, int steps, float eps, const OrthoRule &rule, hipStream_t stream) {
+    OrthoBatch batch;
+    int inb = 0;
+    for (int i = 0; i < n; ++i) {
+        int64_t m, k;
+        ortho_sides(d[i], m, k);
+        if (m > 0 && (m <= 32) == (MB == 1)) ortho_desc(d[i], batch.p[inb++]);
+        if (inb == ORTHO_BATCH || (inb > 0 && i + 1 == n)) {
+            hipLaunchKernelGGL((ortho_small_kernel<T, MB>), dim3(inb), dim3(512), 0, stream, batch, rule, steps, eps);
+            inb = 0;
+        }
+    }
+}
+
+template <typename T, typename S>
+static void ortho_apply(const OrthoTable &tab, int napply, int step, bool last, const OrthoRule &rule, hipStream_t stream) {
+    if (last)
+        hipLaunchKernelGGL((ortho_apply_kernel<T, S, true>), dim3(napply), dim3(S::THREADS), 0, stream, tab, napply, step, rule);
+    else
+        hipLaunchKernelGGL((ortho_apply_kernel<T, S, false>), dim3(napply), dim3(S::THREADS), 0, stream, tab, napply, step,
+                           rule);
+}
+
 template <typename T, typename D>
-static int ortho_run(const D *d, int n, int steps, float eps, const OrthoStep &st, void *workspace, size_t ws_bytes,
+static int ortho_run(const D *d, int n, int steps, float eps, const OrthoRule &rule, void *workspace, size_t ws_bytes,
                      hipStream_t stream) {
     OrthoPlan pl;
     const int rc = ortho_plan(d, n, pl);
     if (rc != SLN_OK) return rc;
-    if (pl.napply == 0) return SLN_OK;
-    if (!workspace || ((uintptr_t)workspace & 255)) return SLN_ERR_INVALID_ARG;
+    if (pl.empty) return SLN_OK;
+    if (pl.bytes && (!workspace || ((uintptr_t)workspace & 255))) return SLN_ERR_INVALID_ARG;
     if (ws_bytes < (size_t)pl.bytes) return SLN_ERR_WORKSPACE;
-    char *ws = (char *)workspace;
-    const OrthoTable tab = {(OrthoProb *)(ws + pl.prob), (OrthoTile *)(ws + pl.sym), (OrthoTile *)(ws + pl.gram),
-                            (OrthoTile *)(ws + pl.apply), (double *)(ws + pl.part), ws, (float *)(ws + pl.slab)};
-    int64_t tile_groups = 0;
-    for (int i = 0; i < n; ++i) {
-        const int64_t m = d[i].rows < d[i].cols ? d[i].rows : d[i].cols, k = d[i].rows < d[i].cols ? d[i].cols : d[i].rows;
-        const int64_t tm = (m + NT_TILE - 1) / NT_TILE;
-        tile_groups += tm * (tm + 1) / 2 * ((k + 31) / 32);
-    }
-    const int cut = ortho_cut_groups(tile_groups);
     sln_enter();
+    if (pl.small) {
+        ortho_run_small<T, D, 1>(d, n, steps, eps, rule, stream);
+        ortho_run_small<T, D, 2>(d, n, steps, eps, rule, stream);
+        return sln_launch_status();
+    }
+    char *ws = (char *)workspace;
+    const OrthoTable tab = {(OrthoProb *)(ws + pl.prob), (OrthoTile *)(ws + pl.split), (OrthoTile *)(ws + pl.sym),
+                            (OrthoTile *)(ws + pl.gram), (OrthoTile *)(ws + pl.poly), (OrthoTile *)(ws + pl.apply),
+                            (double *)(ws + pl.part), ws, (float *)(ws + pl.slab), pl.poly_tile, pl.apply_tile};
     OrthoBatch batch;
-    int prob0 = 0, inb = 0, batch_parts = 1, part0 = 0, sym0 = 0, gram0 = 0, apply0 = 0;
+    int prob0 = 0, inb = 0, parts = 1, part0 = 0, split0 = 0, sym0 = 0, gram0 = 0, poly0 = 0, apply0 = 0;
     int64_t off = pl.operands;
-    auto flush = [&]() {
-        if (inb == 0) return;
-        hipLaunchKernelGGL((ortho_norm_kernel<T>), dim3(batch_parts, inb), dim3(256), 0, stream, batch, prob0, tab,
-                           st.sqnorm, st.max_norm, st.momentum, st.nesterov);
-        prob0 += inb; inb = 0; batch_parts = 1;
-    };
-    for (int i = 0; i < n; ++i) {
-        if (d[i].rows == 0 || d[i].cols == 0) continue;
-        OrthoProb &p = batch.p[inb];
+    for (int i = 0; i <= n; ++i) {
+        if (inb == ORTHO_BATCH || (inb > 0 && i == n)) {
+            hipLaunchKernelGGL((ortho_norm_kernel<T>), dim3(parts, inb), dim3(256), 0, stream, batch, prob0, tab, rule);
+            prob0 += inb; inb = 0; parts = 1;
+        }
+        if (i == n || d[i].rows == 0 || d[i].cols == 0) continue;
+        OrthoProb &p = batch.p[inb++];
         ortho_desc(d[i], p);
-        p.rows = d[i].rows; p.cols = d[i].cols;
         const int m = ortho_m(p), k = ortho_n(p);
-        const int tm = sln_div_up(m, NT_TILE), tn = sln_div_up(k, NT_TILE);
+        const int tm = ortho_tiles(m, GRAM_TILE), tp = ortho_tiles(m, pl.poly_tile);
         p.off = off; off += ortho_align(ortho_operand_bytes(p));
-        p.nsplit = ((k + 31) / 32 + cut - 1) / cut;
+        p.nsplit = ((k + 31) / 32 + pl.cut - 1) / pl.cut;
         p.part0 = part0; p.nparts = sln_div_up((long)p.rows * p.cols, ORTHO_CHUNK); part0 += p.nparts;
+        p.split0 = split0; split0 += ortho_tiles(m, 64) * ortho_tiles(k, 128);
         p.sym0 = sym0; sym0 += tm * (tm + 1) / 2;
         p.gram0 = gram0; gram0 += tm * (tm + 1) / 2 * p.nsplit;
-        p.apply0 = apply0; apply0 += tm * tn;
-        if (p.nparts > batch_parts) batch_parts = p.nparts;
-        if (++inb == ORTHO_BATCH) flush();
+        p.poly0 = poly0; poly0 += tp * (tp + 1) / 2;
+        p.apply0 = apply0; apply0 += ortho_tiles(m, pl.apply_tile) * ortho_tiles(k, pl.apply_tile);
+        if (p.nparts > parts) parts = p.nparts;
     }
-    flush();
-    hipLaunchKernelGGL((ortho_split_kernel<T>), dim3(pl.napply), dim3(256), 0, stream, tab, st.sqnorm, st.max_norm,
-                       st.momentum, st.nesterov, eps);
+    hipLaunchKernelGGL((ortho_split_kernel<T>), dim3(pl.nsplit), dim3(256), 0, stream, tab, rule, eps);
     for (int s = 0; s < steps; ++s) {
-        hipLaunchKernelGGL(ortho_gram_kernel, dim3(pl.ngram), dim3(256), 0, stream, tab, pl.ngram);
-        if (pl.joined) hipLaunchKernelGGL(ortho_join_kernel, dim3(2 * pl.nsym), dim3(256), 0, stream, tab);
-        hipLaunchKernelGGL(ortho_poly_kernel, dim3(pl.nsym), dim3(256), 0, stream, tab, pl.nsym, s, 3.4445f,
-                           -4.7750f, 2.0315f);
-        if (s + 1 < steps)
-            hipLaunchKernelGGL((ortho_apply_kernel<T, false>), dim3(pl.napply), dim3(256), 0, stream, tab, pl.napply, s,
-                               st.sqnorm);
+        hipLaunchKernelGGL(ortho_gram_kernel, dim3(pl.ngram), dim3(256), 0, stream, tab, s, pl.ngram);
+        if (pl.joined) hipLaunchKernelGGL(ortho_join_kernel, dim3(4 * pl.nsym), dim3(256), 0, stream, tab);
+        if (pl.poly_tile == 128)
+            hipLaunchKernelGGL((ortho_poly_kernel<OrthoGram>), dim3(pl.npoly), dim3(256), 0, stream, tab, pl.npoly, s);
         else
-            hipLaunchKernelGGL((ortho_apply_kernel<T, true>), dim3(pl.napply), dim3(256), 0, stream, tab, pl.napply, s,
-                               st.sqnorm);
+            hipLaunchKernelGGL((ortho_poly_kernel<OrthoPolySmall>), dim3(pl.npoly), dim3(256), 0, stream, tab, pl.npoly, s);
+        if (pl.apply_tile == 256) ortho_apply<T, OrthoApplyLarge>(tab, pl.napply, s, s + 1 == steps, rule, stream);
+        else ortho_apply<T, OrthoApplySmall>(tab, pl.napply, s, s + 1 == steps, rule, stream);
     }
     return sln_launch_status();
 }
@@ -595,12 +1027,12 @@ extern "C" int sln_orthogonalize(const sln_ortho_desc_t *descs, int n, int dtype
         if (d.rows == 0 || d.cols == 0) continue;
         if (!d.g || !d.out || d.g_stride < d.cols || d.out_stride < d.cols) return SLN_ERR_INVALID_ARG;
     }
-    const OrthoStep st = {nullptr, 0.f, 0.f, 0};
+    const OrthoRule rule = {nullptr, 0.f, 0.f, 0};
     hipStream_t s = (hipStream_t)stream;
     switch (dtype) {
-        case SLN_DTYPE_F32: return ortho_run<float>(descs, n, steps, eps, st, workspace, workspace_bytes, s);
-        case SLN_DTYPE_BF16: return ortho_run<__bf16>(descs, n, steps, eps, st, workspace, workspace_bytes, s);
-        case SLN_DTYPE_F16: return ortho_run<_Float16>(descs, n, steps, eps, st, workspace, workspace_bytes, s);
+        case SLN_DTYPE_F32: return ortho_run<float>(descs, n, steps, eps, rule, workspace, workspace_bytes, s);
+        case SLN_DTYPE_BF16: return ortho_run<__bf16>(descs, n, steps, eps, rule, workspace, workspace_bytes, s);
+        case SLN_DTYPE_F16: return ortho_run<_Float16>(descs, n, steps, eps, rule, workspace, workspace_bytes, s);
         default: return SLN_ERR_INVALID_ARG;
     }
 }
@@ -620,6 +1052,6 @@ extern "C" int sln_muon_step_f32(const sln_muon_desc_t *descs, int n, int steps,
         if (d.rows == 0 || d.cols == 0) continue;
         if (!d.grad || !d.param || !d.momentum) return SLN_ERR_INVALID_ARG;
     }
-    const OrthoStep st = {sqnorm, max_norm, momentum, nesterov};
-    return ortho_run<float>(descs, n, steps, eps, st, workspace, workspace_bytes, (hipStream_t)stream);
+    const OrthoRule rule = {sqnorm, max_norm, momentum, nesterov};
+    return ortho_run<float>(descs, n, steps, eps, rule, workspace, workspace_bytes, (hipStream_t)stream);
 }

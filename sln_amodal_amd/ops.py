@@ -425,6 +425,7 @@ def orthogonalize(x, steps=5, eps=1e-7):
         for b in range(src.shape[0] if src.dim() == 3 else 1):
             flat.append((base + b * step, o.data_ptr() + b * r * c * es, gs, c, r, c))
     if flat:
+        flat.sort(key=lambda d: -min(d[4], d[5]))            # (the longest products first: the launches end together)
         descs = (_OrthoDesc * len(flat))(*flat)
         L = _lib.lib()
         with torch.cuda.device(mats[0].device):

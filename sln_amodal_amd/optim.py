@@ -319,6 +319,7 @@ class ClippedMuon(ClippedSGD):
                     glr = float(g["lr"])
                     flat.append((p.data_ptr(), gs[k + i].data_ptr(), bs[k + i].data_ptr(), rows, cols,
                                  glr * max(1.0, rows / cols) ** 0.5 if cols else 0.0, 1.0 - glr * float(g["weight_decay"])))
+                flat.sort(key=lambda d: -min(d[3], d[4]))        # (the longest products first: the launches end together)
                 descs = (_MuonDesc * len(flat))(*flat)
                 nbytes = L.sln_muon_step_workspace_bytes(descs, len(flat))
                 ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=dev)

@@ -33,7 +33,9 @@ def test_entries_check_their_arguments():
     buf = (C.c_char * 4096)()
     p = (C.addressof(buf) + 255) // 256 * 256
     vp = C.c_void_p(p)
-    d = (_OrthoDesc * 2)((p, p, 8, 8, 4, 8), (0, 0, 0, 0, 0, 5))
+    small = (_OrthoDesc * 1)((p, p, 8, 8, 4, 8))
+    assert L.sln_orthogonalize_workspace_bytes(small, 1) == 0   # runs on one CU, without a workspace
+    d = (_OrthoDesc * 2)((p, p, 99, 99, 70, 99), (0, 0, 0, 0, 0, 5))
     need = L.sln_orthogonalize_workspace_bytes(d, 2)
     assert need > 0 and L.sln_orthogonalize_workspace_bytes(d, 0) == 0
     run = lambda descs, n, dtype=0, steps=5, eps=1e-7, ws=vp, nbytes=1 << 30: L.sln_orthogonalize(
@@ -49,12 +51,12 @@ def test_entries_check_their_arguments():
     assert run((_OrthoDesc * 1)((p, p, 8, 7, 4, 8)), 1) == 1
     assert run((_OrthoDesc * 1)((p, p, 70000, 70000, 70000, 70000)), 1) == 4
     assert run((_OrthoDesc * 1)((p, p, 8, 8, -4, 8)), 1) == 1
-    m = (_MuonDesc * 1)((p, p, p, 4, 8, 0.1, 1.0))
+    m = (_MuonDesc * 1)((p, p, p, 70, 80, 0.1, 1.0))
     need = L.sln_muon_step_workspace_bytes(m, 1)
     step = lambda descs, sq=vp, ws=vp, nbytes=1 << 30: L.sln_muon_step_f32(descs, 1, 5, 1e-7, sq, 5.0, 0.9, 1, ws, nbytes,
                                                                            None)
     assert step(m, sq=None) == 1 and step(m, ws=None) == 1 and step(m, nbytes=need - 1) == 2
-    assert step((_MuonDesc * 1)((p, 0, p, 4, 8, 0.1, 1.0))) == 1
+    assert step((_MuonDesc * 1)((p, 0, p, 70, 80, 0.1, 1.0))) == 1
 
 
 def test_wrong_calls_are_refused():

@@ -78,6 +78,22 @@ def test_many_matrices_in_one_call_equal_them_alone():
         _check(o.view(6, 48, 80)[i], stack.view(6, 48, 80)[i], torch.float32)
 
 
+def test_a_hundred_matrices_take_the_large_tiles():
+    from sln_amodal_amd import ops
+    gs = [_matrix(*((200, 300) if i % 2 else (300, 200)), seed=i) for i in range(100)]
+    outs = ops.orthogonalize([g.cuda() for g in gs])
+    for g, o in zip(gs, outs):
+        _check(o, g, torch.float32)
+
+
+@pytest.mark.parametrize("rows,cols", [(64, 576), (33, 577), (32, 1152), (20, 1000), (5, 1153), (63, 65), (32, 32), (1, 3000)])
+def test_matrices_that_fit_one_workgroup_and_just_do_not(rows, cols):
+    from sln_amodal_amd import ops
+    gs = [_matrix(rows, cols, 1), _matrix(cols, rows, 2), _matrix(rows, cols, 3) * 1e-12]
+    for o, g in zip(ops.orthogonalize([g.cuda() for g in gs]), gs):
+        _check(o, g, torch.float32)
+
+
 @pytest.mark.parametrize("steps", [1, 2, 7])
 def test_steps(steps):
     from sln_amodal_amd import ops
