@@ -17,7 +17,8 @@
 //   per step: ortho_gram_kernel    A's 128 x 128 tiles on and above the diagonal (A is symmetric), the contraction over n
 //                                  cut so that one round of workgroups fills the chip; one cut: parts of A are written
 //                                  (both triangles), several: fp32 partial tiles, added in order by ortho_join_kernel
-//             ortho_poly_kernel    P's tiles on and above the diagonal from A A^T, parts of both triangles
+//             ortho_poly_kernel    P's 64 x 64 tiles on and above the diagonal from A A^T, parts of both triangles
+//             (both by ortho_square_kernel in calls with little to do)
 //             ortho_apply_kernel   X <- P X; the last step writes the result, or updates the weights.
 // X is kept one way only, rows of n.  The Gram matrix contracts along its rows; P X contracts across them and computes
 // (P X)^T with X as the first operand, read through LDS's transposing loads: the 16 accumulator values of a lane are then
@@ -35,8 +36,8 @@
 #define ORTHO_C 2.0315f
 #define GRAM_TILE 128
 
-typedef NtShape<2, 2, 128, 128, 2, 2, 2> OrthoGram;        // and the polynomial's large tile
-typedef NtShape<2, 2, 64, 64, 2, 2, 4> OrthoPolySmall;
+typedef NtShape<2, 2, 128, 128, 2, 2, 2> OrthoGram;
+typedef NtShape<2, 2, 64, 64, 2, 2, 4> OrthoSquare;
 typedef NtShape<2, 2, 128, 128, 2, 2, 2> OrthoApplySmall;
 typedef NtShape<2, 2, 256, 256, 2, 4, 2> OrthoApplyLarge;
 
@@ -48,7 +49,7 @@ struct OrthoProb {
     int64_t gs, os, off;   // off: byte offset of this matrix's operands in the workspace
     int32_t rows, cols;
     int32_t part0, nparts; // its partial sums of squares
-    int32_t split0, sym0, gram0, poly0, apply0, nsplit;    // first entries in the work lists, cuts of the contraction
+    int32_t split0, sym0, gram0, square0, apply0, nsplit;    // first entries in the work lists, cuts of the contraction
     float lr, decay;       // update: p = p * decay - lr * X
     int32_t shift;         // h of the first step (ortho_split_kernel)
 };
@@ -57,11 +58,11 @@ struct OrthoTile { int32_t prob, ij, first, cut; };        // ij = row tile << 1
 
 struct OrthoTable {
     OrthoProb *prob;
-    OrthoTile *split, *sym, *gram, *poly, *apply;
+    OrthoTile *split, *sym, *gram, *square, *apply;
     double *part;
     char *ws;
     float *slab;           // partial Gram tiles, GRAM_TILE^2 floats per gram entry
-    int poly_tile, apply_tile;
+    int apply_tile;
 };
 
 struct OrthoBatch { OrthoProb p[ORTHO_BATCH]; };
@@ -150,7 +151,7 @@ __device__ __forceinline__ void ortho_lists(const OrthoProb &p, int prob, const 
         tab.split[p.split0 + e] = w;
     }
     const int tm = ortho_tiles(m, GRAM_TILE), nsym = tm * (tm + 1) / 2;
-    for (int e = t; e < tm * tm; e += 256) {
+    for (int e = t; p.nsplit > 0 && e < tm * tm; e += 256) {
         const int i = e / tm, j = e - i * tm;
         if (j < i) continue;
         const int s = i * tm - i * (i - 1) / 2 + (j - i);
@@ -161,12 +162,12 @@ __device__ __forceinline__ void ortho_lists(const OrthoProb &p, int prob, const 
             tab.gram[p.gram0 + k * nsym + s] = w;
         }
     }
-    const int tp = ortho_tiles(m, tab.poly_tile);
-    for (int e = t; e < tp * tp; e += 256) {
+    const int tp = ortho_tiles(m, OrthoSquare::TA);
+    for (int e = t; e < tp * tp; e += 256) {       // the whole square, or its upper triangle
         const int i = e / tp, j = e - i * tp;
-        if (j < i) continue;
+        if (p.nsplit > 0 && j < i) continue;
         const OrthoTile w = {prob, i << 16 | j, 0, 0};
-        tab.poly[p.poly0 + i * tp - i * (i - 1) / 2 + (j - i)] = w;
+        tab.square[p.square0 + (p.nsplit > 0 ? i * tp - i * (i - 1) / 2 + (j - i) : e)] = w;
     }
     const int ti = ortho_tiles(m, tab.apply_tile), tj = ortho_tiles(n, tab.apply_tile);
     for (int e = t; e < ti * tj; e += 256) {       // the m tiles of one column of X run side by side
@@ -201,7 +202,17 @@ __global__ __launch_bounds__(256) void ortho_norm_kernel(OrthoBatch batch, int p
         }
         acc += (double)u * u;
     };
-    if (flat && sizeof(T) == 4 && !(((uintptr_t)p.g | (uintptr_t)p.buf) & 15)) {
+    if (flat && sizeof(T) == 2 && !((uintptr_t)p.g & 15)) {          // (never the optimiser's)
+        typedef T t8 __attribute__((ext_vector_type(8)));
+        const t8 *g8 = (const t8 *)p.g + (e0 >> 3);
+        const int n8 = (int)((e1 - e0) >> 3);
+        for (int i = t; i < n8; i += 256) {
+            const t8 g = g8[i];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) one((float)g[q], nullptr);
+        }
+        for (int64_t e = e0 + (int64_t)n8 * 8 + t; e < e1; e += 256) one(ortho_load<T>(p.g, e), nullptr);
+    } else if (flat && sizeof(T) == 4 && !(((uintptr_t)p.g | (uintptr_t)p.buf) & 15)) {
         const float4 *g4 = (const float4 *)p.g + (e0 >> 2);
         const int n4 = (int)((e1 - e0) >> 2);
         for (int i = t; i < n4; i += 256) {
@@ -296,7 +307,12 @@ __global__ __launch_bounds__(256) void ortho_split_kernel(OrthoTable tab, OrthoR
             float g[8], b[8];
             const bool wide = sizeof(T) == 4 && k + 8 <= n && !(((uintptr_t)((const float *)p.g + at)) & 15) &&
                               !(p.buf && ((uintptr_t)(p.buf + bt) & 15));
-            if (wide) {
+            typedef T t8 __attribute__((ext_vector_type(8)));
+            if (sizeof(T) == 2 && k + 8 <= n && !(((uintptr_t)((const T *)p.g + at)) & 15)) {
+                const t8 a = *(const t8 *)((const T *)p.g + at);
+#pragma unroll
+                for (int q = 0; q < 8; ++q) { g[q] = (float)a[q]; b[q] = 0.f; }
+            } else if (wide) {
                 *(float4 *)g = *(const float4 *)((const float *)p.g + at);
                 *(float4 *)(g + 4) = *(const float4 *)((const float *)p.g + at + 4);
                 if (p.buf) {
@@ -426,12 +442,12 @@ __global__ __launch_bounds__(256) void ortho_join_kernel(OrthoTable tab) {
 }
 
 // ------------------------------------------------------------------------------------------------ P = a I + b A + c A^2
-template <typename S>
 __global__ __launch_bounds__(256, 2) void ortho_poly_kernel(OrthoTable tab, int ntiles, int step) {
+    typedef OrthoSquare S;
     constexpr int TILE = S::TA, R = TILE / 2;
     __shared__ __attribute__((aligned(128))) char smem[S::LDS];
     static_assert(R * (TILE + 5) * 4 <= S::LDS, "epilogue slab must fit the operand stages");
-    const OrthoTile w = tab.poly[nt_xcd_runs(blockIdx.x, ntiles)];
+    const OrthoTile w = tab.square[nt_xcd_runs(blockIdx.x, ntiles)];
     const OrthoProb p = tab.prob[w.prob];
     const OrthoOperands o = ortho_operands(p, tab.ws, step);
     const int m = ortho_m(p);
@@ -465,73 +481,128 @@ __global__ __launch_bounds__(256, 2) void ortho_poly_kernel(OrthoTable tab, int 
     }
 }
 
-// ------------------------------------------------------------------------------------------------ X <- P X
-// Eight neighbours along n (columns k ... k + 7, of which n - k exist) of row `row` of the result.
-template <typename T>
-__device__ __forceinline__ void ortho_result8(const OrthoProb &p, int row, int k, int n, const float *v) {
-    const int64_t at = (int64_t)row * p.os + k;
-    if (p.buf) {
-        float *d = (float *)p.out + at;
-        if (k + 8 <= n && !((uintptr_t)d & 15)) {
-            float4 a = *(float4 *)d, b = *(float4 *)(d + 4);
-            a.x = a.x * p.decay - p.lr * v[0]; a.y = a.y * p.decay - p.lr * v[1];
-            a.z = a.z * p.decay - p.lr * v[2]; a.w = a.w * p.decay - p.lr * v[3];
-            b.x = b.x * p.decay - p.lr * v[4]; b.y = b.y * p.decay - p.lr * v[5];
-            b.z = b.z * p.decay - p.lr * v[6]; b.w = b.w * p.decay - p.lr * v[7];
-            *(float4 *)d = a;
-            *(float4 *)(d + 4) = b;
-            return;
-        }
+// ------------------------------------------------------------------------------------------------ square products
+// A = X X^T and P (POLY) of calls with little to do: every tile of the square, both triangles.  A lane's eight neighbours
+// down a column are eight neighbours along the row of the transpose, and the product is symmetric: parts go from registers
+// to that row.  Twice the products of the triangle, but no cuts, no turn through LDS and no second store (where there is
+// enough work the triangles win: P of the heads' 21 matrices 23 us against 31, of all 124 52 against 69).
+template <bool POLY>
+__global__ __launch_bounds__(256, 2) void ortho_square_kernel(OrthoTable tab, int ntiles, int step) {
+    typedef OrthoSquare S;
+    __shared__ __attribute__((aligned(128))) char smem[S::LDS];
+    const OrthoTile w = tab.square[nt_xcd_runs(blockIdx.x, ntiles)];
+    const OrthoProb p = tab.prob[w.prob];
+    const OrthoOperands o = ortho_operands(p, tab.ws, step);
+    const int m = ortho_m(p), k = POLY ? m : ortho_n(p);
+    const int i0 = (w.ij >> 16) * S::TA, j0 = (w.ij & 0xffff) * S::TB;
+    const int64_t rb = ortho_row_bytes(k), rm = ortho_row_bytes(m);
+    const char *y = POLY ? o.a : o.x;
+    f32x16 acc[S::FA][S::FB];
+    nt_tile<S, f16x8, NT_SPLIT2, false>(y + i0 * rb, rb, m - i0, 0, y + j0 * rb, rb, m - j0, 0, (k + 31) / 32, smem, acc);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int c0 = i0 + S::TA / S::WR * (wave / S::WC), r0 = j0 + S::TB / S::WC * (wave % S::WC) + (lane & 31);
+    const float down = POLY ? ortho_shift(p.shift, step, -1) : 1.f, down2 = down * down;
+    const float un2 = ORTHO_UNSCALE * ORTHO_UNSCALE, fc = POLY ? ORTHO_C * (down2 * down2) * un2 : un2;
+    const float fb = ORTHO_B * down2 * ORTHO_UNSCALE;
+    char *dst = POLY ? o.p : o.a;
+    const int mpad = (m + 31) & ~31;
 #pragma unroll
-        for (int q = 0; q < 8; ++q)
-            if (k + q < n) d[q] = d[q] * p.decay - p.lr * v[q];
-        return;
-    }
-    T *d = (T *)p.out + at;
-    typedef T t4 __attribute__((ext_vector_type(4)));
-    if (k + 8 <= n && !((uintptr_t)d & (4 * sizeof(T) - 1))) {
-        t4 a, b;
+    for (int j = 0; j < S::FB; ++j)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) { a[q] = (T)v[q]; b[q] = (T)v[4 + q]; }
-        *(t4 *)d = a;
-        *(t4 *)(d + 4) = b;
-        return;
-    }
+        for (int i = 0; i < S::FA; ++i)
 #pragma unroll
-    for (int q = 0; q < 8; ++q)
-        if (k + q < n) d[q] = (T)v[q];
+            for (int h = 0; h < 2; ++h) {
+                float v[8];
+                nt_acc_rows8(acc[i][j], h, v);
+                const int row = r0 + 32 * j, c = c0 + 32 * i + 16 * h + 8 * (lane >> 5);
+                if (row >= m || c >= mpad) continue;
+                if (POLY) {
+                    const char *at = ortho_at(o.a, rm, row, c);
+                    const f16x8 h0 = *(const f16x8 *)at, h1 = *(const f16x8 *)(at + 64);
+#pragma unroll
+                    for (int q = 0; q < 8; ++q)
+                        v[q] = fc * v[q] + fb * ((float)h0[q] + (float)h1[q]) + (row == c + q ? ORTHO_A : 0.f);
+                } else {
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) v[q] *= fc;
+                }
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
+                    if (c + q >= m) v[q] = 0.f;    // (copies of the last row: what pads the contraction is zero)
+                ortho_store8(ortho_at(dst, rm, row, c), v);
+            }
 }
 
-// One 32 (n, from k0) x 32 (m, from r0) block of (P X)^T held by a wave: the result in T (or the weights' update).
-template <typename T>
-__device__ __forceinline__ void ortho_result_block(const OrthoProb &p, const f32x16 &acc, int k0, int r0, int m, int n,
-                                                   float unscale) {
+// ------------------------------------------------------------------------------------------------ X <- P X
+// One 32 (n, from k0) x 32 (m, from r0) block of (P X)^T held by a wave.  Wide matrices: a lane's element (h, q) is column
+// k0 + 16 h + 8 (lane >> 5) + q of row r0 + (lane & 31); tall ones: element r is row k0 + nt_acc_row(r), column r0 + (lane
+// & 31), lanes side by side.  ortho_old: the weights of a block, fetched ahead of the stores of the one before.
+__device__ __forceinline__ void ortho_old(const OrthoProb &p, int k0, int r0, int m, int n, float *old) {
     const int lane = threadIdx.x & 63, row = r0 + (lane & 31);
-    if (p.rows > p.cols) {                         // out[n][m]: lanes along its rows
-        if (row >= m) return;
+    const float *w = (const float *)p.out;
+    if (p.rows > p.cols) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int k = k0 + nt_acc_row(r, lane);
+            old[r] = row < m && k < n ? w[(int64_t)k * p.os + row] : 0.f;
+        }
+        return;
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int k = k0 + 16 * h + 8 * (lane >> 5);
+        const float *d = w + (int64_t)row * p.os + k;
+        if (row < m && k + 8 <= n && !((uintptr_t)d & 15)) {
+            *(float4 *)(old + 8 * h) = *(const float4 *)d;
+            *(float4 *)(old + 8 * h + 4) = *(const float4 *)(d + 4);
+        } else {
+#pragma unroll
+            for (int q = 0; q < 8; ++q) old[8 * h + q] = row < m && k + q < n ? d[q] : 0.f;
+        }
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void ortho_result(const OrthoProb &p, const f32x16 &acc, int k0, int r0, int m, int n,
+                                             float unscale, const float *old) {
+    const int lane = threadIdx.x & 63, row = r0 + (lane & 31);
+    if (row >= m) return;
+    if (p.rows > p.cols) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             const int k = k0 + nt_acc_row(r, lane);
             if (k >= n) continue;
             const int64_t at = (int64_t)k * p.os + row;
             const float v = acc[r] * unscale;
-            if (p.buf) {
-                float *d = (float *)p.out + at;
-                *d = *d * p.decay - p.lr * v;
-            } else {
-                ((T *)p.out)[at] = (T)v;
-            }
+            if (p.buf) ((float *)p.out)[at] = old[r] * p.decay - p.lr * v;
+            else ((T *)p.out)[at] = (T)v;
         }
         return;
     }
+    typedef T t4 __attribute__((ext_vector_type(4)));
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         float v[8];
         nt_acc_rows8(acc, h, v);
-#pragma unroll
-        for (int q = 0; q < 8; ++q) v[q] *= unscale;
         const int k = k0 + 16 * h + 8 * (lane >> 5);
-        if (row < m && k < n) ortho_result8<T>(p, row, k, n, v);
+        const int64_t at = (int64_t)row * p.os + k;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+            v[q] *= unscale;
+            if (p.buf) v[q] = old[8 * h + q] * p.decay - p.lr * v[q];
+        }
+        T *d = (T *)p.out + at;                    // (the optimiser: T is float)
+        if (k + 8 <= n && !((uintptr_t)d & (4 * sizeof(T) - 1))) {
+            t4 a, b;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) { a[q] = (T)v[q]; b[q] = (T)v[4 + q]; }
+            *(t4 *)d = a;
+            *(t4 *)(d + 4) = b;
+        } else {
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+                if (k + q < n) d[q] = (T)v[q];
+        }
     }
 }
 
@@ -558,14 +629,21 @@ __global__ __launch_bounds__(S::THREADS, S::THREADS == 256 ? 2 : 1) void ortho_a
     const int k0 = j0 + S::TA / S::WR * (wave / S::WC), r0 = i0 + S::TB / S::WC * (wave % S::WC);
     const float unscale = ORTHO_UNSCALE * ORTHO_UNSCALE * ortho_shift(p.shift, step, -1) *
                           (LAST ? 1.f : ortho_shift(p.shift, step + 1, 1));
+    if (LAST) {
+        float old[2][16];
+        if (p.buf) ortho_old(p, k0, r0, m, n, old[0]);
+#pragma unroll
+        for (int b = 0; b < S::FA * S::FB; ++b) {
+            const int i = b % S::FA, j = b / S::FA, i2 = (b + 1) % S::FA, j2 = (b + 1) / S::FA;
+            if (p.buf && b + 1 < S::FA * S::FB) ortho_old(p, k0 + 32 * i2, r0 + 32 * j2, m, n, old[(b + 1) & 1]);
+            ortho_result<T>(p, acc[i][j], k0 + 32 * i, r0 + 32 * j, m, n, unscale, old[b & 1]);
+        }
+        return;
+    }
 #pragma unroll
     for (int j = 0; j < S::FB; ++j)
 #pragma unroll
         for (int i = 0; i < S::FA; ++i) {
-            if (LAST) {
-                ortho_result_block<T>(p, acc[i][j], k0 + 32 * i, r0 + 32 * j, m, n, unscale);
-                continue;
-            }
             const int row = r0 + 32 * j + (lane & 31);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -621,32 +699,40 @@ __global__ __launch_bounds__(512) void ortho_small_kernel(OrthoBatch batch, Orth
     auto place = [&](int e, int &i, int &k8) {     // lanes run along G's rows
         if (tall) { i = e % MP; k8 = e / MP; } else { k8 = e % (groups * 4); i = e / (groups * 4); }
     };
+    const bool vec = !tall && sizeof(T) == 4 && (n & 3) == 0 && (p.gs & 3) == 0 &&
+                     !(((uintptr_t)p.g | (uintptr_t)p.buf) & 15);
+    // eight neighbours along n from row i, column k: side by side, or ld apart (tall); zeros outside
+    auto fetch = [&](auto *base, int64_t ld, int i, int k, float *v) {
+        if (vec && i < m && k + 8 <= n) {
+            const float *s = (const float *)base + (int64_t)i * ld + k;
+            *(float4 *)v = *(const float4 *)s;
+            *(float4 *)(v + 4) = *(const float4 *)(s + 4);
+            return;
+        }
+        const auto *s = base + (tall ? (int64_t)k * ld + i : (int64_t)i * ld + k);
+        const int64_t next = tall ? ld : 1;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] = i < m && k + q < n ? (float)s[q * next] : 0.f;
+    };
 #pragma unroll
     for (int s = 0; s < RUNS; ++s) {
         int i, k8;
         place(t + 512 * s, i, k8);
-#pragma unroll
-        for (int q = 0; q < 8; ++q) {
-            const int k = k8 * 8 + q;
-            u[s][q] = i < m && k < n ? ortho_load<T>(p.g, tall ? (int64_t)k * p.gs + i : (int64_t)i * p.gs + k) : 0.f;
-        }
+        fetch((const T *)p.g, p.gs, i, k8 * 8, u[s]);
     }
     if (p.buf) {
 #pragma unroll
         for (int s = 0; s < RUNS; ++s) {
             int i, k8;
             place(t + 512 * s, i, k8);
+            const int k = k8 * 8;
             float b[8];
+            fetch((const float *)p.buf, p.cols, i, k, b);
+            float *d = p.buf + (tall ? (int64_t)k * p.cols + i : (int64_t)i * p.cols + k);
 #pragma unroll
             for (int q = 0; q < 8; ++q) {
-                const int k = k8 * 8 + q;
-                b[q] = i < m && k < n ? p.buf[tall ? (int64_t)k * p.cols + i : (int64_t)i * p.cols + k] : 0.f;
-            }
-#pragma unroll
-            for (int q = 0; q < 8; ++q) {
-                const int k = k8 * 8 + q;
                 u[s][q] = ortho_momentum(rule, u[s][q], cf, b[q]);
-                if (apply && i < m && k < n) p.buf[tall ? (int64_t)k * p.cols + i : (int64_t)i * p.cols + k] = b[q];
+                if (apply && i < m && k + q < n) d[tall ? (int64_t)q * p.cols : q] = b[q];
             }
         }
     }
@@ -798,7 +884,11 @@ __global__ __launch_bounds__(512) void ortho_small_kernel(OrthoBatch batch, Orth
             if (last) {
                 if (apply)
 #pragma unroll
-                    for (int b = 0; b < MB; ++b) ortho_result_block<T>(p, y[b], 32 * g, 32 * b, m, n, unscale);
+                    for (int b = 0; b < MB; ++b) {
+                        float old[16];
+                        if (p.buf) ortho_old(p, 32 * g, 32 * b, m, n, old);
+                        ortho_result<T>(p, y[b], 32 * g, 32 * b, m, n, unscale, old);
+                    }
                 continue;
             }
 #pragma unroll
@@ -823,9 +913,9 @@ __global__ __launch_bounds__(512) void ortho_small_kernel(OrthoBatch batch, Orth
 // ------------------------------------------------------------------------------------------------ host side
 // Everything about a call that follows from its shapes.
 struct OrthoPlan {
-    int64_t prob, split, sym, gram, poly, apply, part, slab, operands, bytes;
-    int nsplit, nsym, ngram, npoly, napply, nparts, cut, poly_tile, apply_tile, empty;
-    bool joined, small;
+    int64_t prob, split, sym, gram, square, apply, part, slab, operands, bytes;
+    int nsplit, nsym, ngram, nsquare, napply, nparts, cut, apply_tile, empty;
+    bool joined, small, squares;     // squares: short Gram products, not cut
 };
 
 static inline int64_t ortho_align(int64_t v) { return (v + 255) & ~(int64_t)255; }
@@ -863,7 +953,7 @@ template <typename D>
 static int ortho_plan(const D *d, int n, OrthoPlan &pl) {
     pl = OrthoPlan();
     pl.small = true;
-    int64_t poly128 = 0, apply256 = 0, live = 0;
+    int64_t square64 = 0, apply256 = 0, live = 0, longest = 0;
     for (int i = 0; i < n; ++i) {
         if (d[i].rows < 0 || d[i].cols < 0 || d[i].rows > (1 << 22) || d[i].cols > (1 << 22)) return SLN_ERR_INVALID_ARG;
         int64_t m, k;
@@ -872,48 +962,50 @@ static int ortho_plan(const D *d, int n, OrthoPlan &pl) {
         if (m == 0) continue;
         ++live;
         pl.small = pl.small && ortho_small((int)m, (int)k);
-        const int64_t t = (m + 127) / 128;
-        poly128 += t * (t + 1) / 2;
+        square64 += ((m + 63) / 64) * ((m + 63) / 64);
+        if ((k + 31) / 32 > longest) longest = (k + 31) / 32;
         apply256 += ((m + 255) / 256) * ((k + 255) / 256);
     }
     pl.empty = live == 0;
     if (pl.empty || pl.small) return SLN_OK;
     pl.cut = (int)ortho_gram_cut(d, n);
-    // Tiles: large ones where they fill the chip, else smaller ones (the polynomial's product is short: what counts
-    // is how many CUs take part).
-    pl.poly_tile = poly128 >= 4096 ? 128 : 64;
+    // Tiles: large ones where they fill the chip, else smaller ones.  Few and short Gram products (up to one tile of 64 x 64
+    // per CU, up to 80 k-steps) go without cuts, partial tiles and the launch that joins them.
     pl.apply_tile = apply256 >= 192 ? 256 : 128;
-    int64_t nsplit = 0, nsym = 0, ngram = 0, npoly = 0, napply = 0, nparts = 0, operands = 0;
+    pl.squares = square64 <= 256 && longest <= 80;
+    int64_t nsplit = 0, nsym = 0, ngram = 0, nsquare = 0, napply = 0, nparts = 0, operands = 0;
     for (int i = 0; i < n; ++i) {
         if (d[i].rows == 0 || d[i].cols == 0) continue;
         OrthoProb p = {};
         p.rows = d[i].rows; p.cols = d[i].cols;
         const int64_t m = ortho_m(p), k = ortho_n(p);
         const int64_t tm = (m + GRAM_TILE - 1) / GRAM_TILE, cuts = ((k + 31) / 32 + pl.cut - 1) / pl.cut;
-        const int64_t tp = (m + pl.poly_tile - 1) / pl.poly_tile;
-        pl.joined |= cuts > 1;
+        const int64_t tp = (m + OrthoSquare::TA - 1) / OrthoSquare::TA;
+        pl.joined |= cuts > 1 && !pl.squares;
         nsplit += ((m + 63) / 64) * ((k + 127) / 128);
-        nsym += tm * (tm + 1) / 2;
-        ngram += tm * (tm + 1) / 2 * cuts;
-        npoly += tp * (tp + 1) / 2;
+        if (!pl.squares) {
+            nsym += tm * (tm + 1) / 2;
+            ngram += tm * (tm + 1) / 2 * cuts;
+        }
+        nsquare += pl.squares ? tp * tp : tp * (tp + 1) / 2;
         napply += ((m + pl.apply_tile - 1) / pl.apply_tile) * ((k + pl.apply_tile - 1) / pl.apply_tile);
         nparts += ((int64_t)p.rows * p.cols + ORTHO_CHUNK - 1) / ORTHO_CHUNK;
         operands += ortho_align(ortho_operand_bytes(p));
         const int64_t most = 1 << 28;
-        if (nsplit > most || ngram > most || npoly > most || napply > most || nparts > most) return SLN_ERR_UNSUPPORTED;
+        if (nsplit > most || ngram > most || nsquare > most || napply > most || nparts > most) return SLN_ERR_UNSUPPORTED;
     }
     int64_t at = 0;
     pl.prob = at; at += ortho_align(live * (int64_t)sizeof(OrthoProb));
     pl.split = at; at += ortho_align(nsplit * (int64_t)sizeof(OrthoTile));
     pl.sym = at; at += ortho_align(nsym * (int64_t)sizeof(OrthoTile));
     pl.gram = at; at += ortho_align(ngram * (int64_t)sizeof(OrthoTile));
-    pl.poly = at; at += ortho_align(npoly * (int64_t)sizeof(OrthoTile));
+    pl.square = at; at += ortho_align(nsquare * (int64_t)sizeof(OrthoTile));
     pl.apply = at; at += ortho_align(napply * (int64_t)sizeof(OrthoTile));
     pl.part = at; at += ortho_align(nparts * (int64_t)sizeof(double));
     pl.slab = at; at += pl.joined ? ortho_align(ngram * (int64_t)(GRAM_TILE * GRAM_TILE * 4)) : 0;
     pl.operands = at; at += operands;
     pl.bytes = at;
-    pl.nsplit = (int)nsplit; pl.nsym = (int)nsym; pl.ngram = (int)ngram; pl.npoly = (int)npoly; pl.napply = (int)napply;
+    pl.nsplit = (int)nsplit; pl.nsym = (int)nsym; pl.ngram = (int)ngram; pl.nsquare = (int)nsquare; pl.napply = (int)napply;
     pl.nparts = (int)nparts;
     return SLN_OK;
 }
@@ -974,10 +1066,10 @@ static int ortho_run(const D *d, int n, int steps, float eps, const OrthoRule &r
     }
     char *ws = (char *)workspace;
     const OrthoTable tab = {(OrthoProb *)(ws + pl.prob), (OrthoTile *)(ws + pl.split), (OrthoTile *)(ws + pl.sym),
-                            (OrthoTile *)(ws + pl.gram), (OrthoTile *)(ws + pl.poly), (OrthoTile *)(ws + pl.apply),
-                            (double *)(ws + pl.part), ws, (float *)(ws + pl.slab), pl.poly_tile, pl.apply_tile};
+                            (OrthoTile *)(ws + pl.gram), (OrthoTile *)(ws + pl.square), (OrthoTile *)(ws + pl.apply),
+                            (double *)(ws + pl.part), ws, (float *)(ws + pl.slab), pl.apply_tile};
     OrthoBatch batch;
-    int prob0 = 0, inb = 0, parts = 1, part0 = 0, split0 = 0, sym0 = 0, gram0 = 0, poly0 = 0, apply0 = 0;
+    int prob0 = 0, inb = 0, parts = 1, part0 = 0, split0 = 0, sym0 = 0, gram0 = 0, square0 = 0, apply0 = 0;
     int64_t off = pl.operands;
     for (int i = 0; i <= n; ++i) {
         if (inb == ORTHO_BATCH || (inb > 0 && i == n)) {
@@ -988,25 +1080,27 @@ static int ortho_run(const D *d, int n, int steps, float eps, const OrthoRule &r
         OrthoProb &p = batch.p[inb++];
         ortho_desc(d[i], p);
         const int m = ortho_m(p), k = ortho_n(p);
-        const int tm = ortho_tiles(m, GRAM_TILE), tp = ortho_tiles(m, pl.poly_tile);
+        const int tm = ortho_tiles(m, GRAM_TILE), tp = ortho_tiles(m, OrthoSquare::TA);
         p.off = off; off += ortho_align(ortho_operand_bytes(p));
-        p.nsplit = ((k + 31) / 32 + pl.cut - 1) / pl.cut;
+        p.nsplit = pl.squares ? 0 : ((k + 31) / 32 + pl.cut - 1) / pl.cut;
         p.part0 = part0; p.nparts = sln_div_up((long)p.rows * p.cols, ORTHO_CHUNK); part0 += p.nparts;
         p.split0 = split0; split0 += ortho_tiles(m, 64) * ortho_tiles(k, 128);
-        p.sym0 = sym0; sym0 += tm * (tm + 1) / 2;
+        p.sym0 = sym0; sym0 += pl.squares ? 0 : tm * (tm + 1) / 2;
         p.gram0 = gram0; gram0 += tm * (tm + 1) / 2 * p.nsplit;
-        p.poly0 = poly0; poly0 += tp * (tp + 1) / 2;
+        p.square0 = square0; square0 += pl.squares ? tp * tp : tp * (tp + 1) / 2;
         p.apply0 = apply0; apply0 += ortho_tiles(m, pl.apply_tile) * ortho_tiles(k, pl.apply_tile);
         if (p.nparts > parts) parts = p.nparts;
     }
     hipLaunchKernelGGL((ortho_split_kernel<T>), dim3(pl.nsplit), dim3(256), 0, stream, tab, rule, eps);
     for (int s = 0; s < steps; ++s) {
-        hipLaunchKernelGGL(ortho_gram_kernel, dim3(pl.ngram), dim3(256), 0, stream, tab, s, pl.ngram);
-        if (pl.joined) hipLaunchKernelGGL(ortho_join_kernel, dim3(4 * pl.nsym), dim3(256), 0, stream, tab);
-        if (pl.poly_tile == 128)
-            hipLaunchKernelGGL((ortho_poly_kernel<OrthoGram>), dim3(pl.npoly), dim3(256), 0, stream, tab, pl.npoly, s);
-        else
-            hipLaunchKernelGGL((ortho_poly_kernel<OrthoPolySmall>), dim3(pl.npoly), dim3(256), 0, stream, tab, pl.npoly, s);
+        if (pl.squares) {
+            hipLaunchKernelGGL((ortho_square_kernel<false>), dim3(pl.nsquare), dim3(256), 0, stream, tab, pl.nsquare, s);
+            hipLaunchKernelGGL((ortho_square_kernel<true>), dim3(pl.nsquare), dim3(256), 0, stream, tab, pl.nsquare, s);
+        } else {
+            hipLaunchKernelGGL(ortho_gram_kernel, dim3(pl.ngram), dim3(256), 0, stream, tab, s, pl.ngram);
+            if (pl.joined) hipLaunchKernelGGL(ortho_join_kernel, dim3(4 * pl.nsym), dim3(256), 0, stream, tab);
+            hipLaunchKernelGGL(ortho_poly_kernel, dim3(pl.nsquare), dim3(256), 0, stream, tab, pl.nsquare, s);
+        }
         if (pl.apply_tile == 256) ortho_apply<T, OrthoApplyLarge>(tab, pl.napply, s, s + 1 == steps, rule, stream);
         else ortho_apply<T, OrthoApplySmall>(tab, pl.napply, s, s + 1 == steps, rule, stream);
     }
