@@ -136,3 +136,27 @@ def lib():
 def check(code, what):
     if code != 0:
         raise RuntimeError("%s failed: %s" % (what, lib().sln_error_string(code).decode()))
+
+
+class on_device(object):
+    """`with on_device(t.device):` -- launches go to the tensor's device; nothing is switched where that is the current one
+    already."""
+    __slots__ = ("guard",)
+
+    def __init__(self, dev):
+        import torch
+        self.guard = None if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def stream_of(dev):
+    """torch's current stream on `dev` as the C entries take it."""
+    import torch
+    return torch._C._cuda_getCurrentRawStream(dev.index)

@@ -14,26 +14,6 @@ FEW_ROWS = 16          # rows that sln_mx4_rows_product takes: rounded inside th
 MAX_K = 1 << 22
 
 
-def _stream(dev):
-    return torch._C._cuda_getCurrentRawStream(dev.index)
-
-
-class _On(object):
-    """Launches go to the tensors' device; nothing is switched where that is the current one already."""
-    __slots__ = ("guard",)
-
-    def __init__(self, dev):
-        self.guard = None if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
-
-
 def _need_float(t, name):
     if not torch.is_tensor(t):
         raise TypeError("%s must be a tensor" % name)
@@ -91,9 +71,9 @@ class Mx4Tensor(object):
         dev = self.data.device
         out = torch.empty(self.shape, dtype=dtype, device=dev)
         codes, scales = _pointers(self.data, self.rows, self.shape[-1])
-        with _On(dev):
+        with _lib.on_device(dev):
             _lib.check(_lib.lib().sln_mx4_values(codes, scales, self.rows, self.shape[-1], out.data_ptr(),
-                                                 _DTYPES[dtype], _stream(dev)), "sln_mx4_values")
+                                                 _DTYPES[dtype], _lib.stream_of(dev)), "sln_mx4_values")
         return out
 
     def __repr__(self):
@@ -122,8 +102,8 @@ def mx4_quantize(x):
     dev = x.device
     data = _buffer(R, K, dev)
     codes, scales = _pointers(data, R, K)
-    with _On(dev):
-        _lib.check(_lib.lib().sln_mx4_round(src.data_ptr(), _DTYPES[x.dtype], R, K, pitch, codes, scales, _stream(dev)),
+    with _lib.on_device(dev):
+        _lib.check(_lib.lib().sln_mx4_round(src.data_ptr(), _DTYPES[x.dtype], R, K, pitch, codes, scales, _lib.stream_of(dev)),
                    "sln_mx4_round")
     return Mx4Tensor(data, R, x.shape, x.dtype)
 
@@ -147,11 +127,11 @@ def _forward(x, weight, wq, bias, scale, relu, keep):
     wc, ws = _pointers(wdata, N, K)
     nbytes = L.sln_mx4_product_workspace_bytes(M, N, K, xdata is not None)
     work = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    with _On(dev):
+    with _lib.on_device(dev):
         _lib.check(L.sln_mx4_linear_fwd(src.data_ptr(), _DTYPES[x.dtype], M, K, pitch, xc, xs, w, w_pitch, wc, ws, N,
                                         scale.data_ptr() if scale is not None else 0,
                                         bias.data_ptr() if bias is not None else 0, relu, y.data_ptr(),
-                                        work.data_ptr() if nbytes else 0, nbytes, _stream(dev)), "sln_mx4_linear_fwd")
+                                        work.data_ptr() if nbytes else 0, nbytes, _lib.stream_of(dev)), "sln_mx4_linear_fwd")
     return y, M, K, N, xdata, wdata
 
 
@@ -190,9 +170,9 @@ class _Mx4LinearFn(torch.autograd.Function):
             xc, xs = _pointers(xdata, M, K) if want_w else (0, 0)
             wc, ws = _pointers(wdata, N, K)
             at = lambda t: t.data_ptr() if t is not None else 0
-            with _On(dev):
+            with _lib.on_device(dev):
                 _lib.check(L.sln_mx4_linear_bwd(g.data_ptr(), kind, pitch, at(y), at(scale), xc, xs, wc, ws, M, N, K,
-                                                at(gx), at(gw), at(gb), work.data_ptr(), nbytes, _stream(dev)),
+                                                at(gx), at(gw), at(gb), work.data_ptr(), nbytes, _lib.stream_of(dev)),
                            "sln_mx4_linear_bwd")
         return gx, gw, gb, None, None, None
 

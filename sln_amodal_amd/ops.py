@@ -387,7 +387,13 @@ def orthogonalize(x, steps=5, eps=1e-7):
     zero, one with an infinity or a NaN becomes NaN.  All matrices share every launch.  Products are float32-accurate
     whatever the type, rounded once at the end.  No gradient."""
     many = isinstance(x, (list, tuple))
-    mats = list(x) if many else [x]
+    mats = x if many else (x,)
+    steps, eps = int(steps), float(eps)
+    if not 1 <= steps <= 64 or not eps >= 1e-30:
+        raise ValueError("orthogonalize: 1 <= steps <= 64 and eps >= 1e-30 (got %r, %r)" % (steps, eps))
+    grad = torch.is_grad_enabled()
+    dtype = dev = None
+    outs, flat, keep = [], [], []
     for t in mats:
         if not torch.is_tensor(t):
             raise TypeError("orthogonalize takes tensors")
@@ -395,42 +401,46 @@ def orthogonalize(x, steps=5, eps=1e-7):
             raise RuntimeError("x must live on the GPU (no CPU fallback in sln_amodal_amd)")
         if t.dtype not in _FLOATS:
             raise TypeError("x must be float32, bfloat16 or float16, got %s" % t.dtype)
-        if t.dim() < 2 or (many and t.dim() != 2):
+        shape = t.shape
+        if len(shape) < 2 or (many and len(shape) != 2):
             raise ValueError("orthogonalize takes matrices [rows, cols] (or one stack [..., rows, cols]), got %s" %
-                             (tuple(t.shape),))
-        if t.dtype != mats[0].dtype or t.device != mats[0].device:
+                             (tuple(shape),))
+        if dtype is None:
+            dtype, dev, es = t.dtype, t.device, t.element_size()
+        elif t.dtype != dtype or t.device != dev:
             raise ValueError("the matrices of one call share a type and a device")
-        if t.requires_grad and torch.is_grad_enabled():
+        if grad and t.requires_grad:
             raise RuntimeError("orthogonalize has no gradient: detach x or call it under torch.no_grad()")
-        if min(t.shape[-2:]) > 65535 or max(t.shape[-2:]) > 1 << 22:
-            raise ValueError("orthogonalize: at most 65535 x 2^22, got %s" % (tuple(t.shape),))
-    if not 1 <= int(steps) <= 64 or not float(eps) >= 1e-30:
-        raise ValueError("orthogonalize: 1 <= steps <= 64 and eps >= 1e-30 (got %r, %r)" % (steps, eps))
-    outs, flat, keep = [], [], []
-    for t in mats:
-        o = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+        r, c = shape[-2], shape[-1]
+        if min(r, c) > 65535 or max(r, c) > 1 << 22:
+            raise ValueError("orthogonalize: at most 65535 x 2^22, got %s" % (tuple(shape),))
+        o = torch.empty(shape, dtype=dtype, device=dev)
         outs.append(o)
-        if t.numel() == 0:
+        if o.numel() == 0:
             continue
-        r, c = t.shape[-2:]
-        src = t.detach()
-        if src.dim() != 2:
-            src = src.reshape(-1, r, c)
-        if (c > 1 and src.stride(-1) != 1) or (r > 1 and src.stride(-2) < c):
-            src = src.contiguous()
-        keep.append(src)
-        gs = src.stride(-2) if r > 1 else c
-        es = t.element_size()
-        base, step = src.data_ptr(), (src.stride(0) * es if src.dim() == 3 else 0)
-        for b in range(src.shape[0] if src.dim() == 3 else 1):
-            flat.append((base + b * step, o.data_ptr() + b * r * c * es, gs, c, r, c))
+        src = t if len(shape) == 2 else t.detach().reshape(-1, r, c)
+        strides = src.stride()
+        if (c > 1 and strides[-1] != 1) or (r > 1 and strides[-2] < c):
+            src = src.detach().contiguous()
+            keep.append(src)
+            strides = src.stride()
+        elif src is not t:
+            keep.append(src)
+        gs = strides[-2] if r > 1 else c
+        base, dst = src.data_ptr(), o.data_ptr()
+        if len(shape) == 2:
+            flat.append((base, dst, gs, c, r, c))
+        else:
+            for b in range(src.shape[0]):
+                flat.append((base + b * strides[0] * es, dst + b * r * c * es, gs, c, r, c))
     if flat:
-        flat.sort(key=lambda d: -min(d[4], d[5]))            # (the longest products first: the launches end together)
+        if len(flat) > 1:
+            flat.sort(key=lambda d: -min(d[4], d[5]))        # (the longest products first: the launches end together)
         descs = (_OrthoDesc * len(flat))(*flat)
         L = _lib.lib()
-        with torch.cuda.device(mats[0].device):
-            nbytes = L.sln_orthogonalize_workspace_bytes(descs, len(flat))
-            ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=mats[0].device)
-            _lib.check(L.sln_orthogonalize(descs, len(flat), _FLOATS[mats[0].dtype], int(steps), float(eps), _ptr(ws), nbytes,
-                                           _stream()), "sln_orthogonalize")
+        nbytes = L.sln_orthogonalize_workspace_bytes(descs, len(flat))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        with _lib.on_device(dev):
+            _lib.check(L.sln_orthogonalize(descs, len(flat), _FLOATS[dtype], steps, eps, ws.data_ptr() if nbytes else 0,
+                                           nbytes, _lib.stream_of(dev)), "sln_orthogonalize")
     return type(x)(outs) if many else outs[0]

@@ -30,6 +30,7 @@ class ClippedSGD(object):
         self.skipped_clamped = None          # device int32: of those, the steps vetoed for clamped operand blocks
         self._plan_key, self._plan = None, None
         self._ring, self._turn = [], 0       # pinned staging buffers of the pointer tables
+        self._spare, self._captured = None, []        # the next captured step's, those of captured steps
         self.capturing = False               # inside a HIP-graph capture: no event waits (the tables are static)
         self.last_norm = None
 
@@ -142,7 +143,7 @@ class ClippedSGD(object):
             raise RuntimeError("ClippedSGD runs on the GPU only (no CPU fallback in sln_amodal_amd)")
         ps, gs, bs = self._buffers(act)
         ct, co, numel, partial, wd = self._chunks([p.numel() for p in ps], [w for _, w in act], dev)
-        tab = self._upload(ps, gs, bs, dev)
+        tab = self._upload(ps, gs, bs, dev)[1]
         sq = torch.empty(1, dtype=torch.float64, device=dev)
         if self.skipped is None:
             self.skipped = torch.zeros(1, dtype=torch.int32, device=dev)
@@ -181,27 +182,34 @@ class ClippedSGD(object):
         return ps, gs, bs
 
     def _upload(self, ps, gs, bs, dev):
-        """Pointer tables [3, n] (weights, gradients, momentum) on the device: gradients are fresh allocations every
-        step, so the tables are re-sent each time -- from pinned staging buffers and asynchronously, so the host never
-        waits for the GPU here (a pageable copy would drain the stream once per step).  A staging buffer is reused only
-        after the copy that read it has completed (4 in flight)."""
+        """Pointer tables [3, n] (weights, gradients, momentum), as lists and on the device: gradients are fresh
+        allocations every step, so the tables are re-sent each time -- from pinned staging buffers and asynchronously, so
+        the host never waits for the GPU here (a pageable copy would drain the stream once per step).  A staging buffer
+        is reused only after the copy that read it has completed (4 in flight); one that a captured graph copies from is
+        never written again (its replays read it)."""
         n = len(ps)
         if not self._ring or self._ring[0][0].shape[1] != n:
             self._ring = [[torch.empty((3, n), dtype=torch.int64, pin_memory=True), None] for _ in range(4)]
+        capturing = self.capturing or torch.cuda.is_current_stream_capturing()
         stage = self._ring[self._turn % len(self._ring)]
         self._turn += 1
-        if stage[1] is not None and not self.capturing:
+        if stage[1] is not None and not capturing:
             stage[1].synchronize()
-        host = stage[0].numpy()
-        host[0] = [p.data_ptr() for p in ps]
-        host[1] = [g.data_ptr() for g in gs]
-        host[2] = [b.data_ptr() for b in bs]
+        if capturing:
+            if self._spare is None or self._spare.shape[1] != n:
+                raise RuntimeError("take an eager step over the same parameters before each captured one")
+            stage, self._spare = [self._spare, None], None
+            self._captured.append(stage[0])
+        elif self._spare is None or self._spare.shape[1] != n:
+            self._spare = torch.empty((3, n), dtype=torch.int64, pin_memory=True)
+        host = [[t.data_ptr() for t in ts] for ts in (ps, gs, bs)]
+        stage[0].numpy()[:] = host
         tab = torch.empty((3, n), dtype=torch.int64, device=dev)
         tab.copy_(stage[0], non_blocking=True)
-        if not self.capturing:
+        if not capturing:
             stage[1] = torch.cuda.Event()
             stage[1].record()
-        return tab
+        return host, tab
 
     def _guard(self, sq, veto):
         """The guard's input: +inf instead of the squared norm when the step is vetoed (two 5-us elementwise ops)."""
@@ -273,58 +281,69 @@ class ClippedMuon(ClippedSGD):
     @torch.no_grad()
     def step(self, max_norm, veto=None):
         """See ClippedSGD.step: the same arguments, guard and counters."""
-        rest_groups, ortho_groups = self._split()
-        rest = [(p, float(g["weight_decay"])) for g in rest_groups for p in g["params"] if p.grad is not None]
-        mats = [(p, g) for g in ortho_groups for p in g["params"] if p.grad is not None]
-        act = rest + [(p, 0.0) for p, _ in mats]
+        rest, mats, moms = [], [], set()
+        for g in self.param_groups:
+            if g["orthogonal"]:
+                lr, decay = float(g["lr"]), 1.0 - float(g["lr"]) * float(g["weight_decay"])
+                live = [(p, (lr, decay)) for p in g["params"] if p.grad is not None]
+                mats += live
+                if live:
+                    moms.add(float(g["momentum"]))
+            else:
+                wd = float(g["weight_decay"])
+                rest += [(p, wd) for p in g["params"] if p.grad is not None]
+        act = rest + mats
         if not act:
             return None
+        if len(moms) > 1:
+            raise ValueError("ClippedMuon applies one momentum to its orthogonal groups (got %s)" % sorted(moms))
         dev = act[0][0].device
         if dev.type != "cuda":
             raise RuntimeError("ClippedMuon runs on the GPU only (no CPU fallback in sln_amodal_amd)")
-        if any(p.device != dev or p.grad.device != dev for p, _ in act):
-            raise ValueError("ClippedMuon: the parameters and gradients of one step share a device")
-        moms = {float(g["momentum"]) for _, g in mats}
-        if len(moms) > 1:
-            raise ValueError("ClippedMuon applies one momentum to its orthogonal groups (got %s)" % sorted(moms))
+        for p, _ in act:
+            if p.device != dev or p.grad.device != dev:
+                raise ValueError("ClippedMuon: the parameters and gradients of one step share a device")
         lr, momentum = self._hyper()
-        with torch.cuda.device(dev):
+        with _lib.on_device(dev):
             ps, gs, bs = self._buffers(act)
-            ct, co, numel, partial, wd = self._chunks([p.numel() for p in ps], [w for _, w in act], dev)
-            tab = self._upload(ps, gs, bs, dev)
+            sizes = [p.numel() for p in ps]
+            ct, co, numel, partial, wd = self._chunks(sizes, [w for _, w in rest] + [0.0] * len(mats), dev)
+            host, tab = self._upload(ps, gs, bs, dev)
+            row = 8 * len(ps)
+            at = tab.data_ptr()
             sq = torch.empty(1, dtype=torch.float64, device=dev)
             if self.skipped is None:
                 self.skipped = torch.zeros(1, dtype=torch.int32, device=dev)
-            st = C.c_void_p(torch.cuda.current_stream().cuda_stream)
+            st = _lib.stream_of(dev)
             L = _lib.lib()
-            vp = lambda t: C.c_void_p(t.data_ptr())
-            nch = ct.numel() if sum(p.numel() for p in ps) else 0
-            _lib.check(L.sln_grad_sqnorm_f32(vp(tab[1]), vp(numel), vp(ct), vp(co), nch, CHUNK, vp(partial), vp(sq), st),
+            nch = ct.numel() if sum(sizes) else 0
+            num, ctp, cop = numel.data_ptr(), ct.data_ptr(), co.data_ptr()
+            _lib.check(L.sln_grad_sqnorm_f32(at + row, num, ctp, cop, nch, CHUNK, partial.data_ptr(), sq.data_ptr(), st),
                        "sln_grad_sqnorm_f32")
             guard = self._guard(sq, veto)
             # the vectors come first in the tables: their chunks are a prefix of the chunk list.  (The SGD kernel also
             # counts a skipped step; without vectors that is done here.)
-            nrest = sum(-(-p.numel() // CHUNK) for p, _ in rest)
+            nrest = sum(-(-n // CHUNK) for n in sizes[:len(rest)])
             if nrest:
-                _lib.check(L.sln_sgd_clip_step_f32(vp(tab[0]), vp(tab[1]), vp(tab[2]), vp(numel), vp(wd), vp(ct), vp(co),
-                                                   nrest, CHUNK, vp(guard), float(max_norm), lr, momentum,
-                                                   vp(self.skipped), st), "sln_sgd_clip_step_f32")
+                _lib.check(L.sln_sgd_clip_step_f32(at, at + row, at + 2 * row, num, wd.data_ptr(), ctp, cop, nrest, CHUNK,
+                                                   guard.data_ptr(), float(max_norm), lr, momentum, self.skipped.data_ptr(),
+                                                   st), "sln_sgd_clip_step_f32")
             else:
                 self.skipped += (~torch.isfinite(guard)).to(torch.int32)
             if mats:
-                k, flat = len(rest), []
-                for i, (p, g) in enumerate(mats):
+                flat = []
+                for i, (p, (glr, decay)) in enumerate(mats, len(rest)):
                     rows = p.shape[0]
-                    cols = p.numel() // rows if rows else 0
-                    glr = float(g["lr"])
-                    flat.append((p.data_ptr(), gs[k + i].data_ptr(), bs[k + i].data_ptr(), rows, cols,
-                                 glr * max(1.0, rows / cols) ** 0.5 if cols else 0.0, 1.0 - glr * float(g["weight_decay"])))
+                    cols = sizes[i] // rows if rows else 0
+                    flat.append((host[0][i], host[1][i], host[2][i], rows, cols,
+                                 glr * max(1.0, rows / cols) ** 0.5 if cols else 0.0, decay))
                 flat.sort(key=lambda d: -min(d[3], d[4]))        # (the longest products first: the launches end together)
                 descs = (_MuonDesc * len(flat))(*flat)
                 nbytes = L.sln_muon_step_workspace_bytes(descs, len(flat))
-                ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=dev)
-                _lib.check(L.sln_muon_step_f32(descs, len(flat), self.steps, self.eps, vp(guard), float(max_norm),
-                                               moms.pop(), int(self.nesterov), vp(ws), nbytes, st), "sln_muon_step_f32")
+                ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+                _lib.check(L.sln_muon_step_f32(descs, len(flat), self.steps, self.eps, guard.data_ptr(), float(max_norm),
+                                               moms.pop(), self.nesterov, ws.data_ptr() if nbytes else 0, nbytes, st),
+                           "sln_muon_step_f32")
             torch._C._autograd._unsafe_set_version_counter(ps, [p._version + 1 for p in ps])
             self._keep = (tab, gs, guard)
             self.last_norm = sq.sqrt().to(torch.float32)[0]

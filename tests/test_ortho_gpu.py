@@ -296,3 +296,53 @@ def test_side_streams_and_captured_graphs():
         torch.cuda.synchronize()
         for o, e in zip(outs, eager):
             assert all(torch.equal(a, b) for a, b in zip(flat(o), e))
+
+
+def test_a_captured_step_replays_beside_eager_ones():
+    """The captured step reads its own pointer table: eager steps with other gradients in between do not reach it."""
+    from sln_amodal_amd.optim import ClippedMuon
+
+    def make():
+        gen = torch.Generator().manual_seed(8)
+        ps = [torch.nn.Parameter(torch.randn(s, generator=gen).cuda()) for s in [(20, 30), (100, 130), (30,)]]
+        return ps, ClippedMuon([{"params": ps[:2], "orthogonal": True}, {"params": ps[2:]}], lr=0.1, momentum=0.8)
+
+    gen = torch.Generator().manual_seed(9)
+    draw = lambda: [torch.randn(s, generator=gen).cuda() for s in [(20, 30), (100, 130), (30,)]]
+    a, oa = make()
+    b, ob = make()
+    static = draw()
+    first = draw()
+    for ps, opt in ((a, oa), (b, ob)):
+        for p, g in zip(ps, first):
+            p.grad = g.clone()
+        opt.step(5.0)
+    torch.cuda.synchronize()
+    for p, g in zip(a, static):
+        p.grad = g
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(s):
+        with torch.cuda.graph(graph, stream=s):
+            oa.step(5.0)
+    torch.cuda.current_stream().wait_stream(s)
+    with pytest.raises(RuntimeError):                           # one eager step before each capture
+        oa.capturing = True
+        oa.step(5.0)
+    oa.capturing = False
+    for r in range(6):
+        new = draw()
+        if r % 2 == 0:                                          # a replay against an eager step of the twin
+            for g, v in zip(static, new):
+                g.copy_(v)
+            graph.replay()
+        else:                                                   # an eager step of both, the captured gradients left alone
+            for p, v in zip(a, new):
+                p.grad = v.clone()
+            oa.step(5.0)
+        for p, v in zip(b, new):
+            p.grad = v.clone()
+        ob.step(5.0)
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(a, b)), r
