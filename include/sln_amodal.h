@@ -568,8 +568,8 @@ int sln_conv2d_wgrad_f32(const uint16_t *gz_parts, int Cout, int Cout_pad, const
  * next to the 2 x fp16, 3 x bf16 and 1 x fp16 ones; csrc/mx4.hip has the format).
  *
  * A matrix [R][K] is held as codes (two e2m1 values per byte, the lower nibble first; row pitch Kp / 2 bytes, Kp =
- * sln_mx4_row_values(K) = K rounded up to 256, the padding zero) and scales (one byte s + 127 per 32 values of a row: the
- * block's values are code * 2^s; 255: all NaN; row pitch Kp / 32).  Codes start on 16-byte, scales on 8-byte boundaries.
+ * sln_mx4_row_values(K) = K rounded up to 256, the padding zero) and scales [Kp / 256][R][8] (one byte s + 127 per 32 values
+ * of a row: the block's values are code * 2^s; 255: all NaN).  Codes start on 16-byte, scales on 8-byte boundaries.
  * dtype: SLN_DTYPE_*.  K <= 2^22.
  * ------------------------------------------------------------------------- */
 #define SLN_DTYPE_F32 0

@@ -6,15 +6,22 @@
 // runs along the rows, one k-step of one row is ONE piece of 64 P contiguous bytes: the LDS DMA pays per 128-B line it
 // touches, not per byte, and with two parts a row's step is a line.  The first operand may also be read across its rows
 // (TRA: the matrix is [k][a], two parts): a stage is then 32 rows of TA / 32 groups, and the fragments come out of LDS
-// through the transposing read.  Rows and groups behind the last one are read as copies of it; what they give is dropped
-// (or meets the other operand's zeros).
+// through the transposing read.  Rows (TRA: groups) behind the last one are read as copies of it; what they give is dropped.
 //
 // Tile TA x TB, WR x WC waves, k-step 32, NST LDS stages filled by DMA, NST - 1 of them in flight.  v_mfma_f32_32x32x16:
 // 32 cycles for a k of 16; a wave of 64 x 64 reads 8 fragments for 12 products (two parts each), one of 128 x 64 12 for 24.
 // Measured alone (4096^3, two parts each, random values): 128 x 128, two workgroups per CU: 1089 TFLOP/s of products;
 // 256 x 256, one of eight waves: 1305, which is what the library's fp16 product reaches on this card (1390 at 8192^3).
+// The DMA goes through buffer descriptors: base and step in scalar registers, one 32-bit offset per piece and lane (with
+// flat addresses the loop carries a 64-bit pointer per piece, and the 256 x 256 tile spills).
 #pragma once
 #include "common.h"
+
+typedef __attribute__((address_space(3))) void nt_lds;
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t nt_buffer(const void *base, int64_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, (int)(unsigned)(bytes < 0xffffffffll ? bytes : 0xffffffffll),
+                                             0x00020000);
+}
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
@@ -68,6 +75,46 @@ __device__ __forceinline__ void nt_piece_offsets(int rows_left, int64_t row_byte
     }
 }
 
+// Transposing reads of a 16-value step for FA blocks of 32 columns, two parts each: sixteen lanes turn a 4 (k) x 16 block,
+// lane l addressing 8 B of row l / 4 and receiving column l.  f[i][p]: the fragment.  at[q]: byte of part (q & 1) of the
+// blocks with i & 1 == q >> 1; STEP: bytes to row k + 4 and, times four, KK steps of 16 rows.  One asm block that ends with
+// its own wait: behind the builtin the compiler waits for the DMA that is in flight, too.
+template <int FA, int STEP, int KK, typename V>
+__device__ __forceinline__ void nt_read_turned(const unsigned (&at)[4], V (&f)[FA][2]) {
+    static_assert(FA == 2 || FA == 4, "blocks per wave");
+    union { s16x4 h[2]; V v; } u[FA][2];
+    constexpr int K0 = 4 * STEP * KK, K1 = K0 + STEP;
+    if constexpr (FA == 2) {
+        asm volatile("ds_read_b64_tr_b16 %0, %8 offset:%12\n\tds_read_b64_tr_b16 %1, %8 offset:%13\n\t"
+                     "ds_read_b64_tr_b16 %2, %9 offset:%12\n\tds_read_b64_tr_b16 %3, %9 offset:%13\n\t"
+                     "ds_read_b64_tr_b16 %4, %10 offset:%12\n\tds_read_b64_tr_b16 %5, %10 offset:%13\n\t"
+                     "ds_read_b64_tr_b16 %6, %11 offset:%12\n\tds_read_b64_tr_b16 %7, %11 offset:%13\n\t"
+                     "s_waitcnt lgkmcnt(0)"
+                     : "=&v"(u[0][0].h[0]), "=&v"(u[0][0].h[1]), "=&v"(u[0][1].h[0]), "=&v"(u[0][1].h[1]),
+                       "=&v"(u[1][0].h[0]), "=&v"(u[1][0].h[1]), "=&v"(u[1][1].h[0]), "=&v"(u[1][1].h[1])
+                     : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "n"(K0), "n"(K1)
+                     : "memory");
+    } else {
+        asm volatile("ds_read_b64_tr_b16 %0, %16 offset:%20\n\tds_read_b64_tr_b16 %1, %16 offset:%21\n\t"
+                     "ds_read_b64_tr_b16 %2, %17 offset:%20\n\tds_read_b64_tr_b16 %3, %17 offset:%21\n\t"
+                     "ds_read_b64_tr_b16 %4, %18 offset:%20\n\tds_read_b64_tr_b16 %5, %18 offset:%21\n\t"
+                     "ds_read_b64_tr_b16 %6, %19 offset:%20\n\tds_read_b64_tr_b16 %7, %19 offset:%21\n\t"
+                     "ds_read_b64_tr_b16 %8, %16 offset:%22\n\tds_read_b64_tr_b16 %9, %16 offset:%23\n\t"
+                     "ds_read_b64_tr_b16 %10, %17 offset:%22\n\tds_read_b64_tr_b16 %11, %17 offset:%23\n\t"
+                     "ds_read_b64_tr_b16 %12, %18 offset:%22\n\tds_read_b64_tr_b16 %13, %18 offset:%23\n\t"
+                     "ds_read_b64_tr_b16 %14, %19 offset:%22\n\tds_read_b64_tr_b16 %15, %19 offset:%23\n\t"
+                     "s_waitcnt lgkmcnt(0)"
+                     : "=&v"(u[0][0].h[0]), "=&v"(u[0][0].h[1]), "=&v"(u[0][1].h[0]), "=&v"(u[0][1].h[1]),
+                       "=&v"(u[1][0].h[0]), "=&v"(u[1][0].h[1]), "=&v"(u[1][1].h[0]), "=&v"(u[1][1].h[1]),
+                       "=&v"(u[2][0].h[0]), "=&v"(u[2][0].h[1]), "=&v"(u[2][1].h[0]), "=&v"(u[2][1].h[1]),
+                       "=&v"(u[3][0].h[0]), "=&v"(u[3][0].h[1]), "=&v"(u[3][1].h[0]), "=&v"(u[3][1].h[1])
+                     : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "n"(K0), "n"(K1), "n"(K0 + 256), "n"(K1 + 256)
+                     : "memory");
+    }
+#pragma unroll
+    for (int i = 0; i < FA; ++i) { f[i][0] = u[i][0].v; f[i][1] = u[i][1].v; }
+}
+
 // acc[i][j]: this wave's 32 x 32 blocks of the tile (rows TA / WR * (wave / WC) + 32 i, columns TB / WC * (wave % WC) +
 // 32 j), summed over the k groups [g0, g1).  `a` / `b`: first byte of the tile's first row; a_left / b_left: rows that
 // exist from there on (> 0); TA (TB) rows must span less than 2^32 bytes.  TRA: `a` is the first byte of the tile's first
@@ -77,20 +124,19 @@ template <typename S, typename V, int MODE, bool TRA>
 __device__ __forceinline__ void nt_tile(const char *a, int64_t a_row_bytes, int a_left, int a_rows, const char *b,
                                         int64_t b_row_bytes, int b_left, int g0, int g1, char *smem,
                                         f32x16 (&acc)[S::FA][S::FB]) {
-    typedef __attribute__((address_space(3))) void lds_void;
-    typedef __attribute__((address_space(1))) const void glb_void;
+#ifdef __HIP_DEVICE_COMPILE__                      // (the host pass knows no buffer descriptors in templates)
     constexpr int PA = S::PA, PB = S::PB, QA = S::QA, QB = S::QB, NW = S::NW;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int wr = wave / S::WC, wc = wave % S::WC;
     unsigned aoff[QA], boff[QB];
     if constexpr (!TRA) {
         nt_piece_offsets<PA, QA, NW>(a_left, a_row_bytes, wave, lane, aoff);
-    } else {                                       // offset within a row; the row of the piece is (slot / (TA / 4))
+    } else {                                       // row of the stage, offset within it
 #pragma unroll
         for (int q = 0; q < QA; ++q) {
             const int slot = (q * NW + wave) * 64 + lane, k = slot / (S::TA / 4), p = slot % (S::TA / 4);
             const int unit = (p >> 2) ^ (k & 3);
-            aoff[q] = (unsigned)(min(unit >> 1, a_left - 1) * 128 + (unit & 1) * 64 + (p & 3) * 16);
+            aoff[q] = (unsigned)(k * a_row_bytes + min(unit >> 1, a_left - 1) * 128 + (unit & 1) * 64 + (p & 3) * 16);
         }
     }
     nt_piece_offsets<PB, QB, NW>(b_left, b_row_bytes, wave, lane, boff);
@@ -101,28 +147,29 @@ __device__ __forceinline__ void nt_tile(const char *a, int64_t a_row_bytes, int 
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
 
+    const __amdgpu_buffer_rsrc_t bb = nt_buffer(b, INT64_MAX), ba0 = nt_buffer(a, INT64_MAX);
     auto issue = [&](int g) {
         char *l = smem + (g - g0) % S::NST * S::STAGE + wave * 1024;
-        const char *gb = b + (int64_t)g * (64 * PB);
-        if constexpr (!TRA) {
-            const char *ga = a + (int64_t)g * (64 * PA);
+        // (TRA: rows behind the last one lie outside the descriptor and arrive as zeros)
+        const __amdgpu_buffer_rsrc_t ba =
+            TRA ? nt_buffer(a + 32 * (int64_t)g * a_row_bytes, (int64_t)(a_rows - 32 * g) * a_row_bytes) : ba0;
 #pragma unroll
-            for (int q = 0; q < QA; ++q)
-                __builtin_amdgcn_global_load_lds((glb_void *)(ga + aoff[q]), (lds_void *)(l + q * (NW * 1024)), 16, 0, 0);
-        } else {
-#pragma unroll
-            for (int q = 0; q < QA; ++q) {
-                const int k = ((q * NW + wave) * 64 + lane) / (S::TA / 4);
-                const char *ga = a + (int64_t)min(32 * g + k, a_rows - 1) * a_row_bytes;
-                __builtin_amdgcn_global_load_lds((glb_void *)(ga + aoff[q]), (lds_void *)(l + q * (NW * 1024)), 16, 0, 0);
-            }
-        }
+        for (int q = 0; q < QA; ++q)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(ba, (nt_lds *)(l + q * (NW * 1024)), 16, aoff[q],
+                                                     TRA ? 0u : (unsigned)g * (64 * PA), 0, 0);
 #pragma unroll
         for (int q = 0; q < QB; ++q)
-            __builtin_amdgcn_global_load_lds((glb_void *)(gb + boff[q]), (lds_void *)(l + S::A_BYTES + q * (NW * 1024)), 16,
-                                             0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(bb, (nt_lds *)(l + S::A_BYTES + q * (NW * 1024)), 16, boff[q],
+                                                     (unsigned)g * (64 * PB), 0, 0);
     };
     const int frow = lane & 31, fhalf = lane >> 5;
+    unsigned tr_off[4];
+    if constexpr (TRA) {                           // row k of the first step, part q & 1 of block q >> 1 (of this wave)
+        const int k = 8 * fhalf + ((lane >> 2) & 3), unit = S::TA / S::WR / 16 * wr;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            tr_off[q] = k * (S::TA * 4) + ((unit + q) ^ (k & 3)) * 64 + (frow >> 4) * 32 + (lane & 3) * 8;
+    }
 #pragma unroll
     for (int s = 0; s < S::NST - 1; ++s)
         if (g0 + s < g1) issue(g0 + s);
@@ -147,26 +194,19 @@ __device__ __forceinline__ void nt_tile(const char *a, int64_t a_row_bytes, int 
                 for (int p = 0; p < PB; ++p)
                     fb[j][p] = *(const V *)(lb + row * (64 * PB) + nt_swizzle<PB>(row, 4 * p + 2 * kk + fhalf) * 16);
             }
+            if constexpr (TRA) {
+                unsigned at[4];
 #pragma unroll
-            for (int i = 0; i < S::FA; ++i) {
-                if constexpr (!TRA) {
+                for (int q = 0; q < 4; ++q) at[q] = (unsigned)(uintptr_t)(nt_lds *)la + tr_off[q];
+                if (kk == 0) nt_read_turned<S::FA, 4 * (S::TA * 4), 0>(at, fa);
+                else nt_read_turned<S::FA, 4 * (S::TA * 4), 1>(at, fa);
+            } else {
+#pragma unroll
+                for (int i = 0; i < S::FA; ++i) {
                     const int row = S::TA / S::WR * wr + 32 * i + frow;
 #pragma unroll
                     for (int p = 0; p < PA; ++p)
                         fa[i][p] = *(const V *)(la + row * (64 * PA) + nt_swizzle<PA>(row, 4 * p + 2 * kk + fhalf) * 16);
-                } else {
-                    // sixteen lanes turn a 4 (k) x 16 block: lane l addresses 8 B of row l / 4 and receives column l
-                    const int k = 16 * kk + 8 * fhalf + ((lane >> 2) & 3), group = S::TA / S::WR / 32 * wr + i;
-#pragma unroll
-                    for (int p = 0; p < PA; ++p) {
-                        const char *at = la + k * (S::TA * 4) + ((2 * group + p) ^ (k & 3)) * 64 + (frow >> 4) * 32 +
-                                         (lane & 3) * 8;
-                        union { s16x4 h[2]; V v; } u;
-                        u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)at);
-                        u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                            (__attribute__((address_space(3))) s16x4 *)(at + 4 * (S::TA * 4)));
-                        fa[i][p] = u.v;
-                    }
                 }
             }
 #pragma unroll
@@ -184,6 +224,7 @@ __device__ __forceinline__ void nt_tile(const char *a, int64_t a_row_bytes, int 
                 }
         }
     }
+#endif
 }
 
 // Row (0 ... 31) of accumulator element r of a 32 x 32 block; the column is lane & 31.

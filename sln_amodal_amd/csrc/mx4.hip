@@ -7,8 +7,8 @@
 // is every sum they enter.
 //
 // Memory: codes, two per byte, the lower nibble first; a row is padded with zero codes to whole steps of MX_STEP = 256
-// values (128 B: one cache line and one LDS-DMA row); scales, one byte s + 127 per block, row pitch Kp / 32.  Padding
-// blocks have scale code 0.
+// values (128 B: one cache line and one LDS-DMA row); scales, one byte s + 127 per block, [Kp / 256][R][8] (mx_scale_at).
+// Padding blocks have scale code 0.
 //
 // Product y[m][n] = act(sum_k a[m][k] b[n][k] * scale[n] + bias[n]) on v_mfma_scale_f32_32x32x64_f8f6f4 /
 // 16x16x128: a lane's operand is 32 codes of ONE row = one block, with that block's scale: nothing is unpacked, the
@@ -47,7 +47,7 @@ struct MxRound {
     const void *x;
     unsigned *codes;
     uint8_t *scales;
-    int64_t stride;
+    int64_t stride, R, r0;               // rows of the whole matrix, first row of this job
     unsigned threads, per_row;
     int K, vec;
 };
@@ -63,7 +63,7 @@ __device__ __forceinline__ void mx_round8(const MxRound &p, unsigned at) {
     a = max(a, (unsigned)__shfl_xor((int)a, 2));
     const unsigned sc = mx_scale_code(a);
     p.codes[at] = mx_codes8(v, sc);
-    if ((c & 3) == 0) p.scales[at >> 2] = (uint8_t)sc;
+    if ((c & 3) == 0) p.scales[mx_scale_at(p.R, p.r0 + row, (int)(c >> 2))] = (uint8_t)sc;
 }
 
 // 4 (2) B read and 0.53 B written per value: bound by the read (1600 x 12544 f32: 14.6 us = 6.2 TB/s, the input in the
@@ -77,26 +77,36 @@ __global__ __launch_bounds__(256) void mx4_round_kernel(const MxRound a, const M
 
 template <typename T>
 __global__ __launch_bounds__(256) void mx4_values_kernel(const unsigned *__restrict__ codes,
-                                                         const uint8_t *__restrict__ scales, unsigned rows, int K,
-                                                         unsigned per_row, T *__restrict__ out, int vec) {
+                                                         const uint8_t *__restrict__ scales, int64_t R, int64_t r0,
+                                                         unsigned rows, int K, unsigned per_row, T *__restrict__ out,
+                                                         int vec) {
     const unsigned at = blockIdx.x * 256u + threadIdx.x;
     if (at >= rows * per_row) return;
     const unsigned row = at / per_row, c = at - row * per_row;
     if ((int)c * 8 >= K) return;
     float v[8];
-    mx_values8(codes[at], scales[at >> 2], v);
+    mx_values8(codes[at], scales[mx_scale_at(R, r0 + row, (int)(c >> 2))], v);
     mx_store8(out + (int64_t)row * K, (int)c * 8, K, vec, v);
 }
 
 // ------------------------------------------------------------------------------------------------ product, many rows
-// Tile 128 x 128, four waves of 64 x 64; a step is 256 values of k = 128 B of every row, two LDS stages of 32 KB filled by
-// DMA (two workgroups per CU).  The order in which the eight blocks of a step enter the sum is free, so the two
-// halves of a wave take blocks 0 ... 3 and 4 ... 7: a lane's four scales are one aligned dword of the scale row, and the
-// instruction picks its byte.
-#define MX_TILE 128
+// Tile TA x TB, WR x WC waves; a step is 256 values of k = 128 B of every row, two LDS stages filled by DMA.  The order in
+// which the eight blocks of a step enter the sum is free, so the two halves of a wave take blocks 0 ... 3 and 4 ... 7: a
+// lane's four scales are one aligned dword of the scale row, and the instruction picks its byte.  The scales come by DMA
+// too: with ordinary loads among the DMA's the compiler waits for all of them before the first LDS read of a step, and
+// nothing overlaps (16000 x 12544 x 1024: 155 us instead of MXNEW).
+template <int TA_, int TB_, int WR_, int WC_>
+struct MxShape {
+    static constexpr int TA = TA_, TB = TB_, WR = WR_, WC = WC_, NW = WR * WC, THREADS = NW * 64;
+    static constexpr int FA = TA / WR / 32, FB = TB / WC / 32, QA = TA / 8 / NW, QB = TB / 8 / NW;
+    static constexpr int SCALES = (TA + TB) * 128, STAGE = SCALES + (TA + TB) * 8, LDS = 2 * STAGE;
+    static_assert(TA == 32 * NW && TB == 32 * NW, "a wave fetches the scales of 32 rows of either side");
+};
+typedef MxShape<128, 128, 2, 2> MxSmall;           // two workgroups per CU
+typedef MxShape<256, 256, 2, 4> MxLarge;           // one
 struct MxGemm {
     const uint8_t *a, *b, *sa, *sb;
-    int64_t a_pitch, b_pitch;          // bytes per code row; scales: / 16
+    int64_t a_pitch, b_pitch;          // bytes per code row
     int M, N, steps, nsplit;
     const float *scale, *bias;
     void *y;
@@ -114,85 +124,96 @@ __device__ __forceinline__ void mx_finish(const MxGemm &p, int m, int n, float v
     ((T *)p.y)[(int64_t)m * p.N + n] = (T)mx_act(v, p.scale ? p.scale[n] : 1.f, p.bias ? p.bias[n] : 0.f, p.relu);
 }
 
+// (a vector type: behind a read of HIP's int4 the compiler waits for the DMA in flight)
 __device__ __forceinline__ i32x8 mx_frag(const char *at) {
-    const int4 v = *(const int4 *)at;
+    typedef int i32x4 __attribute__((ext_vector_type(4)));
+    const i32x4 v = *(const i32x4 *)at;
     const i32x8 r = {v.x, v.y, v.z, v.w, 0, 0, 0, 0};
     return r;
 }
 
-template <typename T>
-__global__ __launch_bounds__(256, 2) void mx4_product_kernel(const MxGemm p, int tiles) {
-    typedef __attribute__((address_space(3))) void lds_void;
-    typedef __attribute__((address_space(1))) const void glb_void;
-    constexpr int OPB = MX_TILE * 128, STAGE = 2 * OPB;
-    __shared__ __attribute__((aligned(128))) char smem[2 * STAGE];
+template <typename T, typename S>
+__global__ __launch_bounds__(S::THREADS, S::THREADS == 256 ? 2 : 1) void mx4_product_kernel(const MxGemm p, int tiles) {
+#ifdef __HIP_DEVICE_COMPILE__                      // (the host pass knows no buffer descriptors in templates)
+    constexpr int NW = S::NW, OPA = S::TA * 128;
+    __shared__ __attribute__((aligned(128))) char smem[S::LDS];
     const int at = nt_xcd_order(blockIdx.x, tiles);
-    const int tn = (p.N + MX_TILE - 1) / MX_TILE;
+    const int tn = (p.N + S::TB - 1) / S::TB;
     const int split = at % p.nsplit, tile = at / p.nsplit;
-    const int m0 = tile / tn * MX_TILE, n0 = tile % tn * MX_TILE;
+    const int m0 = tile / tn * S::TA, n0 = tile % tn * S::TB;
     const int s0 = (int)((int64_t)p.steps * split / p.nsplit), s1 = (int)((int64_t)p.steps * (split + 1) / p.nsplit);
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, wr = wave >> 1, wc = wave & 1;
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, wr = wave / S::WC, wc = wave % S::WC;
     const int half = lane >> 5, frow = lane & 31;
-    unsigned aoff[4], boff[4];
+    unsigned aoff[S::QA], boff[S::QB];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        const int slot = (q * 4 + wave) * 64 + lane, row = slot >> 3, c = (slot & 7) ^ ((row >> 1) & 7);
+    for (int q = 0; q < S::QA; ++q) {
+        const int slot = (q * NW + wave) * 64 + lane, row = slot >> 3, c = (slot & 7) ^ ((row >> 1) & 7);
         aoff[q] = (unsigned)(min(row, p.M - 1 - m0) * p.a_pitch + c * 16);
+    }
+#pragma unroll
+    for (int q = 0; q < S::QB; ++q) {
+        const int slot = (q * NW + wave) * 64 + lane, row = slot >> 3, c = (slot & 7) ^ ((row >> 1) & 7);
         boff[q] = (unsigned)(min(row, p.N - 1 - n0) * p.b_pitch + c * 16);
     }
     const uint8_t *ga = p.a + (int64_t)m0 * p.a_pitch, *gb = p.b + (int64_t)n0 * p.b_pitch;
+    // scales: lane l of wave w fetches dword l & 1 of rows 32 w + l / 2
+    const int srow = 32 * wave + (lane >> 1);
+    const unsigned qa = (unsigned)min(m0 + srow, p.M - 1) * 8u + (lane & 1) * 4u;
+    const unsigned qb = (unsigned)min(n0 + srow, p.N - 1) * 8u + (lane & 1) * 4u;
+    const __amdgpu_buffer_rsrc_t ra = nt_buffer(ga, INT64_MAX), rb = nt_buffer(gb, INT64_MAX);
     auto issue = [&](int s, int stage) {
-        char *l = smem + stage * STAGE + wave * 1024;
+        char *l = smem + stage * S::STAGE + wave * 1024;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            __builtin_amdgcn_global_load_lds((glb_void *)(ga + (int64_t)s * 128 + aoff[q]), (lds_void *)(l + q * 4096),
-                                             16, 0, 0);
-            __builtin_amdgcn_global_load_lds((glb_void *)(gb + (int64_t)s * 128 + boff[q]),
-                                             (lds_void *)(l + OPB + q * 4096), 16, 0, 0);
-        }
+        for (int q = 0; q < S::QA; ++q)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (nt_lds *)(l + q * (NW * 1024)), 16, aoff[q], (unsigned)s * 128u, 0,
+                                                     0);
+#pragma unroll
+        for (int q = 0; q < S::QB; ++q)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (nt_lds *)(l + OPA + q * (NW * 1024)), 16, boff[q],
+                                                     (unsigned)s * 128u, 0, 0);
+        char *ls = smem + stage * S::STAGE + S::SCALES + wave * 256;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(nt_buffer(p.sa + (int64_t)s * p.M * 8, INT64_MAX), (nt_lds *)ls, 4, qa, 0, 0,
+                                                 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(nt_buffer(p.sb + (int64_t)s * p.N * 8, INT64_MAX),
+                                                 (nt_lds *)(ls + S::TA * 8), 4, qb, 0, 0, 0);
     };
-    // this lane's scale dwords: row 32 i + frow of the wave's half tiles
-    const uint8_t *sa[2], *sb[2];
+    f32x16 acc[S::FA][S::FB];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        sa[i] = p.sa + (int64_t)min(m0 + 64 * wr + 32 * i + frow, p.M - 1) * (p.a_pitch >> 4) + 4 * half;
-        sb[i] = p.sb + (int64_t)min(n0 + 64 * wc + 32 * i + frow, p.N - 1) * (p.b_pitch >> 4) + 4 * half;
-    }
-    f32x16 acc[2][2];
+    for (int i = 0; i < S::FA; ++i)
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int j = 0; j < S::FB; ++j)
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
-    int xa[2], xb[2];
-    auto scales = [&](int s) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            xa[i] = *(const int *)(sa[i] + (int64_t)s * 8);
-            xb[i] = *(const int *)(sb[i] + (int64_t)s * 8);
-        }
-    };
-    if (s0 < s1) { scales(s0); issue(s0, 0); }
+    if (s0 < s1) issue(s0, 0);
     for (int s = s0; s < s1; ++s) {
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         const int stage = (s - s0) & 1;
-        const int ca[2] = {xa[0], xa[1]}, cb[2] = {xb[0], xb[1]};
-        if (s + 1 < s1) { scales(s + 1); issue(s + 1, stage ^ 1); }
-        const char *la = smem + stage * STAGE, *lb = la + OPB;
+        if (s + 1 < s1) issue(s + 1, stage ^ 1);
+        const char *la = smem + stage * S::STAGE, *lb = la + OPA;
+        int ca[S::FA], cb[S::FB];
+#pragma unroll
+        for (int i = 0; i < S::FA; ++i)
+            ca[i] = *(const int *)(la + S::SCALES + (S::TA / S::WR * wr + 32 * i + frow) * 8 + 4 * half);
+#pragma unroll
+        for (int j = 0; j < S::FB; ++j)
+            cb[j] = *(const int *)(la + S::SCALES + (S::TA + S::TB / S::WC * wc + 32 * j + frow) * 8 + 4 * half);
 #define MX_QUARTER(Q)                                                                                        \
         {                                                                                                    \
-            i32x8 fa[2], fb[2];                                                                              \
-            _Pragma("unroll") for (int i = 0; i < 2; ++i) {                                                  \
-                const int ra = 64 * wr + 32 * i + frow, rb = 64 * wc + 32 * i + frow;                        \
-                fa[i] = mx_frag(la + ra * 128 + (((4 * half + Q) ^ ((ra >> 1) & 7)) << 4));                         \
-                fb[i] = mx_frag(lb + rb * 128 + (((4 * half + Q) ^ ((rb >> 1) & 7)) << 4));                         \
+            i32x8 fa[S::FA], fb[S::FB];                                                                      \
+            _Pragma("unroll") for (int j = 0; j < S::FB; ++j) {                                              \
+                const int row = S::TB / S::WC * wc + 32 * j + frow;                                          \
+                fb[j] = mx_frag(lb + row * 128 + (((4 * half + Q) ^ ((row >> 1) & 7)) << 4));                \
             }                                                                                                \
-            _Pragma("unroll") for (int i = 0; i < 2; ++i) _Pragma("unroll") for (int j = 0; j < 2; ++j)      \
-                acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fa[i], fb[j], acc[i][j], 4, 4,   \
-                                                                            Q, ca[i], Q, cb[j]);             \
+            _Pragma("unroll") for (int i = 0; i < S::FA; ++i) {                                              \
+                const int row = S::TA / S::WR * wr + 32 * i + frow;                                          \
+                fa[i] = mx_frag(la + row * 128 + (((4 * half + Q) ^ ((row >> 1) & 7)) << 4));                \
+            }                                                                                                \
+            _Pragma("unroll") for (int i = 0; i < S::FA; ++i)                                                \
+                _Pragma("unroll") for (int j = 0; j < S::FB; ++j)                                            \
+                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fa[i], fb[j], acc[i][j], 4,  \
+                                                                                4, Q, ca[i], Q, cb[j]);      \
         }
         MX_QUARTER(0)
         MX_QUARTER(1)
@@ -200,24 +221,29 @@ __global__ __launch_bounds__(256, 2) void mx4_product_kernel(const MxGemm p, int
         MX_QUARTER(3)
 #undef MX_QUARTER
     }
-    const int row0 = m0 + 64 * wr, col0 = n0 + 64 * wc + frow;
-    const bool inside = row0 + 64 <= p.M && col0 - frow + 64 <= p.N;              // (uniform: no test per element)
-    float *slab = p.nsplit > 1 ? p.slab + (int64_t)split * p.M * p.N : nullptr;
+    // a lane's elements are rows row0 + 32 i + (r & 3) + 8 (r >> 2): uniform steps from one address
+    const int row0 = m0 + S::TA / S::WR * wr + 4 * half, col0 = n0 + S::TB / S::WC * wc + frow;
+    const bool inside = m0 + S::TA <= p.M && n0 + S::TB <= p.N;                   // (uniform: no test per element)
+    const int64_t first = (int64_t)row0 * p.N + col0;
+    const bool part = p.nsplit > 1;
+    float *slab = part ? p.slab + (int64_t)split * p.M * p.N + first : nullptr;
+    T *y = (T *)p.y + first;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const int n = col0 + 32 * j;
-        const float cs = p.scale ? p.scale[min(n, p.N - 1)] : 1.f, cb = p.bias ? p.bias[min(n, p.N - 1)] : 0.f;
+    for (int j = 0; j < S::FB; ++j) {
+        const int n = min(col0 + 32 * j, p.N - 1);
+        const float cs = !part && p.scale ? p.scale[n] : 1.f, cb = !part && p.bias ? p.bias[n] : 0.f;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < S::FA; ++i)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const int m = row0 + 32 * i + nt_acc_row(r, lane);
-                if (!inside && (m >= p.M || n >= p.N)) continue;
-                const int64_t e = (int64_t)m * p.N + n;
-                if (slab) slab[e] = acc[i][j][r];
-                else ((T *)p.y)[e] = (T)mx_act(acc[i][j][r], cs, cb, p.relu);
+                const int down = 32 * i + (r & 3) + 8 * (r >> 2);
+                if (!inside && (row0 + down >= p.M || col0 + 32 * j >= p.N)) continue;
+                const int64_t e = (int64_t)down * p.N + 32 * j;
+                if (part) slab[e] = acc[i][j][r];
+                else y[e] = (T)mx_act(acc[i][j][r], cs, cb, p.relu);
             }
     }
+#endif
 }
 
 // The cuts of the contraction, added in order, and the epilogue.
@@ -248,12 +274,12 @@ __global__ __launch_bounds__(256) void mx4_rows_kernel(const MxGemm p, const T *
     const int s0 = (int)((int64_t)steps * split / cuts), s1 = (int)((int64_t)steps * (split + 1) / cuts);
     const int wrow = min(n0 + r16, p.N - 1);
     const uint8_t *wb = p.b + (int64_t)wrow * p.b_pitch + blk * 16;
-    const uint8_t *ws = p.sb + (int64_t)wrow * (p.b_pitch >> 4) + blk;
+    const uint8_t *ws = p.sb + (int64_t)wrow * 8 + blk;
     const T *xr = x + (int64_t)min(r16, p.M - 1) * stride;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
     for (int s = s0; s < s1; ++s) {
         const i32x8 fw = mx_frag((const char *)wb + (int64_t)s * 64);
-        const int sw = ws[(int64_t)s * 4];
+        const int sw = ws[(int64_t)(s >> 1) * p.N * 8 + (s & 1) * 4];
         i32x8 fx = {0, 0, 0, 0, 0, 0, 0, 0};
         int sx = 0;
         const int k = s * 128 + blk * 32;
@@ -288,14 +314,16 @@ static inline int mx_bad_dtype(int d) { return d != SLN_DTYPE_F32 && d != SLN_DT
 extern "C" int64_t sln_mx4_row_values(int64_t K) { return K < 0 ? 0 : (K + MX_STEP - 1) / MX_STEP * MX_STEP; }
 
 // Rows [r, r + n) of a matrix, n * per_row < 2^31.
-static MxRound mx_round_job(const void *x, int es, int64_t stride, int64_t r, int64_t n, int K, uint8_t *codes,
-                            uint8_t *scales) {
+static MxRound mx_round_job(const void *x, int es, int64_t stride, int64_t R, int64_t r, int64_t n, int K,
+                            uint8_t *codes, uint8_t *scales) {
     const int64_t kp = sln_mx4_row_values(K);
     MxRound p;
     p.x = (const char *)x + r * stride * es;
     p.codes = (unsigned *)(codes + r * (kp / 2));
-    p.scales = scales + r * (kp / 32);
+    p.scales = scales;
     p.stride = stride;
+    p.R = R;
+    p.r0 = r;
     p.per_row = (unsigned)(kp / 8);
     p.threads = (unsigned)n * p.per_row;
     p.K = K;
@@ -310,7 +338,7 @@ static void mx_round(const void *x, int64_t stride, int64_t R, int K, uint8_t *c
     const int64_t most = mx_round_rows(K);
     MxRound none = {};
     for (int64_t r = 0; r < R; r += most) {
-        const MxRound a = mx_round_job(x, sizeof(T), stride, r, R - r < most ? R - r : most, K, codes, scales);
+        const MxRound a = mx_round_job(x, sizeof(T), stride, R, r, R - r < most ? R - r : most, K, codes, scales);
         const MxRound b = also && r == 0 ? *also : none;
         const unsigned blocks = (a.threads + 255u) / 256u;
         hipLaunchKernelGGL((mx4_round_kernel<T>), dim3(blocks + (b.threads + 255u) / 256u), dim3(256), 0, st, a, b, blocks);
@@ -339,7 +367,7 @@ static void mx_values(const uint8_t *codes, const uint8_t *scales, int64_t R, in
     for (int64_t r = 0; r < R; r += max_rows) {
         const unsigned n = (unsigned)(R - r < max_rows ? R - r : max_rows);
         hipLaunchKernelGGL((mx4_values_kernel<T>), dim3((n * per_row + 255) / 256), dim3(256), 0, st,
-                           (const unsigned *)(codes + r * (kp / 2)), scales + r * (kp / 32), n, K, per_row,
+                           (const unsigned *)(codes + r * (kp / 2)), scales, R, r, n, K, per_row,
                            (T *)out + r * K, vec);
     }
 }
@@ -367,9 +395,11 @@ static inline int mx_cuts(int64_t tiles, int64_t target, int64_t steps, int64_t 
 static inline int mx_rows_cuts(int64_t N, int64_t K) {
     return mx_cuts((N + 15) / 16, 512, 2 * ((K + MX_STEP - 1) / MX_STEP), 8);
 }
+static inline int64_t mx_tiles(int64_t M, int64_t N, int tile) { return ((M + tile - 1) / tile) * ((N + tile - 1) / tile); }
+// Large tiles where three quarters of the CUs get one (16000 x 12544 x 1024: 255 us with 128 x 128).
+static inline bool mx_large(int64_t M, int64_t N) { return mx_tiles(M, N, 256) >= 192; }
 static inline int mx_product_cuts(int64_t M, int64_t N, int64_t K) {
-    const int64_t tiles = ((M + MX_TILE - 1) / MX_TILE) * ((N + MX_TILE - 1) / MX_TILE);
-    return mx_cuts(tiles, 512, (K + MX_STEP - 1) / MX_STEP, 2);
+    return mx_large(M, N) ? 1 : mx_cuts(mx_tiles(M, N, 128), 512, (K + MX_STEP - 1) / MX_STEP, 2);
 }
 
 extern "C" size_t sln_mx4_product_workspace_bytes(int64_t M, int64_t N, int64_t K, int rounded) {
@@ -387,7 +417,7 @@ static void mx_join(const MxGemm &p, hipStream_t st) {
 
 static int mx_gemm(MxGemm &p, const uint8_t *b, const uint8_t *sb, int64_t M, int64_t N, int64_t K, const float *scale,
                    const float *bias, int relu, void *y, int nsplit, void *ws, size_t ws_bytes) {
-    if (M > (1 << 30) || N > (1 << 30) || K > MX_MAX_K) return SLN_ERR_UNSUPPORTED;
+    if (M > (1 << 28) || N > (1 << 28) || K > MX_MAX_K) return SLN_ERR_UNSUPPORTED;   // rows of scales below 2^32 B
     if (!b || !sb || !y || ((uintptr_t)b & 15) || ((uintptr_t)sb & 7)) return SLN_ERR_INVALID_ARG;
     p.b = b; p.sb = sb; p.b_pitch = sln_mx4_row_values(K) / 2;
     p.M = (int)M; p.N = (int)N; p.steps = (int)(sln_mx4_row_values(K) / MX_STEP);
@@ -410,12 +440,18 @@ extern "C" int sln_mx4_product(const uint8_t *a_codes, const uint8_t *a_scales, 
     if (rc != SLN_OK) return rc;
     if (!a_codes || !a_scales || ((uintptr_t)a_codes & 15) || ((uintptr_t)a_scales & 7)) return SLN_ERR_INVALID_ARG;
     p.a = a_codes; p.sa = a_scales; p.a_pitch = p.b_pitch;
-    const int64_t tiles = ((M + MX_TILE - 1) / MX_TILE) * ((N + MX_TILE - 1) / MX_TILE) * p.nsplit;
+    const bool large = mx_large(M, N);
+    const int64_t tiles = mx_tiles(M, N, large ? 256 : 128) * p.nsplit;
     if (tiles > (1 << 30)) return SLN_ERR_UNSUPPORTED;
     sln_enter();
     hipStream_t st = (hipStream_t)stream;
 #define MX_GO(T)                                                                                             \
-    hipLaunchKernelGGL((mx4_product_kernel<T>), dim3((unsigned)tiles), dim3(256), 0, st, p, (int)tiles);     \
+    if (large)                                                                                               \
+        hipLaunchKernelGGL((mx4_product_kernel<T, MxLarge>), dim3((unsigned)tiles), dim3(MxLarge::THREADS),  \
+                           0, st, p, (int)tiles);                                                            \
+    else                                                                                                     \
+        hipLaunchKernelGGL((mx4_product_kernel<T, MxSmall>), dim3((unsigned)tiles), dim3(MxSmall::THREADS),  \
+                           0, st, p, (int)tiles);                                                            \
     mx_join<T>(p, st)
     if (dtype == SLN_DTYPE_F32) { MX_GO(float); }
     else if (dtype == SLN_DTYPE_BF16) { MX_GO(__bf16); }
@@ -468,7 +504,7 @@ extern "C" int sln_mx4_linear_fwd(const void *x, int dtype, int64_t M, int64_t K
     MxRound job;
     if (w) {
         if (x_codes && N <= mx_round_rows(K)) {
-            job = mx_round_job(w, 4, w_stride, 0, N, (int)K, w_codes, w_scales);
+            job = mx_round_job(w, 4, w_stride, N, 0, N, (int)K, w_codes, w_scales);
             also = &job;
         } else {
             mx_round<float>(w, w_stride, N, (int)K, w_codes, w_scales, nullptr, st);

@@ -119,7 +119,7 @@ __device__ __forceinline__ void mg_turn(const unsigned *codes, const uint8_t *sc
         float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
         if (r0 + i < R) {                      // (k < kp: the padded row holds whole tiles of 64)
             const int64_t at = (int64_t)(r0 + i) * (kp / 8) + k / 8;
-            mx_values8(codes[at], scales[at >> 2], v);
+            mx_values8(codes[at], scales[mx_scale_at(R, r0 + i, k >> 5)], v);
         }
 #pragma unroll
         for (int q = 0; q < 8; ++q) z[i * MG_PITCH + (e & 7) * 8 + q] = v[q];

@@ -42,8 +42,9 @@ def _rows(t, name):
 
 
 class Mx4Tensor(object):
-    """A matrix held in 4 bits: `codes` uint8 [R, Kp / 2] (Kp = K rounded up to 256) and `scales` uint8 [R, Kp / 32], both
-    views of one buffer; the `shape` and `dtype` of what it was made from.  Its rows are the last axis' vectors."""
+    """A matrix held in 4 bits, in one buffer: `codes` uint8 [R, Kp / 2] (Kp = K rounded up to 256) and `scales` uint8
+    [R, Kp / 32] (held step by step: [Kp / 256][R][8]); the `shape` and `dtype` of what it was made from.  Its rows are the
+    last axis' vectors."""
     __slots__ = ("data", "rows", "shape", "dtype")
 
     def __init__(self, data, rows, shape, dtype):
@@ -61,7 +62,7 @@ class Mx4Tensor(object):
     @property
     def scales(self):
         kp = _padded(self.shape[-1])
-        return self.data[self.rows * (kp // 2):].view(self.rows, kp // 32)
+        return self.data[self.rows * (kp // 2):].view(kp // 256, self.rows, 8).permute(1, 0, 2).reshape(self.rows, kp // 32)
 
     def dequantize(self, dtype=None):
         """The values that the codes stand for, in `dtype` (default: the source's; exact in float32 and bfloat16)."""
