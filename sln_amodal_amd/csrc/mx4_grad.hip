@@ -146,10 +146,11 @@ __global__ __launch_bounds__(256) void mx4_grad_prep_kernel(const MgPrep p) {
     else mg_turn(p.x_codes, p.x_scales, p.M, p.K, p.xt, blockIdx.x - p.split - p.turn_w, z);
 }
 
-// 128 x 128 tiles, two workgroups per CU
-template <int P>
-struct MgShape : NtShape<P, 1, 128, 128, 2, 2, 2> {};
-#define MG_TILE 128
+// Where there are enough of them, 128 x 256 tiles of eight waves, two workgroups per CU: sixteen waves hide each other's
+// loads and stores (1600 x 12544 x 1024, three parts, both gradients: 230 us; 128 x 128 tiles of four waves 285, 256 x 256
+// tiles, one workgroup per CU, 281, though their k-loop alone is the fastest).
+template <int P> struct MgSmall : NtShape<P, 1, 128, 128, 2, 2, 2> {};
+template <int P> struct MgLarge : NtShape<P, 1, 128, 256, 2, 4, 2> {};
 
 struct MgProduct {
     const char *a, *b;            // parts rows: a [RA] of P parts, b [RB] of one
@@ -160,57 +161,59 @@ struct MgProduct {
     float *slab;                  // nsplit > 1: [nsplit][RA][RB]
 };
 
-template <typename T>
-__device__ __forceinline__ void mg_finish(const MgProduct &p, int i, int64_t at, float v) {
-    ((T *)p.c)[at] = (T)(p.row_scale ? v * p.row_scale[i] : v);
-}
-
-template <typename T, int P>
+template <typename T, typename S>
 __device__ __forceinline__ void mg_product(const MgProduct &p, int at, char *smem) {
-    const int ta = (p.RA + MG_TILE - 1) / MG_TILE;
+    const int ta = (p.RA + S::TA - 1) / S::TA;
     const int split = at % p.nsplit, tile = at / p.nsplit;
-    const int i0 = tile % ta * MG_TILE, j0 = tile / ta * MG_TILE;
-    const int64_t ra = (int64_t)p.groups * 64 * P, rb = (int64_t)p.groups * 64;
+    const int i0 = tile % ta * S::TA, j0 = tile / ta * S::TB;
+    const int64_t ra = (int64_t)p.groups * 64 * S::PA, rb = (int64_t)p.groups * 64;
     const int g0 = (int)((int64_t)p.groups * split / p.nsplit), g1 = (int)((int64_t)p.groups * (split + 1) / p.nsplit);
-    f32x16 acc[2][2];
-    nt_tile<MgShape<P>, b16x8, NT_EXACTB, false>(p.a + i0 * ra, ra, p.RA - i0, 0, p.b + j0 * rb, rb, p.RB - j0, g0, g1, smem, acc);
+    f32x16 acc[S::FA][S::FB];
+    nt_tile<S, b16x8, NT_EXACTB, false>(p.a + i0 * ra, ra, p.RA - i0, 0, p.b + j0 * rb, rb, p.RB - j0, g0, g1, smem, acc);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int row0 = i0 + 64 * (wave >> 1), col0 = j0 + 64 * (wave & 1) + (lane & 31);
-    const bool inside = row0 + 64 <= p.RA && col0 - (lane & 31) + 64 <= p.RB;     // (uniform: no test per element)
-    float *slab = p.nsplit > 1 ? p.slab + (int64_t)split * p.RA * p.RB : nullptr;
+    // a lane's elements are rows row0 + 32 i + (r & 3) + 8 (r >> 2): uniform steps from one address
+    const int row0 = i0 + S::TA / S::WR * (wave / S::WC) + 4 * (lane >> 5);
+    const int col0 = j0 + S::TB / S::WC * (wave % S::WC) + (lane & 31);
+    const bool inside = i0 + S::TA <= p.RA && j0 + S::TB <= p.RB;                 // (uniform: no test per element)
+    const int64_t first = (int64_t)row0 * p.RB + col0;
+    const bool part = p.nsplit > 1;
+    float *slab = part ? p.slab + (int64_t)split * p.RA * p.RB + first : nullptr;
+    T *c = (T *)p.c + first;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < S::FA; ++i) {
         float rs[16];                              // (loads ahead of the stores, which the compiler may not pass)
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-            rs[r] = p.row_scale && !slab ? p.row_scale[min(row0 + 32 * i + nt_acc_row(r, lane), p.RA - 1)] : 1.f;
+            rs[r] = p.row_scale && !part ? p.row_scale[min(row0 + 32 * i + (r & 3) + 8 * (r >> 2), p.RA - 1)] : 1.f;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int col = col0 + 32 * j;
+        for (int j = 0; j < S::FB; ++j)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const int row = row0 + 32 * i + nt_acc_row(r, lane);
-                if (!inside && (row >= p.RA || col >= p.RB)) continue;
-                const int64_t e = (int64_t)row * p.RB + col;
-                if (slab) slab[e] = acc[i][j][r];
-                else ((T *)p.c)[e] = (T)(acc[i][j][r] * rs[r]);
+                const int down = 32 * i + (r & 3) + 8 * (r >> 2);
+                if (!inside && (row0 + down >= p.RA || col0 + 32 * j >= p.RB)) continue;
+                const int64_t e = (int64_t)down * p.RB + 32 * j;
+                if (part) slab[e] = acc[i][j][r];
+                else c[e] = (T)(acc[i][j][r] * rs[r]);
             }
-        }
     }
 }
 
-// Both products and the bias sums in one launch (x: gx, w: gw; tiles = 0: not wanted).
-template <typename T, int P>
-__global__ __launch_bounds__(256, 2) void mx4_grad_product_kernel(const MgProduct x, const MgProduct w,
-                                                                  const float *__restrict__ bias_part, int bias_blocks,
-                                                                  int N, float *__restrict__ gb) {
-    __shared__ __attribute__((aligned(128))) char smem[MgShape<P>::LDS];
-    if (blockIdx.x < x.tiles) {
-        mg_product<T, P>(x, nt_xcd_order(blockIdx.x, x.tiles), smem);
-    } else if (blockIdx.x < x.tiles + w.tiles) {
-        mg_product<float, P>(w, nt_xcd_order(blockIdx.x - x.tiles, w.tiles), smem);
+// Both products (if their tiles are alike) and the bias sums in one launch (x: gx, w: gw; tiles = 0: not here); the tiles with the longer
+// contraction first.
+template <typename T, typename S>
+__global__ __launch_bounds__(S::THREADS, S::THREADS == 256 ? 2 : 4) void mx4_grad_product_kernel(
+    const MgProduct x, const MgProduct w, const float *__restrict__ bias_part, int bias_blocks, int N,
+    float *__restrict__ gb) {
+    __shared__ __attribute__((aligned(128))) char smem[S::LDS];
+    const bool w_first = w.groups > x.groups;
+    const unsigned lead = w_first ? w.tiles : x.tiles, all = x.tiles + w.tiles;
+    if (blockIdx.x < all) {
+        const bool is_w = w_first == (blockIdx.x < lead);
+        const int at = blockIdx.x < lead ? nt_xcd_order(blockIdx.x, lead) : nt_xcd_order(blockIdx.x - lead, all - lead);
+        if (is_w) mg_product<float, S>(w, at, smem);
+        else mg_product<T, S>(x, at, smem);
     } else {                                       // partial bias sums, added in order in double
-        const int n = (blockIdx.x - x.tiles - w.tiles) * 256 + threadIdx.x;
+        const int n = (blockIdx.x - all) * S::THREADS + threadIdx.x;
         if (n >= N) return;
         double s = 0.0;
         for (int b = 0; b < bias_blocks; ++b) s += bias_part[(int64_t)b * N + n];
@@ -224,7 +227,7 @@ __device__ __forceinline__ void mg_join(const MgProduct &p, int64_t first, int64
     for (int64_t e = first; e < total; e += step) {
         float v = 0.f;
         for (int k = 0; k < p.nsplit; ++k) v += p.slab[k * total + e];
-        mg_finish<T>(p, (int)(e / p.RB), e, v);
+        ((T *)p.c)[e] = (T)(p.row_scale ? v * p.row_scale[e / p.RB] : v);
     }
 }
 template <typename T>
@@ -237,10 +240,15 @@ __global__ __launch_bounds__(256) void mx4_grad_join_kernel(const MgProduct x, c
 struct MgPlan {
     int64_t z_rows, z_cols, wt, xt, bias, slab_x, slab_w, bytes;
     int gx_cuts, gw_cuts;
+    bool gx_large, gw_large;
 };
 static inline int64_t mg_align(int64_t v) { return (v + 255) & ~(int64_t)255; }
+static inline int64_t mg_tiles(int64_t RA, int64_t RB, bool large) {
+    return ((RA + 127) / 128) * (large ? (RB + 255) / 256 : (RB + 127) / 128);
+}
+static inline bool mg_large(int64_t RA, int64_t RB) { return mg_tiles(RA, RB, true) >= 384; }   // 3/4 of the CUs' slots
 static inline int mg_cuts(int64_t RA, int64_t RB, int64_t groups) {
-    const int64_t tiles = ((RA + MG_TILE - 1) / MG_TILE) * ((RB + MG_TILE - 1) / MG_TILE);
+    const int64_t tiles = mg_tiles(RA, RB, false);
     int64_t c = 512 / (tiles < 1 ? 1 : tiles);
     if (c > groups / 8) c = groups / 8;
     if (c > 32) c = 32;
@@ -248,8 +256,11 @@ static inline int mg_cuts(int64_t RA, int64_t RB, int64_t groups) {
 }
 static void mg_plan(int64_t M, int64_t N, int64_t K, int parts, bool gx, bool gw, bool gb, MgPlan &p) {
     int64_t at = 0;
-    p.gx_cuts = mg_cuts(M, K, (N + 31) / 32);
-    p.gw_cuts = mg_cuts(N, K, (M + 31) / 32);
+    // (each product's own rule, whatever else is wanted: its bits do not depend on that)
+    p.gx_large = mg_large(M, K);
+    p.gw_large = mg_large(N, K);
+    p.gx_cuts = p.gx_large ? 1 : mg_cuts(M, K, (N + 31) / 32);
+    p.gw_cuts = p.gw_large ? 1 : mg_cuts(N, K, (M + 31) / 32);
     p.z_rows = at; at += gx ? mg_align(M * mg_row_bytes(N, parts)) : 0;
     p.z_cols = at; at += gw ? mg_align(N * mg_row_bytes(M, parts)) : 0;
     p.wt = at; at += gx ? mg_align(K * mg_row_bytes(N, 1)) : 0;
@@ -269,13 +280,13 @@ extern "C" size_t sln_mx4_linear_bwd_workspace_bytes(int64_t M, int64_t N, int64
     return (size_t)p.bytes;
 }
 
-static MgProduct mg_job(const char *a, int64_t RA, const char *b, int64_t RB, int64_t k, int cuts, const float *row_scale,
-                        void *c, char *slab) {
+static MgProduct mg_job(const char *a, int64_t RA, const char *b, int64_t RB, int64_t k, int cuts, bool large,
+                        const float *row_scale, void *c, char *slab) {
     MgProduct p = {};
     if (!c) return p;
     p.a = a; p.b = b; p.RA = (int)RA; p.RB = (int)RB;
     p.groups = (int)((k + 31) / 32); p.nsplit = cuts;
-    p.tiles = (unsigned)(((RA + MG_TILE - 1) / MG_TILE) * ((RB + MG_TILE - 1) / MG_TILE) * cuts);
+    p.tiles = (unsigned)(mg_tiles(RA, RB, large) * cuts);
     p.row_scale = row_scale; p.c = c; p.slab = (float *)slab;
     return p;
 }
@@ -302,10 +313,28 @@ static void mg_run(const void *gy, int64_t stride, const void *y, const float *s
     p.turn_w = gx ? (unsigned)(tk * tn) : 0u;
     hipLaunchKernelGGL((mx4_grad_prep_kernel<T, P>), dim3(p.split + p.turn_w + (gw ? (unsigned)(tk * tm) : 0u)), dim3(256),
                        0, st, p);
-    const MgProduct jx = mg_job(ws + pl.z_rows, M, ws + pl.wt, K, N, pl.gx_cuts, nullptr, gx, ws + pl.slab_x);
-    const MgProduct jw = mg_job(ws + pl.z_cols, N, ws + pl.xt, K, M, pl.gw_cuts, scale, gw, ws + pl.slab_w);
-    hipLaunchKernelGGL((mx4_grad_product_kernel<T, P>), dim3(jx.tiles + jw.tiles + (gb ? (unsigned)((N + 255) / 256) : 0u)),
-                       dim3(256), 0, st, jx, jw, p.bias_part, (int)tm, (int)N, gb);
+    const MgProduct jx = mg_job(ws + pl.z_rows, M, ws + pl.wt, K, N, pl.gx_cuts, pl.gx_large, nullptr, gx,
+                                ws + pl.slab_x);
+    const MgProduct jw = mg_job(ws + pl.z_cols, N, ws + pl.xt, K, M, pl.gw_cuts, pl.gw_large, scale, gw,
+                                ws + pl.slab_w);
+    const MgProduct none = {};
+    auto launch = [&](const MgProduct &x, const MgProduct &w, bool large, float *bias) {
+        const unsigned threads = large ? 512 : 256;
+        const dim3 grid(x.tiles + w.tiles + (bias ? (unsigned)(N + threads - 1) / threads : 0u));
+        if (grid.x == 0) return;
+        if (large)
+            hipLaunchKernelGGL((mx4_grad_product_kernel<T, MgLarge<P>>), grid, dim3(threads), 0, st, x, w, p.bias_part,
+                               (int)tm, (int)N, bias);
+        else
+            hipLaunchKernelGGL((mx4_grad_product_kernel<T, MgSmall<P>>), grid, dim3(threads), 0, st, x, w, p.bias_part,
+                               (int)tm, (int)N, bias);
+    };
+    if (!gx || !gw || pl.gx_large == pl.gw_large) {
+        launch(jx, jw, gx ? pl.gx_large : gw && pl.gw_large, gb);
+    } else {
+        launch(jx, none, pl.gx_large, gb);
+        launch(none, jw, pl.gw_large, nullptr);
+    }
     const unsigned bx = mg_join_blocks(jx), bw = mg_join_blocks(jw);
     if (bx + bw) hipLaunchKernelGGL((mx4_grad_join_kernel<T>), dim3(bx + bw), dim3(256), 0, st, jx, jw, bx);
 }

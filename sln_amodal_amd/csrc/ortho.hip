@@ -36,9 +36,9 @@
 #define ORTHO_C 2.0315f
 #define GRAM_TILE 128
 
-typedef NtShape<2, 2, 128, 128, 2, 2, 2> OrthoGram;
+typedef NtShape<2, 2, 128, 128, 2, 4, 2> OrthoGram;
 typedef NtShape<2, 2, 64, 64, 2, 2, 4> OrthoSquare;
-typedef NtShape<2, 2, 128, 128, 2, 2, 2> OrthoApplySmall;
+typedef NtShape<2, 2, 128, 128, 2, 4, 2> OrthoApplySmall;
 typedef NtShape<2, 2, 256, 256, 2, 4, 2> OrthoApplyLarge;
 
 // What the launches are told about a matrix: by value to the first, a table in the workspace for the others.
@@ -337,11 +337,11 @@ __global__ __launch_bounds__(256) void ortho_split_kernel(OrthoTable tab, OrthoR
 // A R x TILE slab (rows i0 ..., columns j0 ... of an m x m matrix) from LDS to parts of the matrix and, where `mirror`, of
 // its transpose.  Values behind the last column (row) are the zeros that pad the contraction.  The pitch TILE + 5 is odd
 // and 8 pitches are 40 mod 64: neither way of reading meets more than two lanes on a bank.
-template <int R, int TILE>
+template <int R, int TILE, int THREADS>
 __device__ __forceinline__ void ortho_store_sym(const float *slab, int i0, int j0, int m, char *dst, bool mirror) {
     const int t = threadIdx.x, mpad = (m + 31) & ~31;
     const int64_t rb = ortho_row_bytes(m);
-    for (int e = t; e < R * (TILE / 8); e += 256) {
+    for (int e = t; e < R * (TILE / 8); e += THREADS) {
         const int r = e / (TILE / 8), c8 = e % (TILE / 8) * 8, k = j0 + c8;
         if (i0 + r >= m || k >= mpad) continue;
         float v[8];
@@ -350,7 +350,7 @@ __device__ __forceinline__ void ortho_store_sym(const float *slab, int i0, int j
         ortho_store8(ortho_at(dst, rb, i0 + r, k), v);
     }
     if (!mirror) return;
-    for (int e = t; e < TILE * (R / 8); e += 256) {
+    for (int e = t; e < TILE * (R / 8); e += THREADS) {
         const int c = e / (R / 8), r8 = e % (R / 8) * 8, k = i0 + r8;
         if (j0 + c >= m || k >= mpad) continue;
         float v[8];
@@ -376,7 +376,7 @@ __device__ __forceinline__ void ortho_slab_from_acc(float *slab, const f32x16 (&
 }
 
 // ------------------------------------------------------------------------------------------------ A = X X^T
-__global__ __launch_bounds__(256, 2) void ortho_gram_kernel(OrthoTable tab, int step, int ntiles) {
+__global__ __launch_bounds__(OrthoGram::THREADS, 4) void ortho_gram_kernel(OrthoTable tab, int step, int ntiles) {
     typedef OrthoGram S;
     __shared__ __attribute__((aligned(128))) char smem[S::LDS];
     static_assert(64 * (S::TB + 5) * 4 <= S::LDS, "epilogue slab must fit the operand stages");
@@ -400,7 +400,7 @@ __global__ __launch_bounds__(256, 2) void ortho_gram_kernel(OrthoTable tab, int 
             for (int j = 0; j < S::FB; ++j)
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
-                    slab[(64 * (wave >> 1) + 32 * i + nt_acc_row(r, lane)) * GRAM_TILE + 64 * (wave & 1) + 32 * j +
+                    slab[(64 * (wave / S::WC) + 32 * i + nt_acc_row(r, lane)) * GRAM_TILE + 32 * (wave % S::WC) + 32 * j +
                          (lane & 31)] = acc[i][j][r];
         return;
     }
@@ -409,7 +409,7 @@ __global__ __launch_bounds__(256, 2) void ortho_gram_kernel(OrthoTable tab, int 
         __syncthreads();
         ortho_slab_from_acc<S>((float *)smem, acc, h, ORTHO_UNSCALE * ORTHO_UNSCALE);
         __syncthreads();
-        ortho_store_sym<64, GRAM_TILE>((const float *)smem, i0 + 64 * h, j0, m, o.a, i0 != j0);
+        ortho_store_sym<64, GRAM_TILE, S::THREADS>((const float *)smem, i0 + 64 * h, j0, m, o.a, i0 != j0);
     }
 }
 
@@ -438,7 +438,7 @@ __global__ __launch_bounds__(256) void ortho_join_kernel(OrthoTable tab) {
         d[0] = s.x * u; d[1] = s.y * u; d[2] = s.z * u; d[3] = s.w * u;
     }
     __syncthreads();
-    ortho_store_sym<32, GRAM_TILE>(slab, i0, j0, m, ortho_operands(p, tab.ws, 0).a, (w.ij >> 16) != (w.ij & 0xffff));
+    ortho_store_sym<32, GRAM_TILE, 256>(slab, i0, j0, m, ortho_operands(p, tab.ws, 0).a, (w.ij >> 16) != (w.ij & 0xffff));
 }
 
 // ------------------------------------------------------------------------------------------------ P = a I + b A + c A^2
@@ -477,7 +477,7 @@ __global__ __launch_bounds__(256, 2) void ortho_poly_kernel(OrthoTable tab, int 
             }
         }
         __syncthreads();
-        ortho_store_sym<R, TILE>(slab, r0, j0, m, o.p, i0 != j0);
+        ortho_store_sym<R, TILE, 256>(slab, r0, j0, m, o.p, i0 != j0);
     }
 }
 
@@ -608,7 +608,7 @@ __device__ __forceinline__ void ortho_result(const OrthoProb &p, const f32x16 &a
 
 // LAST: the result instead of the next step's X.
 template <typename T, typename S, bool LAST>
-__global__ __launch_bounds__(S::THREADS, S::THREADS == 256 ? 2 : 1) void ortho_apply_kernel(OrthoTable tab, int ntiles,
+__global__ __launch_bounds__(S::THREADS, S::TA == 128 ? 4 : 2) void ortho_apply_kernel(OrthoTable tab, int ntiles,
                                                                                             int step, OrthoRule rule) {
     __shared__ __attribute__((aligned(128))) char smem[S::LDS];
     const OrthoTile w = tab.apply[nt_xcd_runs(blockIdx.x, ntiles)];
@@ -1097,7 +1097,7 @@ static int ortho_run(const D *d, int n, int steps, float eps, const OrthoRule &r
             hipLaunchKernelGGL((ortho_square_kernel<false>), dim3(pl.nsquare), dim3(256), 0, stream, tab, pl.nsquare, s);
             hipLaunchKernelGGL((ortho_square_kernel<true>), dim3(pl.nsquare), dim3(256), 0, stream, tab, pl.nsquare, s);
         } else {
-            hipLaunchKernelGGL(ortho_gram_kernel, dim3(pl.ngram), dim3(256), 0, stream, tab, s, pl.ngram);
+            hipLaunchKernelGGL(ortho_gram_kernel, dim3(pl.ngram), dim3(OrthoGram::THREADS), 0, stream, tab, s, pl.ngram);
             if (pl.joined) hipLaunchKernelGGL(ortho_join_kernel, dim3(4 * pl.nsym), dim3(256), 0, stream, tab);
             hipLaunchKernelGGL(ortho_poly_kernel, dim3(pl.nsquare), dim3(256), 0, stream, tab, pl.nsquare, s);
         }

@@ -90,7 +90,8 @@ def _product_bound(xq, wq, y, scale, bias, dtype):
 @pytest.mark.parametrize("M,N,K,relu,affine", [
     (1, 1, 1, False, False), (1, 1024, 12544, True, True), (13, 324, 1024, False, True), (16, 17, 33, True, False),
     (17, 16, 255, False, True), (128, 128, 256, False, False), (129, 127, 257, True, True), (37, 1024, 1000, False, True),
-    (1000, 81, 3000, True, True), (300, 300, 64, False, False)])
+    (1000, 81, 3000, True, True), (300, 300, 64, False, False),
+    (6201, 2001, 70, True, True), (6145, 1793, 300, False, False)])      # (the large tiles)
 def test_product_matches_the_definition(M, N, K, relu, affine, dtype):
     from sln_amodal_amd import ops
     x, w = _x((M, K), M + K, dtype), _x((N, K), N * 7 + K) / K ** 0.5
@@ -140,7 +141,8 @@ def test_sums_that_float32_holds_are_exact(M, K):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("M,N,K,relu,affine", [
     (1, 1, 1, False, False), (3, 5, 40, True, True), (16, 324, 100, False, True), (65, 63, 257, True, True),
-    (130, 129, 300, False, False), (501, 324, 1000, True, True), (1600, 6, 33, False, True)])
+    (130, 129, 300, False, False), (501, 324, 1000, True, True), (1600, 6, 33, False, True),
+    (301, 701, 12544, False, True), (2000, 33, 6400, True, False)])       # (the large tiles)
 def test_gradients_match_the_straight_through_formula(M, N, K, relu, affine, dtype):
     from sln_amodal_amd import ops
     x, w = _x((M, K), M + K, dtype), _x((N, K), N * 7 + K) / K ** 0.5
