@@ -49,7 +49,7 @@ struct OrthoProb {
     int64_t gs, os, off;   // off: byte offset of this matrix's operands in the workspace
     int32_t rows, cols;
     int32_t part0, nparts; // its partial sums of squares
-    int32_t split0, sym0, gram0, square0, apply0, nsplit;    // first entries in the work lists, cuts of the contraction
+    int32_t split0, sym0, gram0, square0, apply0, last0, nsplit;    // first entries in the work lists, cuts of the contraction
     float lr, decay;       // update: p = p * decay - lr * X
     int32_t shift;         // h of the first step (ortho_split_kernel)
 };
@@ -58,7 +58,7 @@ struct OrthoTile { int32_t prob, ij, first, cut; };        // ij = row tile << 1
 
 struct OrthoTable {
     OrthoProb *prob;
-    OrthoTile *split, *sym, *gram, *square, *apply;
+    OrthoTile *split, *sym, *gram, *square, *apply, *last;
     double *part;
     char *ws;
     float *slab;           // partial Gram tiles, GRAM_TILE^2 floats per gram entry
@@ -173,6 +173,11 @@ __device__ __forceinline__ void ortho_lists(const OrthoProb &p, int prob, const 
     for (int e = t; e < ti * tj; e += 256) {       // the m tiles of one column of X run side by side
         const OrthoTile w = {prob, (e % ti) << 16 | (e / ti), 0, 0};
         tab.apply[p.apply0 + e] = w;
+    }
+    const int li = ortho_tiles(m, OrthoApplySmall::TB), lj = ortho_tiles(n, OrthoApplySmall::TA);
+    for (int e = t; e < li * lj; e += 256) {
+        const OrthoTile w = {prob, (e % li) << 16 | (e / li), 0, 0};
+        tab.last[p.last0 + e] = w;
     }
 }
 
@@ -608,10 +613,11 @@ __device__ __forceinline__ void ortho_result(const OrthoProb &p, const f32x16 &a
 
 // LAST: the result instead of the next step's X.
 template <typename T, typename S, bool LAST>
-__global__ __launch_bounds__(S::THREADS, S::TA == 128 ? 4 : 2) void ortho_apply_kernel(OrthoTable tab, int ntiles,
-                                                                                            int step, OrthoRule rule) {
+__global__ __launch_bounds__(S::THREADS, S::TA == 128 ? 4 : 2) void ortho_apply_kernel(OrthoTable tab,
+                                                                                         const OrthoTile *list, int ntiles,
+                                                                                         int step, OrthoRule rule) {
     __shared__ __attribute__((aligned(128))) char smem[S::LDS];
-    const OrthoTile w = tab.apply[nt_xcd_runs(blockIdx.x, ntiles)];
+    const OrthoTile w = list[nt_xcd_runs(blockIdx.x, ntiles)];
     const OrthoProb p = tab.prob[w.prob];
     const OrthoOperands o = ortho_operands(p, tab.ws, step);
     const int m = ortho_m(p), n = ortho_n(p);
@@ -913,8 +919,8 @@ __global__ __launch_bounds__(512) void ortho_small_kernel(OrthoBatch batch, Orth
 // ------------------------------------------------------------------------------------------------ host side
 // Everything about a call that follows from its shapes.
 struct OrthoPlan {
-    int64_t prob, split, sym, gram, square, apply, part, slab, operands, bytes;
-    int nsplit, nsym, ngram, nsquare, napply, nparts, cut, apply_tile, empty;
+    int64_t prob, split, sym, gram, square, apply, last, part, slab, operands, bytes;
+    int nsplit, nsym, ngram, nsquare, napply, nlast, nparts, cut, apply_tile, empty;
     bool joined, small, squares;     // squares: short Gram products, not cut
 };
 
@@ -971,9 +977,11 @@ static int ortho_plan(const D *d, int n, OrthoPlan &pl) {
     pl.cut = (int)ortho_gram_cut(d, n);
     // Tiles: large ones where they fill the chip, else smaller ones.  Few and short Gram products (up to one tile of 64 x 64
     // per CU, up to 80 k-steps) go without cuts, partial tiles and the launch that joins them.
-    pl.apply_tile = apply256 >= 192 ? 256 : 128;
+    // (the large ones where the rounds of 256 they make are three quarters full: alone on its CU a workgroup's stores are
+    // not covered by another's loads; the optimiser's last step, which also reads the weights, takes the small ones)
+    pl.apply_tile = 4 * apply256 >= 3 * ((apply256 + 255) / 256 * 256) ? 256 : 128;
     pl.squares = square64 <= 256 && longest <= 80;
-    int64_t nsplit = 0, nsym = 0, ngram = 0, nsquare = 0, napply = 0, nparts = 0, operands = 0;
+    int64_t nsplit = 0, nsym = 0, ngram = 0, nsquare = 0, napply = 0, nlast = 0, nparts = 0, operands = 0;
     for (int i = 0; i < n; ++i) {
         if (d[i].rows == 0 || d[i].cols == 0) continue;
         OrthoProb p = {};
@@ -989,10 +997,11 @@ static int ortho_plan(const D *d, int n, OrthoPlan &pl) {
         }
         nsquare += pl.squares ? tp * tp : tp * (tp + 1) / 2;
         napply += ((m + pl.apply_tile - 1) / pl.apply_tile) * ((k + pl.apply_tile - 1) / pl.apply_tile);
+        nlast += ((m + 127) / 128) * ((k + 127) / 128);
         nparts += ((int64_t)p.rows * p.cols + ORTHO_CHUNK - 1) / ORTHO_CHUNK;
         operands += ortho_align(ortho_operand_bytes(p));
         const int64_t most = 1 << 28;
-        if (nsplit > most || ngram > most || nsquare > most || napply > most || nparts > most) return SLN_ERR_UNSUPPORTED;
+        if (nsplit > most || ngram > most || nsquare > most || nlast > most || nparts > most) return SLN_ERR_UNSUPPORTED;
     }
     int64_t at = 0;
     pl.prob = at; at += ortho_align(live * (int64_t)sizeof(OrthoProb));
@@ -1001,11 +1010,13 @@ static int ortho_plan(const D *d, int n, OrthoPlan &pl) {
     pl.gram = at; at += ortho_align(ngram * (int64_t)sizeof(OrthoTile));
     pl.square = at; at += ortho_align(nsquare * (int64_t)sizeof(OrthoTile));
     pl.apply = at; at += ortho_align(napply * (int64_t)sizeof(OrthoTile));
+    pl.last = at; at += ortho_align(nlast * (int64_t)sizeof(OrthoTile));
     pl.part = at; at += ortho_align(nparts * (int64_t)sizeof(double));
     pl.slab = at; at += pl.joined ? ortho_align(ngram * (int64_t)(GRAM_TILE * GRAM_TILE * 4)) : 0;
     pl.operands = at; at += operands;
     pl.bytes = at;
     pl.nsplit = (int)nsplit; pl.nsym = (int)nsym; pl.ngram = (int)ngram; pl.nsquare = (int)nsquare; pl.napply = (int)napply;
+    pl.nlast = (int)nlast;
     pl.nparts = (int)nparts;
     return SLN_OK;
 }
@@ -1041,12 +1052,12 @@ static void ortho_run_small(const D *d, int n, int steps, float eps, const Ortho
 }
 
 template <typename T, typename S>
-static void ortho_apply(const OrthoTable &tab, int napply, int step, bool last, const OrthoRule &rule, hipStream_t stream) {
+static void ortho_apply(const OrthoTable &tab, const OrthoTile *list, int n, int step, bool last, const OrthoRule &rule,
+                        hipStream_t stream) {
     if (last)
-        hipLaunchKernelGGL((ortho_apply_kernel<T, S, true>), dim3(napply), dim3(S::THREADS), 0, stream, tab, napply, step, rule);
+        hipLaunchKernelGGL((ortho_apply_kernel<T, S, true>), dim3(n), dim3(S::THREADS), 0, stream, tab, list, n, step, rule);
     else
-        hipLaunchKernelGGL((ortho_apply_kernel<T, S, false>), dim3(napply), dim3(S::THREADS), 0, stream, tab, napply, step,
-                           rule);
+        hipLaunchKernelGGL((ortho_apply_kernel<T, S, false>), dim3(n), dim3(S::THREADS), 0, stream, tab, list, n, step, rule);
 }
 
 template <typename T, typename D>
@@ -1067,9 +1078,9 @@ static int ortho_run(const D *d, int n, int steps, float eps, const OrthoRule &r
     char *ws = (char *)workspace;
     const OrthoTable tab = {(OrthoProb *)(ws + pl.prob), (OrthoTile *)(ws + pl.split), (OrthoTile *)(ws + pl.sym),
                             (OrthoTile *)(ws + pl.gram), (OrthoTile *)(ws + pl.square), (OrthoTile *)(ws + pl.apply),
-                            (double *)(ws + pl.part), ws, (float *)(ws + pl.slab), pl.apply_tile};
+                            (OrthoTile *)(ws + pl.last), (double *)(ws + pl.part), ws, (float *)(ws + pl.slab), pl.apply_tile};
     OrthoBatch batch;
-    int prob0 = 0, inb = 0, parts = 1, part0 = 0, split0 = 0, sym0 = 0, gram0 = 0, square0 = 0, apply0 = 0;
+    int prob0 = 0, inb = 0, parts = 1, part0 = 0, split0 = 0, sym0 = 0, gram0 = 0, square0 = 0, apply0 = 0, last0 = 0;
     int64_t off = pl.operands;
     for (int i = 0; i <= n; ++i) {
         if (inb == ORTHO_BATCH || (inb > 0 && i == n)) {
@@ -1089,6 +1100,7 @@ static int ortho_run(const D *d, int n, int steps, float eps, const OrthoRule &r
         p.gram0 = gram0; gram0 += tm * (tm + 1) / 2 * p.nsplit;
         p.square0 = square0; square0 += pl.squares ? tp * tp : tp * (tp + 1) / 2;
         p.apply0 = apply0; apply0 += ortho_tiles(m, pl.apply_tile) * ortho_tiles(k, pl.apply_tile);
+        p.last0 = last0; last0 += ortho_tiles(m, 128) * ortho_tiles(k, 128);
         if (p.nparts > parts) parts = p.nparts;
     }
     hipLaunchKernelGGL((ortho_split_kernel<T>), dim3(pl.nsplit), dim3(256), 0, stream, tab, rule, eps);
@@ -1101,8 +1113,10 @@ static int ortho_run(const D *d, int n, int steps, float eps, const OrthoRule &r
             if (pl.joined) hipLaunchKernelGGL(ortho_join_kernel, dim3(4 * pl.nsym), dim3(256), 0, stream, tab);
             hipLaunchKernelGGL(ortho_poly_kernel, dim3(pl.nsquare), dim3(256), 0, stream, tab, pl.nsquare, s);
         }
-        if (pl.apply_tile == 256) ortho_apply<T, OrthoApplyLarge>(tab, pl.napply, s, s + 1 == steps, rule, stream);
-        else ortho_apply<T, OrthoApplySmall>(tab, pl.napply, s, s + 1 == steps, rule, stream);
+        const bool last = s + 1 == steps, weights = last && rule.sqnorm;
+        if (pl.apply_tile == 256 && !weights) ortho_apply<T, OrthoApplyLarge>(tab, tab.apply, pl.napply, s, last, rule, stream);
+        else if (weights) ortho_apply<T, OrthoApplySmall>(tab, tab.last, pl.nlast, s, last, rule, stream);
+        else ortho_apply<T, OrthoApplySmall>(tab, tab.apply, pl.napply, s, last, rule, stream);
     }
     return sln_launch_status();
 }
