@@ -921,8 +921,17 @@ __global__ __launch_bounds__(512) void ortho_small_kernel(OrthoBatch batch, Orth
 struct OrthoPlan {
     int64_t prob, split, sym, gram, square, apply, last, part, slab, operands, bytes;
     int nsplit, nsym, ngram, nsquare, napply, nlast, nparts, cut, apply_tile, empty;
+    int64_t gram_at[17];             // first entry of each class of Gram items, the long ones first
     bool joined, small, squares;     // squares: short Gram products, not cut
 };
+
+// Cuts of a matrix with k columns and their class (0: the longest sixteenth): the launch ends together if it begins with
+// the long ones (125 matrices of a detector, c = 79: 147 us instead of 179 in the order of their rows).
+static inline int64_t ortho_cuts(const OrthoPlan &pl, int64_t k) { return pl.squares ? 0 : ((k + 31) / 32 + pl.cut - 1) / pl.cut; }
+static inline int ortho_gram_class(const OrthoPlan &pl, int64_t k) {
+    const int64_t g = (k + 31) / 32, cuts = (g + pl.cut - 1) / pl.cut;
+    return 15 - (int)(((g + cuts - 1) / cuts - 1) * 16 / pl.cut);
+}
 
 static inline int64_t ortho_align(int64_t v) { return (v + 255) & ~(int64_t)255; }
 
@@ -932,25 +941,36 @@ static void ortho_sides(const D &d, int64_t &m, int64_t &n) {
     n = d.rows < d.cols ? d.cols : d.rows;
 }
 
-// Cuts of the Gram contraction.  With W k-steps in all and two workgroups per CU the launch takes about
-// (W + 8 items) / 512 + cut / 2 k-steps: an item costs about eight more (its epilogue, or its partial tile and the join),
-// and the last ones end half a cut apart.  The power of two times 8 or 12 that makes this least.
+// Cuts of the Gram contraction: the longest run of k-steps that one item gets.  A workgroup alone on its CU takes 0.65 us
+// a k-step, one of two 1.13; an item costs about six steps more than it has, and a partial tile a sixteenth of a step to
+// store and to join (all launches together).  In quarters of a step: items that each have a CU end after 4 (c + 6), two on
+// a CU after 7 (c + 6); W k-steps in more items take about 7 (W + 6 items) / 512, the last ones ending half a cut apart.
+// The c, in steps of an eighth, that makes this least.  Measured per step of the iteration, relative to a shorter cut: 23
+// matrices of 256 x 2304, c = 24 (207 items) 9 us less than 12, 36 6 more, 72 24 more; 21 of 2 x 256 to 1024 x 12544, c =
+// 40 (493 items) 11 us less than 24, 72 15 more; 125 of a whole detector, c = 100 (636) 16 us less than 32, 200 29 more.
 template <typename D>
 static int64_t ortho_gram_cut(const D *d, int n) {
-    int64_t best = 8, least = INT64_MAX;
-    for (int64_t c = 8; c <= (1 << 18); c += (c & (c - 1)) ? c / 3 : c / 2) {
-        int64_t steps = 0, items = 0, longest = 0;
+    int64_t best = 8, least = INT64_MAX, steps = 0, longest = 0;
+    for (int i = 0; i < n; ++i) {
+        int64_t m, k;
+        ortho_sides(d[i], m, k);
+        const int64_t t = (m + GRAM_TILE - 1) / GRAM_TILE, g = (k + 31) / 32;
+        steps += t * (t + 1) / 2 * g;
+        if (g > longest) longest = g;
+    }
+    for (int64_t c = steps / 1024 > 8 ? steps / 1024 : 8;; c += c / 8 + 1) {
+        int64_t items = 0;
         for (int i = 0; i < n; ++i) {
             int64_t m, k;
             ortho_sides(d[i], m, k);
-            const int64_t t = (m + GRAM_TILE - 1) / GRAM_TILE, tiles = t * (t + 1) / 2, g = (k + 31) / 32;
-            steps += tiles * g;
-            items += tiles * ((g + c - 1) / c);
-            if (g > longest) longest = g;
+            const int64_t t = (m + GRAM_TILE - 1) / GRAM_TILE;
+            items += t * (t + 1) / 2 * (((k + 31) / 32 + c - 1) / c);
         }
-        const int64_t cost = (steps + 8 * items) + 256 * (c < longest ? c : longest);
+        const int64_t most = c < longest ? c : longest;
+        const int64_t cost = items / 4 + (items <= 256 ? 4 * (most + 6) : items <= 512 ? 7 * (most + 6)
+                                                                                       : 7 * (steps + 6 * items) / 512 + 2 * most);
         if (cost < least) { least = cost; best = c; }
-        if (c >= longest) break;
+        if (items <= 256 || c >= longest) break;
     }
     return best;
 }
@@ -987,13 +1007,14 @@ static int ortho_plan(const D *d, int n, OrthoPlan &pl) {
         OrthoProb p = {};
         p.rows = d[i].rows; p.cols = d[i].cols;
         const int64_t m = ortho_m(p), k = ortho_n(p);
-        const int64_t tm = (m + GRAM_TILE - 1) / GRAM_TILE, cuts = ((k + 31) / 32 + pl.cut - 1) / pl.cut;
+        const int64_t tm = (m + GRAM_TILE - 1) / GRAM_TILE, cuts = ortho_cuts(pl, k);
         const int64_t tp = (m + OrthoSquare::TA - 1) / OrthoSquare::TA;
-        pl.joined |= cuts > 1 && !pl.squares;
+        pl.joined |= cuts > 1;
         nsplit += ((m + 63) / 64) * ((k + 127) / 128);
         if (!pl.squares) {
             nsym += tm * (tm + 1) / 2;
             ngram += tm * (tm + 1) / 2 * cuts;
+            pl.gram_at[ortho_gram_class(pl, k) + 1] += tm * (tm + 1) / 2 * cuts;
         }
         nsquare += pl.squares ? tp * tp : tp * (tp + 1) / 2;
         napply += ((m + pl.apply_tile - 1) / pl.apply_tile) * ((k + pl.apply_tile - 1) / pl.apply_tile);
@@ -1003,6 +1024,7 @@ static int ortho_plan(const D *d, int n, OrthoPlan &pl) {
         const int64_t most = 1 << 28;
         if (nsplit > most || ngram > most || nsquare > most || nlast > most || nparts > most) return SLN_ERR_UNSUPPORTED;
     }
+    for (int i = 1; i < 17; ++i) pl.gram_at[i] += pl.gram_at[i - 1];
     int64_t at = 0;
     pl.prob = at; at += ortho_align(live * (int64_t)sizeof(OrthoProb));
     pl.split = at; at += ortho_align(nsplit * (int64_t)sizeof(OrthoTile));
@@ -1080,7 +1102,7 @@ static int ortho_run(const D *d, int n, int steps, float eps, const OrthoRule &r
                             (OrthoTile *)(ws + pl.gram), (OrthoTile *)(ws + pl.square), (OrthoTile *)(ws + pl.apply),
                             (OrthoTile *)(ws + pl.last), (double *)(ws + pl.part), ws, (float *)(ws + pl.slab), pl.apply_tile};
     OrthoBatch batch;
-    int prob0 = 0, inb = 0, parts = 1, part0 = 0, split0 = 0, sym0 = 0, gram0 = 0, square0 = 0, apply0 = 0, last0 = 0;
+    int prob0 = 0, inb = 0, parts = 1, part0 = 0, split0 = 0, sym0 = 0, square0 = 0, apply0 = 0, last0 = 0;
     int64_t off = pl.operands;
     for (int i = 0; i <= n; ++i) {
         if (inb == ORTHO_BATCH || (inb > 0 && i == n)) {
@@ -1093,11 +1115,14 @@ static int ortho_run(const D *d, int n, int steps, float eps, const OrthoRule &r
         const int m = ortho_m(p), k = ortho_n(p);
         const int tm = ortho_tiles(m, GRAM_TILE), tp = ortho_tiles(m, OrthoSquare::TA);
         p.off = off; off += ortho_align(ortho_operand_bytes(p));
-        p.nsplit = pl.squares ? 0 : ((k + 31) / 32 + pl.cut - 1) / pl.cut;
+        p.nsplit = (int)ortho_cuts(pl, k);
         p.part0 = part0; p.nparts = sln_div_up((long)p.rows * p.cols, ORTHO_CHUNK); part0 += p.nparts;
         p.split0 = split0; split0 += ortho_tiles(m, 64) * ortho_tiles(k, 128);
         p.sym0 = sym0; sym0 += pl.squares ? 0 : tm * (tm + 1) / 2;
-        p.gram0 = gram0; gram0 += tm * (tm + 1) / 2 * p.nsplit;
+        if (!pl.squares) {
+            int64_t &g0 = pl.gram_at[ortho_gram_class(pl, k)];
+            p.gram0 = (int)g0; g0 += tm * (tm + 1) / 2 * p.nsplit;
+        }
         p.square0 = square0; square0 += pl.squares ? tp * tp : tp * (tp + 1) / 2;
         p.apply0 = apply0; apply0 += ortho_tiles(m, pl.apply_tile) * ortho_tiles(k, pl.apply_tile);
         p.last0 = last0; last0 += ortho_tiles(m, 128) * ortho_tiles(k, 128);
