@@ -37,7 +37,8 @@
 #define GRAM_TILE 128
 
 typedef NtShape<2, 2, 128, 128, 2, 4, 2> OrthoGram;
-typedef NtShape<2, 2, 64, 64, 2, 2, 4> OrthoSquare;
+typedef NtShape<2, 2, 64, 64, 2, 2, 4> OrthoSquare;                // few workgroups: depth
+typedef NtShape<2, 2, 64, 64, 2, 2, 3> OrthoPoly;                  // three on a CU (a detector's 125: 46 us; four stages 52)
 typedef NtShape<2, 2, 128, 128, 2, 4, 2> OrthoApplySmall;
 typedef NtShape<2, 2, 256, 256, 2, 4, 2> OrthoApplyLarge;
 
@@ -447,8 +448,8 @@ __global__ __launch_bounds__(256) void ortho_join_kernel(OrthoTable tab) {
 }
 
 // ------------------------------------------------------------------------------------------------ P = a I + b A + c A^2
-__global__ __launch_bounds__(256, 2) void ortho_poly_kernel(OrthoTable tab, int ntiles, int step) {
-    typedef OrthoSquare S;
+__global__ __launch_bounds__(256, 3) void ortho_poly_kernel(OrthoTable tab, int ntiles, int step) {
+    typedef OrthoPoly S;
     constexpr int TILE = S::TA, R = TILE / 2;
     __shared__ __attribute__((aligned(128))) char smem[S::LDS];
     static_assert(R * (TILE + 5) * 4 <= S::LDS, "epilogue slab must fit the operand stages");
@@ -490,7 +491,7 @@ __global__ __launch_bounds__(256, 2) void ortho_poly_kernel(OrthoTable tab, int 
 // A = X X^T and P (POLY) of calls with little to do: every tile of the square, both triangles.  A lane's eight neighbours
 // down a column are eight neighbours along the row of the transpose, and the product is symmetric: parts go from registers
 // to that row.  Twice the products of the triangle, but no cuts, no turn through LDS and no second store (where there is
-// enough work the triangles win: P of the heads' 21 matrices 23 us against 31, of all 124 52 against 69).
+// enough work the triangles win: P of the heads' 21 matrices 24 us against 31, of all 125 46 against 69).
 template <bool POLY>
 __global__ __launch_bounds__(256, 2) void ortho_square_kernel(OrthoTable tab, int ntiles, int step) {
     typedef OrthoSquare S;
