@@ -94,16 +94,20 @@ __global__ __launch_bounds__(256) void mx4_values_kernel(const unsigned *__restr
 // which the eight blocks of a step enter the sum is free, so the two halves of a wave take blocks 0 ... 3 and 4 ... 7: a
 // lane's four scales are one aligned dword of the scale row, and the instruction picks its byte.  The scales come by DMA
 // too: with ordinary loads among the DMA's the compiler waits for all of them before the first LDS read of a step, and
-// nothing overlaps (16000 x 12544 x 1024: 155 us instead of MXNEW).
+// nothing overlaps (16000 x 12544 x 1024: 155 us instead of 130).
 template <int TA_, int TB_, int WR_, int WC_>
 struct MxShape {
     static constexpr int TA = TA_, TB = TB_, WR = WR_, WC = WC_, NW = WR * WC, THREADS = NW * 64;
     static constexpr int FA = TA / WR / 32, FB = TB / WC / 32, QA = TA / 8 / NW, QB = TB / 8 / NW;
     static constexpr int SCALES = (TA + TB) * 128, STAGE = SCALES + (TA + TB) * 8, LDS = 2 * STAGE;
-    static_assert(TA == 32 * NW && TB == 32 * NW, "a wave fetches the scales of 32 rows of either side");
+    static constexpr int OCC = 163840 / LDS * NW / 4;                             // waves per SIMD
+    static constexpr int RA = TA / NW, RB = TB / NW;                              // rows whose scales a wave fetches
+    static_assert(RA <= 32 && RB <= 32, "64 lanes fetch two dwords of at most 32 rows");
 };
-typedef MxShape<128, 128, 2, 2> MxSmall;           // two workgroups per CU
-typedef MxShape<256, 256, 2, 4> MxLarge;           // one
+// Small: two workgroups per CU (1000 x 12544 x 1024: 20 us, with four waves each 24).  Large: one (16000 rows: 130 us; with
+// 16 waves 128, small tiles 155; 256 x 128 with a third stage 168: the reads out of L2, not their latency, are the bound).
+typedef MxShape<128, 128, 2, 4> MxSmall;
+typedef MxShape<256, 256, 2, 4> MxLarge;
 struct MxGemm {
     const uint8_t *a, *b, *sa, *sb;
     int64_t a_pitch, b_pitch;          // bytes per code row
@@ -133,7 +137,7 @@ __device__ __forceinline__ i32x8 mx_frag(const char *at) {
 }
 
 template <typename T, typename S>
-__global__ __launch_bounds__(S::THREADS, S::THREADS == 256 ? 2 : 1) void mx4_product_kernel(const MxGemm p, int tiles) {
+__global__ __launch_bounds__(S::THREADS, S::OCC) void mx4_product_kernel(const MxGemm p, int tiles) {
 #ifdef __HIP_DEVICE_COMPILE__                      // (the host pass knows no buffer descriptors in templates)
     constexpr int NW = S::NW, OPA = S::TA * 128;
     __shared__ __attribute__((aligned(128))) char smem[S::LDS];
@@ -156,10 +160,9 @@ __global__ __launch_bounds__(S::THREADS, S::THREADS == 256 ? 2 : 1) void mx4_pro
         boff[q] = (unsigned)(min(row, p.N - 1 - n0) * p.b_pitch + c * 16);
     }
     const uint8_t *ga = p.a + (int64_t)m0 * p.a_pitch, *gb = p.b + (int64_t)n0 * p.b_pitch;
-    // scales: lane l of wave w fetches dword l & 1 of rows 32 w + l / 2
-    const int srow = 32 * wave + (lane >> 1);
-    const unsigned qa = (unsigned)min(m0 + srow, p.M - 1) * 8u + (lane & 1) * 4u;
-    const unsigned qb = (unsigned)min(n0 + srow, p.N - 1) * 8u + (lane & 1) * 4u;
+    // scales: lane l of wave w fetches dword l & 1 of rows RA w + l / 2 and RB w + l / 2
+    const unsigned qa = (unsigned)min(m0 + S::RA * wave + (lane >> 1), p.M - 1) * 8u + (lane & 1) * 4u;
+    const unsigned qb = (unsigned)min(n0 + S::RB * wave + (lane >> 1), p.N - 1) * 8u + (lane & 1) * 4u;
     const __amdgpu_buffer_rsrc_t ra = nt_buffer(ga, INT64_MAX), rb = nt_buffer(gb, INT64_MAX);
     auto issue = [&](int s, int stage) {
         char *l = smem + stage * S::STAGE + wave * 1024;
@@ -171,11 +174,13 @@ __global__ __launch_bounds__(S::THREADS, S::THREADS == 256 ? 2 : 1) void mx4_pro
         for (int q = 0; q < S::QB; ++q)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (nt_lds *)(l + OPA + q * (NW * 1024)), 16, boff[q],
                                                      (unsigned)s * 128u, 0, 0);
-        char *ls = smem + stage * S::STAGE + S::SCALES + wave * 256;
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(nt_buffer(p.sa + (int64_t)s * p.M * 8, INT64_MAX), (nt_lds *)ls, 4, qa, 0, 0,
-                                                 0);
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(nt_buffer(p.sb + (int64_t)s * p.N * 8, INT64_MAX),
-                                                 (nt_lds *)(ls + S::TA * 8), 4, qb, 0, 0, 0);
+        char *ls = smem + stage * S::STAGE + S::SCALES;
+        if (S::RA == 32 || lane < 2 * S::RA)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(nt_buffer(p.sa + (int64_t)s * p.M * 8, INT64_MAX),
+                                                     (nt_lds *)(ls + wave * (S::RA * 8)), 4, qa, 0, 0, 0);
+        if (S::RB == 32 || lane < 2 * S::RB)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(nt_buffer(p.sb + (int64_t)s * p.N * 8, INT64_MAX),
+                                                     (nt_lds *)(ls + S::TA * 8 + wave * (S::RB * 8)), 4, qb, 0, 0, 0);
     };
     f32x16 acc[S::FA][S::FB];
 #pragma unroll
@@ -396,10 +401,10 @@ static inline int mx_rows_cuts(int64_t N, int64_t K) {
     return mx_cuts((N + 15) / 16, 512, 2 * ((K + MX_STEP - 1) / MX_STEP), 8);
 }
 static inline int64_t mx_tiles(int64_t M, int64_t N, int tile) { return ((M + tile - 1) / tile) * ((N + tile - 1) / tile); }
-// Large tiles where three quarters of the CUs get one (16000 x 12544 x 1024: 255 us with 128 x 128).
+// Large tiles where three quarters of the CUs get one (16000 x 12544 x 1024: 155 us with 128 x 128, 130 so).
 static inline bool mx_large(int64_t M, int64_t N) { return mx_tiles(M, N, 256) >= 192; }
 static inline int mx_product_cuts(int64_t M, int64_t N, int64_t K) {
-    return mx_large(M, N) ? 1 : mx_cuts(mx_tiles(M, N, 128), 512, (K + MX_STEP - 1) / MX_STEP, 2);
+    return mx_large(M, N) ? 1 : mx_cuts(mx_tiles(M, N, 128), 256, (K + MX_STEP - 1) / MX_STEP, 2);
 }
 
 extern "C" size_t sln_mx4_product_workspace_bytes(int64_t M, int64_t N, int64_t K, int rounded) {
