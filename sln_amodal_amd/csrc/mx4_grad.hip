@@ -198,8 +198,8 @@ __device__ __forceinline__ void mg_product(const MgProduct &p, int at, char *sme
     }
 }
 
-// Both products (if their tiles are alike) and the bias sums in one launch (x: gx, w: gw; tiles = 0: not here); the tiles with the longer
-// contraction first.
+// Both products (if their tiles are alike) and the bias sums in one launch (x: gx, w: gw; tiles = 0: not here); the tiles
+// with the longer contraction first.
 template <typename T, typename S>
 __global__ __launch_bounds__(S::THREADS, S::THREADS == 256 ? 2 : 4) void mx4_grad_product_kernel(
     const MgProduct x, const MgProduct w, const float *__restrict__ bias_part, int bias_blocks, int N,
@@ -351,6 +351,7 @@ extern "C" int sln_mx4_linear_bwd(const void *gy, int dtype, int64_t gy_stride, 
         (K + 63) / 64 * ((M + 63) / 64) > (1 << 28) || (K + 63) / 64 * ((N + 63) / 64) > (1 << 28))
         return SLN_ERR_UNSUPPORTED;
     if ((gx && (!w_codes || !w_scales)) || (gw && (!x_codes || !x_scales))) return SLN_ERR_INVALID_ARG;
+    if ((gx && ((uintptr_t)w_codes & 15)) || (gw && ((uintptr_t)x_codes & 15))) return SLN_ERR_INVALID_ARG;
     MgPlan pl;
     mg_plan(M, N, K, mg_parts(dtype), gx, gw, gb, pl);
     if (pl.bytes && (!workspace || ((uintptr_t)workspace & 255))) return SLN_ERR_INVALID_ARG;

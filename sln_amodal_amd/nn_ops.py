@@ -70,6 +70,15 @@ def bn_affine(bn):
     return scale, shift
 
 
+class _Mx4Codes(tuple):
+    """(what a weight's codes were made from, the codes).  Copies and pickles of the parameter start without them: version,
+    address and stream mean nothing elsewhere."""
+    __slots__ = ()
+
+    def __reduce__(self):
+        return _Mx4Codes, ()
+
+
 def _mx4_rows(x, weight, w2, bias, scale, relu):
     """act((x w2^T) * scale + bias) on microscaled 4-bit operands; w2() makes the [N, K] rows of `weight`.  In evaluation
     the weight's codes are kept on the parameter until its version counter moves (edits through `.data` do not move it:
@@ -86,9 +95,9 @@ def _mx4_rows(x, weight, w2, bias, scale, relu):
         return mx4.mx4_linear(x, codes, bias, scale=scale, relu=relu)
     key = (weight._version, weight.data_ptr(), torch.cuda.current_stream(x.device).cuda_stream)
     hit = getattr(weight, "_sln_mx4_codes", None)
-    if hit is None or hit[0] != key:
+    if not hit or hit[0] != key:
         with torch.no_grad():
-            hit = weight._sln_mx4_codes = (key, mx4.mx4_quantize(w2()))
+            hit = weight._sln_mx4_codes = _Mx4Codes((key, mx4.mx4_quantize(w2())))
     return mx4.mx4_linear(x, hit[1], bias, scale=scale, relu=relu)
 
 
@@ -96,7 +105,7 @@ def _mx4_conv(x, conv, bn, relu):
     """A tagged convolution that is one product of rows: a window as large as its input, or 1x1 with stride 1."""
     kh, kw = conv.kernel_size
     N, Cc, H, W = x.shape
-    whole = (kh, kw) == (H, W)
+    whole = (kh, kw) == (H, W) and (tuple(conv.dilation) == (1, 1) or (kh, kw) == (1, 1))
     if conv.groups != 1 or not (whole or ((kh, kw) == (1, 1) and tuple(conv.stride) == (1, 1))) or \
             tuple(conv.padding) != (0, 0):
         raise RuntimeError("conv %s -> %s k%s on a %dx%d map is no product of rows: no 4-bit form" %

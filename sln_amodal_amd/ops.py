@@ -443,4 +443,4 @@ def orthogonalize(x, steps=5, eps=1e-7):
         with _lib.on_device(dev):
             _lib.check(L.sln_orthogonalize(descs, len(flat), _FLOATS[dtype], steps, eps, ws.data_ptr() if nbytes else 0,
                                            nbytes, _lib.stream_of(dev)), "sln_orthogonalize")
-    return type(x)(outs) if many else outs[0]
+    return (tuple(outs) if isinstance(x, tuple) else outs) if many else outs[0]

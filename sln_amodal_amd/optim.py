@@ -178,6 +178,8 @@ class ClippedSGD(object):
             b = self.state.get(p)
             if b is None:
                 b = self.state[p] = torch.zeros_like(p, memory_format=torch.preserve_format)
+            elif b.stride() != p.stride():     # (and of the momentum: the weight may have changed its memory format)
+                b = self.state[p] = torch.empty_like(p).copy_(b)
             ps.append(p); gs.append(g); bs.append(b)
         return ps, gs, bs
 
@@ -253,9 +255,11 @@ class ClippedMuon(ClippedSGD):
                 if id(p) in seen:
                     raise ValueError("a parameter appears twice in the parameter groups")
                 seen.add(id(p))
-                if g["orthogonal"] and (p.dim() < 2 or min(p.shape[0], p[0].numel() if p.shape[0] else 0) > 65535):
-                    raise ValueError("an orthogonal group takes matrices (two or more axes, the shorter side at most "
-                                     "65535), got %s" % (tuple(p.shape),))
+                rows = p.shape[0] if p.dim() else 0
+                cols = p.numel() // rows if rows else 0
+                if g["orthogonal"] and (p.dim() < 2 or min(rows, cols) > 65535 or max(rows, cols) > 1 << 22):
+                    raise ValueError("an orthogonal group takes matrices (two or more axes, at most 65535 x 2^22), got %s" %
+                                     (tuple(p.shape),))
 
     def _split(self):
         rest = [g for g in self.param_groups if not g["orthogonal"]]
@@ -316,6 +320,17 @@ class ClippedMuon(ClippedSGD):
                 self.skipped = torch.zeros(1, dtype=torch.int32, device=dev)
             st = _lib.stream_of(dev)
             L = _lib.lib()
+            # (the workspace before the first launch: nothing is written if there is no memory for it)
+            flat = []
+            for i, (p, (glr, decay)) in enumerate(mats, len(rest)):
+                rows = p.shape[0]
+                cols = sizes[i] // rows if rows else 0
+                flat.append((host[0][i], host[1][i], host[2][i], rows, cols,
+                             glr * max(1.0, rows / cols) ** 0.5 if cols else 0.0, decay))
+            flat.sort(key=lambda d: -min(d[3], d[4]))            # (the longest products first: the launches end together)
+            descs = (_MuonDesc * len(flat))(*flat)
+            nbytes = L.sln_muon_step_workspace_bytes(descs, len(flat))
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
             nch = ct.numel() if sum(sizes) else 0
             num, ctp, cop = numel.data_ptr(), ct.data_ptr(), co.data_ptr()
             _lib.check(L.sln_grad_sqnorm_f32(at + row, num, ctp, cop, nch, CHUNK, partial.data_ptr(), sq.data_ptr(), st),
@@ -331,16 +346,6 @@ class ClippedMuon(ClippedSGD):
             else:
                 self.skipped += (~torch.isfinite(guard)).to(torch.int32)
             if mats:
-                flat = []
-                for i, (p, (glr, decay)) in enumerate(mats, len(rest)):
-                    rows = p.shape[0]
-                    cols = sizes[i] // rows if rows else 0
-                    flat.append((host[0][i], host[1][i], host[2][i], rows, cols,
-                                 glr * max(1.0, rows / cols) ** 0.5 if cols else 0.0, decay))
-                flat.sort(key=lambda d: -min(d[3], d[4]))        # (the longest products first: the launches end together)
-                descs = (_MuonDesc * len(flat))(*flat)
-                nbytes = L.sln_muon_step_workspace_bytes(descs, len(flat))
-                ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
                 _lib.check(L.sln_muon_step_f32(descs, len(flat), self.steps, self.eps, guard.data_ptr(), float(max_norm),
                                                moms.pop(), self.nesterov, ws.data_ptr() if nbytes else 0, nbytes, st),
                            "sln_muon_step_f32")

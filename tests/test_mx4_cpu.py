@@ -64,3 +64,39 @@ def test_host_tensors_and_wrong_arguments_are_refused():
         ops.mx4_linear(torch.zeros(2, 32), torch.zeros(4, 32))
     with pytest.raises(TypeError):
         ops.mx4_linear(None, torch.zeros(4, 32))
+
+
+def test_kept_codes_do_not_travel_with_a_parameter():
+    """Version, address and stream of a weight mean nothing in a copy or another process: what was kept stays behind."""
+    import copy
+    import io
+    import pickle
+    from sln_amodal_amd import nn_ops
+    kept = nn_ops._Mx4Codes((("version", 1, 2), "codes"))
+    assert kept[1] == "codes"
+    assert not pickle.loads(pickle.dumps(kept)) and not copy.deepcopy(kept)
+    w = torch.nn.Parameter(torch.zeros(2, 3))
+    w._sln_mx4_codes = kept
+    f = io.BytesIO()
+    torch.save(w, f)
+    f.seek(0)
+    assert not getattr(torch.load(f, weights_only=False), "_sln_mx4_codes", ())
+
+
+def test_only_products_of_rows_have_a_4bit_form():
+    from sln_amodal_amd import nn_ops
+    for conv, shape in ((torch.nn.Conv2d(4, 8, 3), (2, 4, 5, 5)), (torch.nn.Conv2d(4, 8, 3, dilation=2), (2, 4, 3, 3)),
+                        (torch.nn.Conv2d(4, 8, 3, padding=1), (2, 4, 3, 3)), (torch.nn.Conv2d(4, 8, 1, stride=2), (2, 4, 5, 5)),
+                        (torch.nn.Conv2d(4, 8, 1, groups=2), (2, 4, 1, 1))):
+        with pytest.raises(RuntimeError, match="no product of rows"):
+            nn_ops._mx4_conv(torch.zeros(shape), conv, None, False)
+
+
+def test_codes_of_a_backward_pass_are_aligned():
+    from sln_amodal_amd import _lib
+    L = _lib.lib()
+    buf = (C.c_char * 8192)()
+    p = C.c_void_p((C.addressof(buf) + 255) // 256 * 256)
+    odd = C.c_void_p(p.value + 4)
+    run = lambda xc, wc: L.sln_mx4_linear_bwd(p, 0, 4, None, None, xc, p, wc, p, 2, 4, 8, p, p, p, p, 4096, None)
+    assert run(odd, p) == 1 and run(p, odd) == 1

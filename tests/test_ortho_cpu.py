@@ -120,3 +120,11 @@ def test_model_tags_and_groups():
     m.config.OPTIMIZER = "adam"
     with pytest.raises(ValueError):
         m.make_optimizer(0.001)
+
+
+def test_matrices_longer_than_the_entries_take_are_refused_when_the_optimiser_is_made():
+    from sln_amodal_amd.optim import ClippedMuon
+    p = torch.nn.Parameter(torch.empty(1, (1 << 22) + 1, device="meta"))
+    with pytest.raises(ValueError):
+        ClippedMuon([{"params": [p], "orthogonal": True}], lr=0.1)
+    ClippedMuon([{"params": [torch.nn.Parameter(torch.empty(1, 1 << 22, device="meta"))], "orthogonal": True}], lr=0.1)

@@ -346,3 +346,39 @@ def test_a_captured_step_replays_beside_eager_ones():
         ob.step(5.0)
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(a, b)), r
+
+
+@pytest.mark.parametrize("kind", ["ClippedSGD", "ClippedMuon"])
+def test_momentum_follows_a_weight_into_another_memory_format(kind):
+    """Element i of the momentum is element i of the weight, also after the weight changed to channels-last."""
+    from sln_amodal_amd import optim
+
+    def run(change):
+        gen = torch.Generator().manual_seed(3)
+        p = torch.nn.Parameter(torch.randn(6, 5, 3, 3, generator=gen).cuda())
+        groups = [{"params": [p]}]
+        if kind == "ClippedMuon":
+            groups[0]["orthogonal"] = True
+        opt = getattr(optim, kind)(groups, lr=0.1, momentum=0.5)
+        for r in range(3):
+            if change and r == 1:
+                p.data = p.data.contiguous(memory_format=torch.channels_last)
+            g = torch.zeros(6, 5, 3, 3)                # (one element per row: no sum depends on the order)
+            for i in range(6):
+                g[i, i % 5, i // 5, 0] = 1.0 + i
+            p.grad = g.cuda()
+            opt.step(1e9)
+        return p.detach(), opt.state[p]
+
+    (a, ba), (b, bb) = run(False), run(True)
+    assert b.is_contiguous(memory_format=torch.channels_last) and not b.is_contiguous()
+    assert torch.equal(ba, bb)
+    assert torch.equal(a, b)
+
+
+def test_a_tuple_of_another_type_comes_back_as_a_tuple():
+    import collections
+    from sln_amodal_amd import ops
+    pair = collections.namedtuple("pair", "a b")(torch.randn(4, 6).cuda(), torch.randn(6, 4).cuda())
+    out = ops.orthogonalize(pair)
+    assert isinstance(out, tuple) and torch.equal(out[0], ops.orthogonalize(pair.a)) and out[1].shape == (6, 4)
