@@ -294,3 +294,40 @@ def test_side_streams_and_captured_graphs():
             g.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(outs, eager))
+
+
+@pytest.mark.parametrize("M,N,K", [(7, 20, 70), (300, 130, 1000)])
+def test_a_captured_training_pass_replays(M, N, K):
+    """Forward and backward in one graph (all of it on the stream that captures): every replay equals the eager pass over
+    the same values, with eager passes of other tensors between the replays."""
+    from sln_amodal_amd import ops
+
+    def fresh(seed):
+        return [_x((M, K), seed).cuda(), _x((N, K), seed + 1).cuda(), _x((N,), seed + 2).cuda(), _x((M, N), seed + 3).cuda()]
+
+    def run(x, w, b, gy):
+        y = ops.mx4_linear(x, w, b, relu=True)
+        return (y.detach(),) + torch.autograd.grad(y, (x, w, b), gy)
+
+    static = fresh(1)
+    for t in static[:3]:
+        t.requires_grad_(True)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        run(*static)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            outs = run(*static)
+    torch.cuda.current_stream().wait_stream(s)
+    for r in range(3):
+        new = fresh(10 * r + 20)
+        with torch.no_grad():
+            for t, v in zip(static, new):
+                t.copy_(v)
+        for t in new[:3]:
+            t.requires_grad_(True)
+        want = run(*new)
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
