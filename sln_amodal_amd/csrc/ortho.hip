@@ -671,6 +671,8 @@ __global__ __launch_bounds__(S::THREADS, S::TA == 128 ? 4 : 2) void ortho_apply_
 // one chunk, four rows of four chunks -- meet at most two lanes on a bank.
 //   Gram: wave (block, part of the contraction); the parts meet in S; the block's sums stay in registers for b A.
 //   Apply: a wave takes a group of 32 columns, reads all of its X, and writes P X in its place.
+// Latency-bound: 64 x 576 takes 54 us, 13 to read, norm and lay out, 8.3 a step (clock counts: the Gram products 2.4 us,
+// what is between them and P X 3, P X 3: three rounds of groups, 24 matrix instructions and 220 others each).
 #define SMALL_X 147456
 #define SMALL_S 16384
 __host__ __device__ static inline bool ortho_small(int m, int n) {
@@ -693,7 +695,7 @@ __global__ __launch_bounds__(512) void ortho_small_kernel(OrthoBatch batch, Orth
     constexpr int MP = 32 * MB, CUTS = MB == 2 ? 2 : 4, SP = MB * 128;      // contraction cuts, pitch of S
     char *lx = smem, *ls = smem + SMALL_X;
     const OrthoProb p = batch.p[blockIdx.x];
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int m = ortho_m(p), n = ortho_n(p), groups = (n + 31) / 32, pitch = groups * 128;
     const bool tall = p.rows > p.cols;
     float cf = 1.f;
@@ -702,47 +704,54 @@ __global__ __launch_bounds__(512) void ortho_small_kernel(OrthoBatch batch, Orth
     // ---- u (and the momentum) and its norm: a thread holds up to nine runs of eight neighbours along n
     constexpr int RUNS = SMALL_X / 4 / 8 / 512;
     float u[RUNS][8];
-    double sum = 0.0;
-    auto place = [&](int e, int &i, int &k8) {     // lanes run along G's rows
-        if (tall) { i = e % MP; k8 = e / MP; } else { k8 = e % (groups * 4); i = e / (groups * 4); }
+    // f(s, row, run of eight): runs t + 512 s, lanes along G's rows; stepped, not divided
+    const int width = tall ? MP : groups * 4, dq = 512 / width, dr = 512 - dq * width, b0 = t / width, a0 = t - b0 * width;
+    auto each = [&](auto f) {
+        int a = a0, b = b0;
+#pragma unroll
+        for (int s = 0; s < RUNS; ++s) {
+            f(s, tall ? a : b, tall ? b : a);
+            a += dr; b += dq;
+            if (a >= width) { a -= width; ++b; }
+        }
     };
     const bool vec = !tall && sizeof(T) == 4 && (n & 3) == 0 && (p.gs & 3) == 0 &&
                      !(((uintptr_t)p.g | (uintptr_t)p.buf) & 15);
-    // eight neighbours along n from row i, column k: side by side, or ld apart (tall); zeros outside
-    auto fetch = [&](auto *base, int64_t ld, int i, int k, float *v) {
-        if (vec && i < m && k + 8 <= n) {
-            const float *s = (const float *)base + (int64_t)i * ld + k;
-            *(float4 *)v = *(const float4 *)s;
-            *(float4 *)(v + 4) = *(const float4 *)(s + 4);
-            return;
-        }
-        const auto *s = base + (tall ? (int64_t)k * ld + i : (int64_t)i * ld + k);
-        const int64_t next = tall ? ld : 1;
+    // eight neighbours along n, side by side or ld apart (tall); zeros outside.  (One branch around all the loads: none
+    // waits for another.)
+    auto fetch = [&](auto *base, int64_t ld, float (&v)[RUNS][8]) {
+        if (vec)
+            each([&](int s, int i, int k8) {
+                const float *at = (const float *)base + (int64_t)i * ld + k8 * 8;
 #pragma unroll
-        for (int q = 0; q < 8; ++q) v[q] = i < m && k + q < n ? (float)s[q * next] : 0.f;
+                for (int h = 0; h < 2; ++h) {
+                    float4 x = {0.f, 0.f, 0.f, 0.f};
+                    if (i < m && k8 * 8 + 4 * h < n) x = *(const float4 *)(at + 4 * h);
+                    *(float4 *)(v[s] + 4 * h) = x;
+                }
+            });
+        else
+            each([&](int s, int i, int k8) {
+                const auto *at = base + (tall ? (int64_t)k8 * 8 * ld + i : (int64_t)i * ld + k8 * 8);
+                const int64_t next = tall ? ld : 1;
+#pragma unroll
+                for (int q = 0; q < 8; ++q) v[s][q] = i < m && k8 * 8 + q < n ? (float)at[q * next] : 0.f;
+            });
     };
-#pragma unroll
-    for (int s = 0; s < RUNS; ++s) {
-        int i, k8;
-        place(t + 512 * s, i, k8);
-        fetch((const T *)p.g, p.gs, i, k8 * 8, u[s]);
-    }
+    fetch((const T *)p.g, p.gs, u);
     if (p.buf) {
-#pragma unroll
-        for (int s = 0; s < RUNS; ++s) {
-            int i, k8;
-            place(t + 512 * s, i, k8);
-            const int k = k8 * 8;
-            float b[8];
-            fetch((const float *)p.buf, p.cols, i, k, b);
-            float *d = p.buf + (tall ? (int64_t)k * p.cols + i : (int64_t)i * p.cols + k);
+        float b[RUNS][8];
+        fetch((const float *)p.buf, p.cols, b);
+        each([&](int s, int i, int k8) {
+            float *d = p.buf + (tall ? (int64_t)k8 * 8 * p.cols + i : (int64_t)i * p.cols + k8 * 8);
 #pragma unroll
             for (int q = 0; q < 8; ++q) {
-                u[s][q] = ortho_momentum(rule, u[s][q], cf, b[q]);
-                if (apply && i < m && k + q < n) d[tall ? (int64_t)q * p.cols : q] = b[q];
+                u[s][q] = ortho_momentum(rule, u[s][q], cf, b[s][q]);
+                if (apply && i < m && k8 * 8 + q < n) d[tall ? (int64_t)q * p.cols : q] = b[s][q];
             }
-        }
+        });
     }
+    double sum = 0.0;
 #pragma unroll
     for (int s = 0; s < RUNS; ++s)
 #pragma unroll
@@ -751,11 +760,8 @@ __global__ __launch_bounds__(512) void ortho_small_kernel(OrthoBatch batch, Orth
     const float inv = ortho_inverse(ortho_block_sum(sum, (double *)ls), eps, shift);
     const float up = ldexpf(1.f, shift);
     // ---- X
-#pragma unroll
-    for (int s = 0; s < RUNS; ++s) {
-        int i, k8;
-        place(t + 512 * s, i, k8);
-        if (t + 512 * s >= MP * groups * 4) continue;
+    each([&](int s, int i, int k8) {
+        if (t + 512 * s >= MP * groups * 4) return;
         float v[8];
 #pragma unroll
         for (int q = 0; q < 8; ++q) v[q] = u[s][q] * up * inv;
@@ -763,29 +769,46 @@ __global__ __launch_bounds__(512) void ortho_small_kernel(OrthoBatch batch, Orth
         ortho_parts8(v, h0, h1);
         *(f16x8 *)(lx + small_at(i, pitch, k8 >> 2, k8 & 3)) = h0;
         *(f16x8 *)(lx + small_at(i, pitch, k8 >> 2, 4 + (k8 & 3))) = h1;
-    }
+    });
     __syncthreads();
-    const int frow = lane & 31, fhalf = lane >> 5;
     const int blk = wave % (MB * MB), cut = wave / (MB * MB), bi = blk / MB, bj = blk % MB;
     const float un2 = ORTHO_UNSCALE * ORTHO_UNSCALE;
     for (int step = 0; step < steps; ++step) {
+        // (opaque: addresses that follow from the lane are made where they are used; kept over all the phases they spill)
+        int lane = t & 63;
+        asm volatile("" : "+v"(lane));
+        const int frow = lane & 31, fhalf = lane >> 5;
         // ---- A = X X^T: block (bi, bj), groups of this cut
         f32x16 ga, gb;                             // (two sums: a product waits for the one before it in its own only)
 #pragma unroll
         for (int r = 0; r < 16; ++r) ga[r] = gb[r] = 0.f;
         if (cut < CUTS) {
-            for (int g = groups * cut / CUTS; g < groups * (cut + 1) / CUTS; ++g)
+            auto take = [&](int g, f16x8 (&fa)[2][2], f16x8 (&fb)[2][2]) {
 #pragma unroll
-                for (int kk = 0; kk < 2; ++kk) {
-                    f16x8 fa[2], fb[2];
+                for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
                     for (int q = 0; q < 2; ++q) {
-                        fa[q] = *(const f16x8 *)(lx + small_at(32 * bi + frow, pitch, g, 4 * q + 2 * kk + fhalf));
-                        fb[q] = *(const f16x8 *)(lx + small_at(32 * bj + frow, pitch, g, 4 * q + 2 * kk + fhalf));
+                        fa[kk][q] = *(const f16x8 *)(lx + small_at(32 * bi + frow, pitch, g, 4 * q + 2 * kk + fhalf));
+                        fb[kk][q] = *(const f16x8 *)(lx + small_at(32 * bj + frow, pitch, g, 4 * q + 2 * kk + fhalf));
                     }
-                    if (kk == 0) ga = small_products(fa, fb, ga);
-                    else gb = small_products(fa, fb, gb);
-                }
+            };
+            auto multiply = [&](const f16x8 (&fa)[2][2], const f16x8 (&fb)[2][2]) {
+                ga = small_products(fa[0], fb[0], ga);
+                gb = small_products(fa[1], fb[1], gb);
+            };
+            int g = groups * cut / CUTS;
+            const int end = groups * (cut + 1) / CUTS;
+            f16x8 fa[2][2][2], fb[2][2][2];
+            if (g < end) take(g, fa[0], fb[0]);
+            for (; g + 2 < end; g += 2) {          // the next group's reads behind this one's products
+                take(g + 1, fa[1], fb[1]);
+                multiply(fa[0], fb[0]);
+                take(g + 2, fa[0], fb[0]);
+                multiply(fa[1], fb[1]);
+            }
+            if (g + 1 < end) take(g + 1, fa[1], fb[1]);
+            if (g < end) multiply(fa[0], fb[0]);
+            if (g + 1 < end) multiply(fa[1], fb[1]);
 #pragma unroll
             for (int r = 0; r < 16; ++r) ga[r] += gb[r];
             if (cut > 0) {
@@ -826,7 +849,7 @@ __global__ __launch_bounds__(512) void ortho_small_kernel(OrthoBatch batch, Orth
         f32x16 pa;
         if (cut == 0) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) pa[r] = 0.f;
+            for (int r = 0; r < 16; ++r) pa[r] = gb[r] = 0.f;
 #pragma unroll
             for (int g = 0; g < MB; ++g)
 #pragma unroll
@@ -837,11 +860,12 @@ __global__ __launch_bounds__(512) void ortho_small_kernel(OrthoBatch batch, Orth
                         fa[q] = *(const f16x8 *)(ls + small_at(32 * bi + frow, SP, g, 4 * q + 2 * kk + fhalf));
                         fb[q] = *(const f16x8 *)(ls + small_at(32 * bj + frow, SP, g, 4 * q + 2 * kk + fhalf));
                     }
-                    pa = small_products(fa, fb, pa);
+                    if (kk == 0) pa = small_products(fa, fb, pa);
+                    else gb = small_products(fa, fb, gb);
                 }
 #pragma unroll
             for (int r = 0; r < 16; ++r)
-                pa[r] = ORTHO_C * (down2 * down2) * un2 * pa[r] + ORTHO_B * down2 * ga[r] +
+                pa[r] = ORTHO_C * (down2 * down2) * un2 * (pa[r] + gb[r]) + ORTHO_B * down2 * ga[r] +
                         (32 * bi + nt_acc_row(r, lane) == 32 * bj + frow ? ORTHO_A : 0.f);
         }
         __syncthreads();
