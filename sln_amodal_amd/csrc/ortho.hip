@@ -184,7 +184,8 @@ __device__ __forceinline__ void ortho_lists(const OrthoProb &p, int prob, const 
 
 // Block (c, i): elements [c, c + 1) * ORTHO_CHUNK of matrix i (row-major order) -> one partial sum of squares, added in a
 // fixed order.  The optimiser (buf != NULL): b <- momentum b + cf g is written on the way and the sum is that of
-// u = cf g + momentum b (nesterov) or u = b.  Memory-bound: 4 B read (optimiser: 8 read + 4 written) per element.
+// u = cf g + momentum b (nesterov) or u = b.  Memory-bound: 4 B read (optimiser: 8 read + 4 written) per element (63.9 M
+// elements of an optimiser step, four launches: 182 us = 4.2 TB/s).
 template <typename T>
 __global__ __launch_bounds__(256) void ortho_norm_kernel(OrthoBatch batch, int prob0, OrthoTable tab, OrthoRule rule) {
     __shared__ double s_red[4];
@@ -269,7 +270,8 @@ __device__ __forceinline__ void ortho_store8(char *at, const float *v) {
 }
 
 // ------------------------------------------------------------------------------------------------ G -> X
-// Block = 64 x 128 of X.  Reads 4 B (optimiser: 8, u is made again from g and the new momentum), writes 4 B per element.
+// Block = 64 x 128 of X.  Reads 4 B (optimiser: 8, u is made again from g and the new momentum), writes 4 B per element:
+// bound by memory (63.9 M elements of an optimiser step: 169 us = 4.5 TB/s, a large copy's rate here 4.7).
 template <typename T>
 __global__ __launch_bounds__(256) void ortho_split_kernel(OrthoTable tab, OrthoRule rule, float eps) {
     __shared__ float slab[64 * 129];
@@ -382,6 +384,10 @@ __device__ __forceinline__ void ortho_slab_from_acc(float *slab, const f32x16 (&
 }
 
 // ------------------------------------------------------------------------------------------------ A = X X^T
+// Bound by the matrix instructions and by LDS together: a k-step of 128 x 128 takes 768 clocks of products, and 96 KB of
+// fragments and 32 KB of DMA at 128 B a clock 1024; the two workgroups of a CU cover each other's waits.  125 matrices of
+// a detector (97 GFLOP of products, m (m + 1) n for every matrix and part product): 147 us = 660 TFLOP/s, whole tiles 830;
+// four waves per tile (64 KB of fragments, half the waves) took 5 % of the optimiser step more.
 __global__ __launch_bounds__(OrthoGram::THREADS, 4) void ortho_gram_kernel(OrthoTable tab, int step, int ntiles) {
     typedef OrthoGram S;
     __shared__ __attribute__((aligned(128))) char smem[S::LDS];
@@ -612,7 +618,8 @@ __device__ __forceinline__ void ortho_result(const OrthoProb &p, const f32x16 &a
     }
 }
 
-// LAST: the result instead of the next step's X.
+// LAST: the result instead of the next step's X.  Bound as the Gram products are, and by its stores: 125 matrices of a
+// detector (193 GFLOP of products) 227 us = 850 TFLOP/s with 256 x 256 tiles, the library's fp16 product 1390.
 template <typename T, typename S, bool LAST>
 __global__ __launch_bounds__(S::THREADS, S::TA == 128 ? 4 : 2) void ortho_apply_kernel(OrthoTable tab,
                                                                                          const OrthoTile *list, int ntiles,
