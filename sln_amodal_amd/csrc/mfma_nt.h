@@ -29,7 +29,9 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 // which part products make up a * b
-#define NT_SPLIT2 0   // two parts each: a1 b0 + a0 b1 + a0 b0 (a1 b1 is below the last bit of a0 b0's sum)
+#define NT_SPLIT2 0   // two parts each: a1 b0 + a0 b1 + a0 b0 (a1 b1 is below the last bit of a0 b0's sum); without TRA, a
+                      // wave of up to two blocks sums the corrections apart: the large sum is rounded once per 16 values, not
+                      // three times (with TRA, P X, the roundings differ from element to element and average out)
 #define NT_EXACTB 1   // any number of parts of a, b exact in one part: sum over the parts of a, smallest first
 
 template <typename V>
@@ -146,6 +148,16 @@ __device__ __forceinline__ void nt_tile(const char *a, int64_t a_row_bytes, int 
         for (int j = 0; j < S::FB; ++j)
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+    constexpr bool APART = MODE == NT_SPLIT2 && !TRA && S::FA * S::FB <= 2;
+    f32x16 cor[APART ? S::FA : 1][APART ? S::FB : 1];
+    if constexpr (APART) {
+#pragma unroll
+        for (int i = 0; i < S::FA; ++i)
+#pragma unroll
+            for (int j = 0; j < S::FB; ++j)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) cor[i][j][r] = 0.f;
+    }
 
     const __amdgpu_buffer_rsrc_t bb = nt_buffer(b, INT64_MAX), ba0 = nt_buffer(a, INT64_MAX);
     auto issue = [&](int g) {
@@ -213,7 +225,11 @@ __device__ __forceinline__ void nt_tile(const char *a, int64_t a_row_bytes, int 
             for (int i = 0; i < S::FA; ++i)
 #pragma unroll
                 for (int j = 0; j < S::FB; ++j) {
-                    if constexpr (MODE == NT_SPLIT2) {
+                    if constexpr (APART) {
+                        cor[i][j] = nt_mfma<V>(fa[i][1], fb[j][0], cor[i][j]);
+                        acc[i][j] = nt_mfma<V>(fa[i][0], fb[j][0], acc[i][j]);
+                        cor[i][j] = nt_mfma<V>(fa[i][0], fb[j][1], cor[i][j]);
+                    } else if constexpr (MODE == NT_SPLIT2) {
                         acc[i][j] = nt_mfma<V>(fa[i][1], fb[j][0], acc[i][j]);
                         acc[i][j] = nt_mfma<V>(fa[i][0], fb[j][1], acc[i][j]);
                         acc[i][j] = nt_mfma<V>(fa[i][0], fb[j][0], acc[i][j]);
@@ -223,6 +239,14 @@ __device__ __forceinline__ void nt_tile(const char *a, int64_t a_row_bytes, int 
                     }
                 }
         }
+    }
+    if constexpr (APART) {
+#pragma unroll
+        for (int i = 0; i < S::FA; ++i)
+#pragma unroll
+            for (int j = 0; j < S::FB; ++j)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[i][j][r] += cor[i][j][r];
     }
 #endif
 }

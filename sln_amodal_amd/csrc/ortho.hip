@@ -692,10 +692,10 @@ __device__ __forceinline__ int small_swizzle(int row, int c) { return c ^ (((row
 __device__ __forceinline__ int small_at(int row, int pitch, int g, int c) {
     return row * pitch + g * 128 + small_swizzle(row, c) * 16;
 }
-__device__ __forceinline__ f32x16 small_products(const f16x8 *a, const f16x8 *b, f32x16 acc) {
-    acc = nt_mfma<f16x8>(a[1], b[0], acc);
-    acc = nt_mfma<f16x8>(a[0], b[1], acc);
-    return nt_mfma<f16x8>(a[0], b[0], acc);
+__device__ __forceinline__ void small_products(const f16x8 *a, const f16x8 *b, f32x16 &acc, f32x16 &cor) {
+    cor = nt_mfma<f16x8>(a[1], b[0], cor);
+    acc = nt_mfma<f16x8>(a[0], b[0], acc);
+    cor = nt_mfma<f16x8>(a[0], b[1], cor);
 }
 
 template <typename T, int MB>
@@ -788,7 +788,7 @@ __global__ __launch_bounds__(512) void ortho_small_kernel(OrthoBatch batch, Orth
         asm volatile("" : "+v"(lane));
         const int frow = lane & 31, fhalf = lane >> 5;
         // ---- A = X X^T: block (bi, bj), groups of this cut
-        f32x16 ga, gb;                             // (two sums: a product waits for the one before it in its own only)
+        f32x16 ga, gb;                             // a0 b0; the corrections
 #pragma unroll
         for (int r = 0; r < 16; ++r) ga[r] = gb[r] = 0.f;
         if (cut < CUTS) {
@@ -802,8 +802,8 @@ __global__ __launch_bounds__(512) void ortho_small_kernel(OrthoBatch batch, Orth
                     }
             };
             auto multiply = [&](const f16x8 (&fa)[2][2], const f16x8 (&fb)[2][2]) {
-                ga = small_products(fa[0], fb[0], ga);
-                gb = small_products(fa[1], fb[1], gb);
+                small_products(fa[0], fb[0], ga, gb);
+                small_products(fa[1], fb[1], ga, gb);
             };
             int g = groups * cut / CUTS;
             const int end = groups * (cut + 1) / CUTS;
@@ -869,8 +869,7 @@ __global__ __launch_bounds__(512) void ortho_small_kernel(OrthoBatch batch, Orth
                         fa[q] = *(const f16x8 *)(ls + small_at(32 * bi + frow, SP, g, 4 * q + 2 * kk + fhalf));
                         fb[q] = *(const f16x8 *)(ls + small_at(32 * bj + frow, SP, g, 4 * q + 2 * kk + fhalf));
                     }
-                    if (kk == 0) pa = small_products(fa, fb, pa);
-                    else gb = small_products(fa, fb, gb);
+                    small_products(fa, fb, pa, gb);
                 }
 #pragma unroll
             for (int r = 0; r < 16; ++r)
@@ -919,7 +918,7 @@ __global__ __launch_bounds__(512) void ortho_small_kernel(OrthoBatch batch, Orth
 #pragma unroll
                 for (int kg = 0; kg < MB; ++kg)
 #pragma unroll
-                    for (int kk = 0; kk < 2; ++kk) y[b] = small_products(fx[kg][kk], fp[b][kg][kk], y[b]);
+                    for (int kk = 0; kk < 2; ++kk) small_products(fx[kg][kk], fp[b][kg][kk], y[b], y[b]);
             }
             if (last) {
                 if (apply)
