@@ -20,6 +20,11 @@
 //             ortho_poly_kernel    P's 64 x 64 tiles on and above the diagonal from A A^T, parts of both triangles
 //             (both by ortho_square_kernel in calls with little to do)
 //             ortho_apply_kernel   X <- P X; the last step writes the result, or updates the weights.
+// Where the matrices are wide (ortho_pairs) two steps share their passes over X: P1 and A are symmetric and commute, so the
+// second step's A is P1 A P1, and X <- (P2 P1) X once.  Three products of m^3 (ortho_poly_kernel's other kinds) instead of
+// one of m^2 n and two of m^2 n.  The second A has up to a^2 = 12 times the first one's rounding errors; a pair is followed by
+// a single step, five are 2 + 1 + 2: errors as without pairs, over all spectra that were tried (2 + 2 + 1 loses where half of
+// the singular values are a tenth of the others: 6.7e-6, 2 + 1 + 2 1.0e-6, a float32 evaluation 1.8e-6).
 // X is kept one way only, rows of n.  The Gram matrix contracts along its rows; P X contracts across them and computes
 // (P X)^T with X as the first operand, read through LDS's transposing loads: the 16 accumulator values of a lane are then
 // neighbours along n, and parts go straight from registers to X's rows, 16 bytes a store.
@@ -78,23 +83,24 @@ __host__ __device__ __forceinline__ int ortho_n(const OrthoProb &p) { return p.r
 __host__ __device__ __forceinline__ int64_t ortho_row_bytes(int k) { return (int64_t)((k + 31) / 32) * 128; }
 __host__ __device__ __forceinline__ int ortho_tiles(int v, int tile) { return (v + tile - 1) / tile; }
 
-// operands of a matrix inside the workspace: X (two, in turn), A, P
+// operands of a matrix inside the workspace: X (two, in turn), A, P and, in calls that take steps in pairs, one more
 struct OrthoOperands {
-    char *x, *next, *a, *p;                        // this step's X, the next one's
+    char *x, *next, *a, *p, *t;                    // this turn's X, the next one's
 };
-__device__ __forceinline__ OrthoOperands ortho_operands(const OrthoProb &p, char *ws, int step) {
+__device__ __forceinline__ OrthoOperands ortho_operands(const OrthoProb &p, char *ws, int turn) {
     const int m = ortho_m(p), n = ortho_n(p);
     const int64_t bx = m * ortho_row_bytes(n);
     OrthoOperands o;
-    o.x = ws + p.off + (step & 1) * bx;
-    o.next = ws + p.off + ((step & 1) ^ 1) * bx;
+    o.x = ws + p.off + (turn & 1) * bx;
+    o.next = ws + p.off + ((turn & 1) ^ 1) * bx;
     o.a = ws + p.off + 2 * bx;
     o.p = o.a + m * ortho_row_bytes(m);
+    o.t = o.p + m * ortho_row_bytes(m);
     return o;
 }
-static int64_t ortho_operand_bytes(const OrthoProb &p) {
+static int64_t ortho_operand_bytes(const OrthoProb &p, bool pairs) {
     const int m = ortho_m(p), n = ortho_n(p);
-    return 2 * m * ortho_row_bytes(n) + 2 * m * ortho_row_bytes(m);
+    return 2 * m * ortho_row_bytes(n) + (pairs ? 3 : 2) * m * ortho_row_bytes(m);
 }
 
 // 2^(sign h) for step `step`
@@ -388,14 +394,14 @@ __device__ __forceinline__ void ortho_slab_from_acc(float *slab, const f32x16 (&
 // fragments and 32 KB of DMA at 128 B a clock 1024; the two workgroups of a CU cover each other's waits.  125 matrices of
 // a detector (97 GFLOP of products, m (m + 1) n for every matrix and part product): 147 us = 660 TFLOP/s, whole tiles 830;
 // four waves per tile (64 KB of fragments, half the waves) took 5 % of the optimiser step more.
-__global__ __launch_bounds__(OrthoGram::THREADS, 4) void ortho_gram_kernel(OrthoTable tab, int step, int ntiles) {
+__global__ __launch_bounds__(OrthoGram::THREADS, 4) void ortho_gram_kernel(OrthoTable tab, int turn, int ntiles) {
     typedef OrthoGram S;
     __shared__ __attribute__((aligned(128))) char smem[S::LDS];
     static_assert(64 * (S::TB + 5) * 4 <= S::LDS, "epilogue slab must fit the operand stages");
     const int at = nt_xcd_runs(blockIdx.x, ntiles);
     const OrthoTile w = tab.gram[at];
     const OrthoProb p = tab.prob[w.prob];
-    const OrthoOperands o = ortho_operands(p, tab.ws, step);
+    const OrthoOperands o = ortho_operands(p, tab.ws, turn);
     const int m = ortho_m(p), n = ortho_n(p);
     const int i0 = (w.ij >> 16) * GRAM_TILE, j0 = (w.ij & 0xffff) * GRAM_TILE;
     const int64_t rb = ortho_row_bytes(n);
@@ -455,7 +461,12 @@ __global__ __launch_bounds__(256) void ortho_join_kernel(OrthoTable tab) {
 
 // ------------------------------------------------------------------------------------------------ P = a I + b A + c A^2
 // Short contractions (8 to 32 k-steps): many small tiles and three workgroups per CU hide their latency.  125 matrices of a
-// detector 46 us, 128 x 128 tiles of eight waves 51; 21 matrices 25 and 36.
+// detector (18 GFLOP of products) 46 us, 128 x 128 tiles of eight waves 51; 21 matrices 25 and 36.
+//
+// The kinds of a pair of steps (all symmetric, all from the tiles on and above the diagonal): B = P1 A, A <- P1 B (held
+// times 4^h of the second step), P2 from the new A, and P2 P1, held as a quarter (its norm is up to 3.45^2).
+enum OrthoKind { PAIR_P, PAIR_B, PAIR_A, PAIR_P2, PAIR_PP };
+template <OrthoKind KIND>
 __global__ __launch_bounds__(256, 3) void ortho_poly_kernel(OrthoTable tab, int ntiles, int step) {
     typedef OrthoPoly S;
     constexpr int TILE = S::TA, R = TILE / 2;
@@ -463,22 +474,29 @@ __global__ __launch_bounds__(256, 3) void ortho_poly_kernel(OrthoTable tab, int 
     static_assert(R * (TILE + 5) * 4 <= S::LDS, "epilogue slab must fit the operand stages");
     const OrthoTile w = tab.square[nt_xcd_runs(blockIdx.x, ntiles)];
     const OrthoProb p = tab.prob[w.prob];
-    const OrthoOperands o = ortho_operands(p, tab.ws, step);
+    const OrthoOperands o = ortho_operands(p, tab.ws, 0);
     const int m = ortho_m(p);
     const int i0 = (w.ij >> 16) * TILE, j0 = (w.ij & 0xffff) * TILE;
     const int64_t rb = ortho_row_bytes(m);
     f32x16 acc[S::FA][S::FB];
-    nt_tile<S, f16x8, NT_SPLIT2, false>(o.a + i0 * rb, rb, m - i0, 0, o.a + j0 * rb, rb, m - j0, 0, (m + 31) / 32, smem, acc);
+    constexpr bool POLY = KIND == PAIR_P || KIND == PAIR_P2;
+    const char *u = POLY ? o.a : KIND == PAIR_PP ? o.t : o.p;
+    const char *v = POLY || KIND == PAIR_B ? o.a : KIND == PAIR_A ? o.t : o.p;
+    char *out = KIND == PAIR_P ? o.p : KIND == PAIR_B || KIND == PAIR_P2 ? o.t : o.a;
+    nt_tile<S, f16x8, NT_SPLIT2, false>(u + i0 * rb, rb, m - i0, 0, v + j0 * rb, rb, m - j0, 0, (m + 31) / 32, smem, acc);
     const int t = threadIdx.x;
     float *slab = (float *)smem;
     const float down = ortho_shift(p.shift, step, -1), down2 = down * down;
+    const int fewer = max(0, p.shift - 2 * step) - max(0, p.shift - 2 * (step + 1));        // of h, in the next step
+    const float scale = POLY ? ORTHO_C * (down2 * down2) : KIND == PAIR_A ? ldexpf(1.f, -2 * fewer)
+                                                         : KIND == PAIR_PP ? 0.25f : 1.f;
     for (int h = 0; h < 2; ++h) {
         const int r0 = i0 + R * h;
         if (r0 >= m) break;
         __syncthreads();
-        ortho_slab_from_acc<S>(slab, acc, h, ORTHO_C * (down2 * down2) * (ORTHO_UNSCALE * ORTHO_UNSCALE));
+        ortho_slab_from_acc<S>(slab, acc, h, scale * (ORTHO_UNSCALE * ORTHO_UNSCALE));
         __syncthreads();
-        for (int e = t; e < R * (TILE / 8); e += 256) {     // + b A + a I, in place
+        for (int e = t; POLY && e < R * (TILE / 8); e += 256) {     // + b A + a I, in place
             const int r = e / (TILE / 8), c8 = e % (TILE / 8) * 8, k = j0 + c8;
             if (r0 + r >= m || k >= m) continue;
             const char *at = ortho_at(o.a, rb, r0 + r, k);
@@ -491,7 +509,7 @@ __global__ __launch_bounds__(256, 3) void ortho_poly_kernel(OrthoTable tab, int 
             }
         }
         __syncthreads();
-        ortho_store_sym<R, TILE, 256>(slab, r0, j0, m, o.p, i0 != j0);
+        ortho_store_sym<R, TILE, 256>(slab, r0, j0, m, out, i0 != j0);
     }
 }
 
@@ -620,22 +638,23 @@ __device__ __forceinline__ void ortho_result(const OrthoProb &p, const f32x16 &a
     }
 }
 
+struct OrthoTurn { int turn, step, pair; };         // passes over X before this one; the (first) step it makes; of two
 // LAST: the result instead of the next step's X.  Bound as the Gram products are, and by its stores: 125 matrices of a
 // detector (193 GFLOP of products) 227 us = 850 TFLOP/s with 256 x 256 tiles, the library's fp16 product 1390.
 template <typename T, typename S, bool LAST>
 __global__ __launch_bounds__(S::THREADS, S::TA == 128 ? 4 : 2) void ortho_apply_kernel(OrthoTable tab,
                                                                                          const OrthoTile *list, int ntiles,
-                                                                                         int step, OrthoRule rule) {
+                                                                                         OrthoTurn turn, OrthoRule rule) {
     __shared__ __attribute__((aligned(128))) char smem[S::LDS];
     const OrthoTile w = list[nt_xcd_runs(blockIdx.x, ntiles)];
     const OrthoProb p = tab.prob[w.prob];
-    const OrthoOperands o = ortho_operands(p, tab.ws, step);
+    const OrthoOperands o = ortho_operands(p, tab.ws, turn.turn);
     const int m = ortho_m(p), n = ortho_n(p);
     const int i0 = (w.ij >> 16) * S::TB, j0 = (w.ij & 0xffff) * S::TA;
     const int64_t rx = ortho_row_bytes(n), rp = ortho_row_bytes(m);
     const int groups = (n + 31) / 32;
     f32x16 acc[S::FA][S::FB];
-    nt_tile<S, f16x8, NT_SPLIT2, true>(o.x + (j0 / 32) * 128, rx, groups - j0 / 32, m, o.p + i0 * rp, rp, m - i0, 0,
+    nt_tile<S, f16x8, NT_SPLIT2, true>(o.x + (j0 / 32) * 128, rx, groups - j0 / 32, m, (turn.pair ? o.a : o.p) + i0 * rp, rp, m - i0, 0,
                                        (m + 31) / 32, smem, acc);
     if (LAST && p.buf) {
         const double sq = rule.sqnorm[0];
@@ -643,8 +662,8 @@ __global__ __launch_bounds__(S::THREADS, S::TA == 128 ? 4 : 2) void ortho_apply_
     }
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int k0 = j0 + S::TA / S::WR * (wave / S::WC), r0 = i0 + S::TB / S::WC * (wave % S::WC);
-    const float unscale = ORTHO_UNSCALE * ORTHO_UNSCALE * ortho_shift(p.shift, step, -1) *
-                          (LAST ? 1.f : ortho_shift(p.shift, step + 1, 1));
+    const float unscale = ORTHO_UNSCALE * ORTHO_UNSCALE * (turn.pair ? 4.f : 1.f) * ortho_shift(p.shift, turn.step, -1) *
+                          (LAST ? 1.f : ortho_shift(p.shift, turn.step + 1 + turn.pair, 1));
     if (LAST) {
         float old[2][16];
         if (p.buf) ortho_old(p, k0, r0, m, n, old[0]);
@@ -956,6 +975,7 @@ struct OrthoPlan {
     int nsplit, nsym, ngram, nsquare, napply, nlast, nparts, cut, apply_tile, empty;
     int64_t gram_at[17];             // first entry of each class of Gram items, the long ones first
     bool joined, small, squares;     // squares: short Gram products, not cut
+    bool pairs;                      // two steps per pass over X
 };
 
 // Cuts of a matrix with k columns and their class (0: the longest sixteenth): the launch ends together if it begins with
@@ -1008,11 +1028,17 @@ static int64_t ortho_gram_cut(const D *d, int n) {
     return best;
 }
 
+// A pair of steps saves three times m^2 n and costs three times m^3, in short products that run at half the rate.  Five
+// steps, 2 + 1 + 2, against single ones, measured in turn: 23 matrices of 256 x 2304 315 us and 372, 21 of the heads (m^2 n
+// 6.6 times m^3, an optimiser step) 958 and 1133, 125 of a detector (5.2 times) 2096 and 2484.
+static inline bool ortho_pairs(double wide, double cubes) { return wide > 2. * cubes; }
+
 template <typename D>
 static int ortho_plan(const D *d, int n, OrthoPlan &pl) {
     pl = OrthoPlan();
     pl.small = true;
     int64_t square64 = 0, apply256 = 0, live = 0, longest = 0;
+    double wide = 0., cubes = 0.;                  // m^2 n and m^3 over the matrices
     for (int i = 0; i < n; ++i) {
         if (d[i].rows < 0 || d[i].cols < 0 || d[i].rows > (1 << 22) || d[i].cols > (1 << 22)) return SLN_ERR_INVALID_ARG;
         int64_t m, k;
@@ -1023,6 +1049,8 @@ static int ortho_plan(const D *d, int n, OrthoPlan &pl) {
         pl.small = pl.small && ortho_small((int)m, (int)k);
         square64 += ((m + 63) / 64) * ((m + 63) / 64);
         if ((k + 31) / 32 > longest) longest = (k + 31) / 32;
+        wide += (double)m * m * k;
+        cubes += (double)m * m * m;
         apply256 += ((m + 255) / 256) * ((k + 255) / 256);
     }
     pl.empty = live == 0;
@@ -1034,6 +1062,7 @@ static int ortho_plan(const D *d, int n, OrthoPlan &pl) {
     // not covered by another's loads; the optimiser's last step, which also reads the weights, takes the small ones)
     pl.apply_tile = 4 * apply256 >= 3 * ((apply256 + 255) / 256 * 256) ? 256 : 128;
     pl.squares = square64 <= 256 && longest <= 80;
+    pl.pairs = !pl.squares && ortho_pairs(wide, cubes);
     int64_t nsplit = 0, nsym = 0, ngram = 0, nsquare = 0, napply = 0, nlast = 0, nparts = 0, operands = 0;
     for (int i = 0; i < n; ++i) {
         if (d[i].rows == 0 || d[i].cols == 0) continue;
@@ -1053,7 +1082,7 @@ static int ortho_plan(const D *d, int n, OrthoPlan &pl) {
         napply += ((m + pl.apply_tile - 1) / pl.apply_tile) * ((k + pl.apply_tile - 1) / pl.apply_tile);
         nlast += ((m + 127) / 128) * ((k + 127) / 128);
         nparts += ((int64_t)p.rows * p.cols + ORTHO_CHUNK - 1) / ORTHO_CHUNK;
-        operands += ortho_align(ortho_operand_bytes(p));
+        operands += ortho_align(ortho_operand_bytes(p, pl.pairs));
         const int64_t most = 1 << 28;
         if (nsplit > most || ngram > most || nsquare > most || nlast > most || nparts > most) return SLN_ERR_UNSUPPORTED;
     }
@@ -1107,12 +1136,12 @@ static void ortho_run_small(const D *d, int n, int steps, float eps, const Ortho
 }
 
 template <typename T, typename S>
-static void ortho_apply(const OrthoTable &tab, const OrthoTile *list, int n, int step, bool last, const OrthoRule &rule,
+static void ortho_apply(const OrthoTable &tab, const OrthoTile *list, int n, OrthoTurn turn, bool last, const OrthoRule &rule,
                         hipStream_t stream) {
     if (last)
-        hipLaunchKernelGGL((ortho_apply_kernel<T, S, true>), dim3(n), dim3(S::THREADS), 0, stream, tab, list, n, step, rule);
+        hipLaunchKernelGGL((ortho_apply_kernel<T, S, true>), dim3(n), dim3(S::THREADS), 0, stream, tab, list, n, turn, rule);
     else
-        hipLaunchKernelGGL((ortho_apply_kernel<T, S, false>), dim3(n), dim3(S::THREADS), 0, stream, tab, list, n, step, rule);
+        hipLaunchKernelGGL((ortho_apply_kernel<T, S, false>), dim3(n), dim3(S::THREADS), 0, stream, tab, list, n, turn, rule);
 }
 
 template <typename T, typename D>
@@ -1147,7 +1176,7 @@ static int ortho_run(const D *d, int n, int steps, float eps, const OrthoRule &r
         ortho_desc(d[i], p);
         const int m = ortho_m(p), k = ortho_n(p);
         const int tm = ortho_tiles(m, GRAM_TILE), tp = ortho_tiles(m, OrthoSquare::TA);
-        p.off = off; off += ortho_align(ortho_operand_bytes(p));
+        p.off = off; off += ortho_align(ortho_operand_bytes(p, pl.pairs));
         p.nsplit = (int)ortho_cuts(pl, k);
         p.part0 = part0; p.nparts = sln_div_up((long)p.rows * p.cols, ORTHO_CHUNK); part0 += p.nparts;
         p.split0 = split0; split0 += ortho_tiles(m, 64) * ortho_tiles(k, 128);
@@ -1162,19 +1191,29 @@ static int ortho_run(const D *d, int n, int steps, float eps, const OrthoRule &r
         if (p.nparts > parts) parts = p.nparts;
     }
     hipLaunchKernelGGL((ortho_split_kernel<T>), dim3(pl.nsplit), dim3(256), 0, stream, tab, rule, eps);
-    for (int s = 0; s < steps; ++s) {
+    OrthoTurn turn = {0, 0, 0};
+    for (; turn.step < steps; turn.step += 1 + turn.pair, ++turn.turn) {
+        const int s = turn.step;
+        turn.pair = pl.pairs && s % 3 == 0 && s + 1 < steps;
         if (pl.squares) {
             hipLaunchKernelGGL((ortho_square_kernel<false>), dim3(pl.nsquare), dim3(256), 0, stream, tab, pl.nsquare, s);
             hipLaunchKernelGGL((ortho_square_kernel<true>), dim3(pl.nsquare), dim3(256), 0, stream, tab, pl.nsquare, s);
         } else {
-            hipLaunchKernelGGL(ortho_gram_kernel, dim3(pl.ngram), dim3(OrthoGram::THREADS), 0, stream, tab, s, pl.ngram);
-            if (pl.joined) hipLaunchKernelGGL(ortho_join_kernel, dim3(4 * pl.nsym), dim3(256), 0, stream, tab);
-            hipLaunchKernelGGL(ortho_poly_kernel, dim3(pl.nsquare), dim3(256), 0, stream, tab, pl.nsquare, s);
+            const dim3 tri(pl.nsquare), block(256);
+            hipLaunchKernelGGL(ortho_gram_kernel, dim3(pl.ngram), dim3(OrthoGram::THREADS), 0, stream, tab, turn.turn, pl.ngram);
+            if (pl.joined) hipLaunchKernelGGL(ortho_join_kernel, dim3(4 * pl.nsym), block, 0, stream, tab);
+            hipLaunchKernelGGL((ortho_poly_kernel<PAIR_P>), tri, block, 0, stream, tab, pl.nsquare, s);
+            if (turn.pair) {
+                hipLaunchKernelGGL((ortho_poly_kernel<PAIR_B>), tri, block, 0, stream, tab, pl.nsquare, s);
+                hipLaunchKernelGGL((ortho_poly_kernel<PAIR_A>), tri, block, 0, stream, tab, pl.nsquare, s);
+                hipLaunchKernelGGL((ortho_poly_kernel<PAIR_P2>), tri, block, 0, stream, tab, pl.nsquare, s + 1);
+                hipLaunchKernelGGL((ortho_poly_kernel<PAIR_PP>), tri, block, 0, stream, tab, pl.nsquare, s);
+            }
         }
-        const bool last = s + 1 == steps, weights = last && rule.sqnorm;
-        if (pl.apply_tile == 256 && !weights) ortho_apply<T, OrthoApplyLarge>(tab, tab.apply, pl.napply, s, last, rule, stream);
-        else if (weights) ortho_apply<T, OrthoApplySmall>(tab, tab.last, pl.nlast, s, last, rule, stream);
-        else ortho_apply<T, OrthoApplySmall>(tab, tab.apply, pl.napply, s, last, rule, stream);
+        const bool last = s + 1 + turn.pair == steps, weights = last && rule.sqnorm;
+        if (pl.apply_tile == 256 && !weights) ortho_apply<T, OrthoApplyLarge>(tab, tab.apply, pl.napply, turn, last, rule, stream);
+        else if (weights) ortho_apply<T, OrthoApplySmall>(tab, tab.last, pl.nlast, turn, last, rule, stream);
+        else ortho_apply<T, OrthoApplySmall>(tab, tab.apply, pl.napply, turn, last, rule, stream);
     }
     return sln_launch_status();
 }

@@ -382,3 +382,60 @@ def test_a_tuple_of_another_type_comes_back_as_a_tuple():
     pair = collections.namedtuple("pair", "a b")(torch.randn(4, 6).cuda(), torch.randn(6, 4).cuda())
     out = ops.orthogonalize(pair)
     assert isinstance(out, tuple) and torch.equal(out[0], ops.orthogonalize(pair.a)) and out[1].shape == (6, 4)
+
+
+# wide and long enough for steps in pairs (the second of a pair takes A from the first one's products)
+WIDE = (140, 2700)
+
+
+def _spectrum(s, seed):
+    g = torch.Generator().manual_seed(seed)
+    m, n = WIDE
+    u = torch.linalg.qr(torch.randn(m, m, generator=g, dtype=torch.double))[0]
+    v = torch.linalg.qr(torch.randn(n, m, generator=g, dtype=torch.double))[0]
+    return ((u * s) @ v.t()).float()
+
+
+@pytest.mark.parametrize("kind", ["flat", "linear", "geometric", "outlier", "rank 1", 0.3, 0.1, 0.03, 0.01, 0.003])
+def test_steps_in_pairs_over_spectra(kind):
+    """A number: half of the singular values are that small beside the others."""
+    from sln_amodal_amd import ops
+    m = WIDE[0]
+    s = torch.ones(m, dtype=torch.double)
+    if kind == "linear":
+        s = torch.linspace(1, 1 / m, m, dtype=torch.double)
+    elif kind == "geometric":
+        s = torch.logspace(0, -6, m, dtype=torch.double)
+    elif kind == "outlier":
+        s[0] = 20.0
+    elif kind == "rank 1":
+        s[1:] = 0.0
+    elif kind != "flat":
+        s[m // 2:] = kind
+    g = _spectrum(s, 11)
+    _check(ops.orthogonalize(g.cuda()), g, torch.float32)
+    _check(ops.orthogonalize(g.t().contiguous().cuda()), g.t(), torch.float32)
+
+
+@pytest.mark.parametrize("steps", [1, 2, 3, 4, 6, 7, 10])
+def test_steps_in_pairs_any_number(steps):
+    from sln_amodal_amd import ops
+    g = _matrix(WIDE[0], WIDE[1], steps)
+    _check(ops.orthogonalize(g.cuda(), steps=steps), g, torch.float32, steps=steps)
+
+
+@pytest.mark.parametrize("size", [1e30, 1e-8, 1e-12, 1e-20, 0.0])
+def test_steps_in_pairs_of_large_and_tiny_matrices(size):
+    """Where eps outweighs the norm the operands are held times a power of two that shrinks from step to step."""
+    from sln_amodal_amd import ops
+    g = _matrix(WIDE[0], WIDE[1], 7, size)
+    _check(ops.orthogonalize(g.cuda()), g, torch.float32)
+
+
+def test_steps_in_pairs_keep_non_finite_matrices_apart():
+    from sln_amodal_amd import ops
+    good, bad = _matrix(WIDE[0], WIDE[1], 1), _matrix(WIDE[0], WIDE[1], 2)
+    bad[3, 5] = float("inf")
+    a, b = ops.orthogonalize([good.cuda(), bad.cuda()])
+    _check(a, good, torch.float32)
+    assert torch.isnan(b).all()
