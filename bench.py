@@ -376,7 +376,7 @@ def main_resnext(args, rank, world, dev):
         prof = prof_eager_step
     t = torch.tensor([elapsed], dtype=torch.float64, device=dev)
     if world > 1:
-        dist.all_reduce(t, op=dist.ReduceOp.MAX)
+        parallel.all_reduce(t, op=dist.ReduceOp.MAX)
     elapsed = float(t.item())
     if rank == 0:
         value = batch * world * args.steps / elapsed
@@ -430,7 +430,7 @@ def main_detect(args, rank, world, dev):
     hand-off of amodal_train.py:370-400 per image (unmold to full-size masks + COCO RLE on the device; one count read
     per batch).  Same JSON schema; `metric` names what is timed."""
     import numpy as np
-    from sln_amodal_amd import conv_hip, mask_rle, nn_ops
+    from sln_amodal_amd import conv_hip, mask_rle, nn_ops, parallel
     from sln_amodal_amd.config import Config
     from sln_amodal_amd.model import MaskRCNN
     batch = args.batch if args.batch is not None else 8
@@ -539,7 +539,7 @@ def main_detect(args, rank, world, dev):
     prof, conv_hip.PROFILE = conv_hip.PROFILE, None
     t = torch.tensor([elapsed], dtype=torch.float64, device=dev)
     if world > 1:
-        dist.all_reduce(t, op=dist.ReduceOp.MAX)
+        parallel.all_reduce(t, op=dist.ReduceOp.MAX)
     elapsed = float(t.item())
     if rank == 0:
         counts = model.last_num_detections.cpu().numpy()
@@ -765,7 +765,7 @@ def main():
         skipc_timed = clamped_skips() - skipc_before
         if world > 1:
             tt = torch.tensor([skipc_timed], dtype=torch.int64, device=dev)
-            dist.all_reduce(tt, op=dist.ReduceOp.MAX)
+            parallel.all_reduce(tt, op=dist.ReduceOp.MAX)
             skipc_timed = int(tt.item())
         if skipc_timed == 0 or reruns == 2:
             break
@@ -833,7 +833,7 @@ def main():
         print("bn_affine cache hits/misses:", nn_ops.BN_CACHE_STATS, file=sys.stderr)
     t = torch.tensor([elapsed], dtype=torch.float64, device=dev)
     if world > 1:
-        dist.all_reduce(t, op=dist.ReduceOp.MAX)
+        parallel.all_reduce(t, op=dist.ReduceOp.MAX)
     elapsed = float(t.item())
     final_loss = float(losses[-1]) if losses else float("nan")
     skipped_all = opt.skipped_steps() if hasattr(opt, "skipped_steps") else 0

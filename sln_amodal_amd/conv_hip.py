@@ -290,7 +290,8 @@ class ScaleBook(object):
             self.amax[-1] = -float(self.n)
             torch._C._autograd._unsafe_set_version_counter([self.amax], [v])
             self._n_written = self.n
-        dist.all_reduce(self.amax, op=dist.ReduceOp.MAX)
+        from . import parallel
+        parallel.all_reduce(self.amax, op=dist.ReduceOp.MAX)
         self._n_reduced = True
 
     def link(self, idxs):

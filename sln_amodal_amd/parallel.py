@@ -77,13 +77,50 @@ def set_cpu_affinity(local_rank, local_world):
         return None
 
 
+class _StagedWork(object):
+    """A collective over a host copy of a device tensor: wait() writes the result back."""
+
+    def __init__(self, work, host, tensor):
+        self.work, self.host, self.tensor = work, host, tensor
+
+    def wait(self):
+        self.work.wait()
+        self.tensor.data.copy_(self.host)              # (like the collectives: no new version)
+
+
+def _needs_host(t):
+    """gloo's collectives on device tensors can hang where several ranks share a GPU: it is given host memory only."""
+    return t.is_cuda and dist.get_backend() == "gloo"
+
+
+def all_reduce(t, op=None, async_op=False):
+    """dist.all_reduce in place; under gloo a device tensor goes through host memory (synchronous copies)."""
+    op = dist.ReduceOp.SUM if op is None else op
+    if not _needs_host(t):
+        return dist.all_reduce(t, op=op, async_op=async_op)
+    host = t.detach().cpu()
+    work = _StagedWork(dist.all_reduce(host, op=op, async_op=True), host, t)
+    if async_op:
+        return work
+    work.wait()
+
+
+def broadcast(t, src):
+    """dist.broadcast in place; under gloo a device tensor goes through host memory (synchronous copies)."""
+    if not _needs_host(t):
+        return dist.broadcast(t, src)
+    host = t.detach().cpu()
+    dist.broadcast(host, src)
+    t.data.copy_(host)
+
+
 def broadcast_parameters(module, src=0):
     """Replicas start from identical weights."""
     if not (dist.is_available() and dist.is_initialized()):
         return
     with torch.no_grad():
         for t in list(module.parameters()) + list(module.buffers()):
-            dist.broadcast(t.data, src)
+            broadcast(t.data, src)
             # Caches derived from these tensors (bf16 weight parts, frozen-BN scale/shift) are keyed
             # by the tensors' version counters, which writing through `.data` does not advance: bump
             # them, or a rank would keep computing with what it held before the broadcast.
@@ -256,7 +293,7 @@ class GradientAllReducer(object):
                 else:
                     flat[self._veto_off:self._veto_off + 4].copy_(v.expand(4))
         self.trace.append(bi)
-        self._work[bi] = dist.all_reduce(flat, op=dist.ReduceOp.SUM, async_op=True)
+        self._work[bi] = all_reduce(flat, async_op=True)
 
     def _local_veto(self, flat):
         """This rank's veto of the step: conv_hip.clamp_veto() on the GPU, nothing on the host (tests override it)."""

@@ -263,3 +263,33 @@ def test_self_launcher_names_the_rank_that_died_first():
     assert not [l for l in r.stdout.splitlines() if l.startswith("{")]
     assert "bench.py: rank exit codes [1, 1]" in r.stderr, r.stderr[-1500:]
     assert "No HIP GPUs are available" in r.stderr
+
+
+def test_gloo_is_given_host_memory_only(tmp_path, monkeypatch):
+    """Device tensors go through a host copy under gloo (its collectives on device tensors can hang where ranks share a
+    GPU): what gloo is handed is never the tensor itself, and the tensor holds the result after wait()."""
+    import torch.distributed as dist
+    from sln_amodal_amd import parallel
+    dist.init_process_group("gloo", init_method="file://%s" % (tmp_path / "store"), rank=0, world_size=1)
+    try:
+        handed = []
+        reduce, cast = dist.all_reduce, dist.broadcast
+        monkeypatch.setattr(dist, "all_reduce", lambda t, **kw: (handed.append(t), t.mul_(3), reduce(t, **kw))[-1])
+        monkeypatch.setattr(dist, "broadcast", lambda t, src: (handed.append(t), t.add_(1), cast(t, src))[-1])
+        t = torch.arange(4.0)
+        assert not parallel._needs_host(t)
+        parallel.all_reduce(t)
+        assert handed.pop() is t and t.tolist() == [0, 3, 6, 9]
+        monkeypatch.setattr(parallel, "_needs_host", lambda t: True)
+        monkeypatch.setattr(torch.Tensor, "cpu", lambda self: self.clone())      # (a device tensor's copy)
+        v = t._version
+        work = parallel.all_reduce(t, async_op=True)
+        assert t.tolist() == [0, 3, 6, 9]
+        work.wait()
+        assert t.tolist() == [0, 9, 18, 27] and handed.pop() is not t and t._version == v
+        parallel.all_reduce(t, op=dist.ReduceOp.MAX)
+        assert t.tolist() == [0, 27, 54, 81] and handed.pop() is not t
+        parallel.broadcast(t, 0)
+        assert t.tolist() == [1, 28, 55, 82] and handed.pop() is not t
+    finally:
+        dist.destroy_process_group()
