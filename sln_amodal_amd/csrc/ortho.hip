@@ -1030,7 +1030,8 @@ static int64_t ortho_gram_cut(const D *d, int n) {
 
 // A pair of steps saves three times m^2 n and costs three times m^3, in short products that run at half the rate.  Five
 // steps, 2 + 1 + 2, against single ones, measured in turn: 23 matrices of 256 x 2304 315 us and 372, 21 of the heads (m^2 n
-// 6.6 times m^3, an optimiser step) 958 and 1133, 125 of a detector (5.2 times) 2096 and 2484.
+// 6.6 times m^3, an optimiser step) 958 and 1133, 125 of a detector (5.2 times) 2096 and 2484.  Around the limit: 16 of 512 x
+// 768 442 and 422, x 1024 452 and 449, x 1536 522 and 564; 4 of 1024 x 1536 611 and 604, x 2048 641 and 655.
 static inline bool ortho_pairs(double wide, double cubes) { return wide > 2. * cubes; }
 
 template <typename D>
