@@ -5,9 +5,11 @@
 // The rounding passes its gradient through unchanged, saturated values included.  w^ and x^ are what the forward
 // multiplied: e2m1 values times powers of two have two significant bits, so ONE bf16 part holds them exactly, and a
 // float32 gradient is exactly the sum of three bf16 parts (8 bits of its significand each, cut, not rounded).
-// Three (two: 16-bit gradients) products on the bf16 matrix instructions into fp32 accumulators are therefore the
-// float32 products: nothing is rounded before the sum.  (Parts below bf16's smallest normal, 2^-126, may be lost.)
-// For 16-bit types z * scale is cut to 16 bits: gx has 8 or 11.
+// Products of as many parts on the bf16 matrix instructions into fp32 accumulators are therefore the float32 products:
+// nothing is rounded before the sum but z * scale, to float32.  (Parts below bf16's smallest normal, 2^-126, may be lost.)
+// Three parts for float32 gradients and for z * scale of any type, two where a 16-bit z is taken as it is.  (z * scale cut
+// to two parts, 16 bits, costs the sums of gx up to 2^-15 of their terms, all in one direction: of 1501 x 1024 bfloat16
+// results over 324 outputs 0.6 % were not the nearest; with three parts 0.014 %, a float32 product's 0.023 %.)
 //
 // Both products contract along rows (mfma_nt.h): gx over the outputs, so w^ is laid out [K][N]; gw over the rows of the
 // batch, so z is laid out [N][M] and x^ [K][M].
@@ -59,7 +61,7 @@ struct MgPrep {
     unsigned split, turn_w;
 };
 
-template <typename T, int P>
+template <typename T, int PX, int PW>
 __device__ __forceinline__ void mg_split(const MgPrep &p, unsigned b, float *z, float (*s_bias)[64]) {
     const unsigned tn = (unsigned)(p.N + 63) / 64;
     const int t = threadIdx.x, m0 = (int)(b / tn) * 64, n0 = (int)(b % tn) * 64;
@@ -80,7 +82,7 @@ __device__ __forceinline__ void mg_split(const MgPrep &p, unsigned b, float *z, 
     if (p.bias_part && t < 64 && n0 + t < N)
         p.bias_part[(int64_t)(m0 / 64) * N + n0 + t] = (s_bias[0][t] + s_bias[1][t]) + (s_bias[2][t] + s_bias[3][t]);
     if (p.rows) {
-        const int64_t rb = mg_row_bytes(N, P);
+        const int64_t rb = mg_row_bytes(N, PX);
         const int npad = (N + 31) & ~31;
         for (int e = t; e < 512; e += 256) {
             const int i = e >> 3, k = (e & 7) * 8;
@@ -91,11 +93,11 @@ __device__ __forceinline__ void mg_split(const MgPrep &p, unsigned b, float *z, 
                 v[q] = z[i * MG_PITCH + k + q];
                 if (p.scale && n0 + k + q < N) v[q] *= p.scale[n0 + k + q];
             }
-            mg_store8<P>(p.rows, m0 + i, rb, n0 + k, v);
+            mg_store8<PX>(p.rows, m0 + i, rb, n0 + k, v);
         }
     }
     if (p.cols) {
-        const int64_t rb = mg_row_bytes(M, P);
+        const int64_t rb = mg_row_bytes(M, PW);
         const int mpad = (M + 31) & ~31;
         for (int e = t; e < 512; e += 256) {
             const int j = e >> 3, k = (e & 7) * 8;
@@ -103,7 +105,7 @@ __device__ __forceinline__ void mg_split(const MgPrep &p, unsigned b, float *z, 
             float v[8];
 #pragma unroll
             for (int q = 0; q < 8; ++q) v[q] = z[(k + q) * MG_PITCH + j];
-            mg_store8<P>(p.cols, n0 + j, rb, m0 + k, v);
+            mg_store8<PW>(p.cols, n0 + j, rb, m0 + k, v);
         }
     }
 }
@@ -137,11 +139,11 @@ __device__ __forceinline__ void mg_turn(const unsigned *codes, const uint8_t *sc
     }
 }
 
-template <typename T, int P>
+template <typename T, int PX, int PW>
 __global__ __launch_bounds__(256) void mx4_grad_prep_kernel(const MgPrep p) {
     __shared__ float z[64 * MG_PITCH];
     __shared__ float s_bias[4][64];
-    if (blockIdx.x < p.split) mg_split<T, P>(p, blockIdx.x, z, s_bias);
+    if (blockIdx.x < p.split) mg_split<T, PX, PW>(p, blockIdx.x, z, s_bias);
     else if (blockIdx.x < p.split + p.turn_w) mg_turn(p.w_codes, p.w_scales, p.N, p.K, p.wt, blockIdx.x - p.split, z);
     else mg_turn(p.x_codes, p.x_scales, p.M, p.K, p.xt, blockIdx.x - p.split - p.turn_w, z);
 }
@@ -201,21 +203,22 @@ __device__ __forceinline__ void mg_product(const MgProduct &p, int at, char *sme
 }
 
 // Both products (if their tiles are alike) and the bias sums in one launch (x: gx, w: gw; tiles = 0: not here); the tiles
-// with the longer contraction first.
-template <typename T, typename S>
-__global__ __launch_bounds__(S::THREADS, 4) void mx4_grad_product_kernel(
+// with the longer contraction first.  SX, SW: the same tile, as many parts as each first operand has.
+template <typename T, typename SX, typename SW>
+__global__ __launch_bounds__(SX::THREADS, 4) void mx4_grad_product_kernel(
     const MgProduct x, const MgProduct w, const float *__restrict__ bias_part, int bias_blocks, int N,
     float *__restrict__ gb) {
-    __shared__ __attribute__((aligned(128))) char smem[S::LDS];
+    static_assert(SX::THREADS == SW::THREADS, "one launch shape");
+    __shared__ __attribute__((aligned(128))) char smem[SX::LDS > SW::LDS ? SX::LDS : SW::LDS];
     const bool w_first = w.groups > x.groups;
     const unsigned lead = w_first ? w.tiles : x.tiles, all = x.tiles + w.tiles;
     if (blockIdx.x < all) {
         const bool is_w = w_first == (blockIdx.x < lead);
         const int at = blockIdx.x < lead ? nt_xcd_order(blockIdx.x, lead) : nt_xcd_order(blockIdx.x - lead, all - lead);
-        if (is_w) mg_product<float, S>(w, at, smem);
-        else mg_product<T, S>(x, at, smem);
+        if (is_w) mg_product<float, SW>(w, at, smem);
+        else mg_product<T, SX>(x, at, smem);
     } else {                                       // partial bias sums, added in order in double
-        const int n = (blockIdx.x - all) * S::THREADS + threadIdx.x;
+        const int n = (blockIdx.x - all) * SX::THREADS + threadIdx.x;
         if (n >= N) return;
         double s = 0.0;
         for (int b = 0; b < bias_blocks; ++b) s += bias_part[(int64_t)b * N + n];
@@ -256,15 +259,15 @@ static inline int mg_cuts(int64_t RA, int64_t RB, int64_t groups) {
     if (c > 32) c = 32;
     return c < 1 ? 1 : (int)c;
 }
-static void mg_plan(int64_t M, int64_t N, int64_t K, int parts, bool gx, bool gw, bool gb, MgPlan &p) {
+static void mg_plan(int64_t M, int64_t N, int64_t K, int px, int pw, bool gx, bool gw, bool gb, MgPlan &p) {
     int64_t at = 0;
     // (each product's own rule, whatever else is wanted: its bits do not depend on that)
     p.gx_large = mg_large(M, K);
     p.gw_large = mg_large(N, K);
     p.gx_cuts = p.gx_large ? 1 : mg_cuts(M, K, (N + 31) / 32);
     p.gw_cuts = p.gw_large ? 1 : mg_cuts(N, K, (M + 31) / 32);
-    p.z_rows = at; at += gx ? mg_align(M * mg_row_bytes(N, parts)) : 0;
-    p.z_cols = at; at += gw ? mg_align(N * mg_row_bytes(M, parts)) : 0;
+    p.z_rows = at; at += gx ? mg_align(M * mg_row_bytes(N, px)) : 0;
+    p.z_cols = at; at += gw ? mg_align(N * mg_row_bytes(M, pw)) : 0;
     p.wt = at; at += gx ? mg_align(K * mg_row_bytes(N, 1)) : 0;
     p.xt = at; at += gw ? mg_align(K * mg_row_bytes(M, 1)) : 0;
     p.bias = at; at += gb ? mg_align((M + 63) / 64 * N * 4) : 0;
@@ -272,13 +275,14 @@ static void mg_plan(int64_t M, int64_t N, int64_t K, int parts, bool gx, bool gw
     p.slab_w = at; at += gw && p.gw_cuts > 1 ? mg_align(p.gw_cuts * N * K * 4) : 0;
     p.bytes = at;
 }
-static inline int mg_parts(int dtype) { return dtype == SLN_DTYPE_F32 ? 3 : 2; }
+// parts of z, and of z * scale
+static inline int mg_parts(int dtype, bool scaled) { return dtype == SLN_DTYPE_F32 || scaled ? 3 : 2; }
 
 extern "C" size_t sln_mx4_linear_bwd_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype, int want_gx, int want_gw,
                                                      int want_gb) {
     if (M < 1 || N < 1 || K < 1) return 0;
     MgPlan p;
-    mg_plan(M, N, K, mg_parts(dtype), want_gx, want_gw, want_gb, p);
+    mg_plan(M, N, K, mg_parts(dtype, true), mg_parts(dtype, false), want_gx, want_gw, want_gb, p);   // with or without scale
     return (size_t)p.bytes;
 }
 
@@ -298,7 +302,7 @@ static inline unsigned mg_join_blocks(const MgProduct &p) {
     return (unsigned)(blocks < 4096 ? blocks : 4096);
 }
 
-template <typename T, int P>
+template <typename T, int PX, int PW>
 static void mg_run(const void *gy, int64_t stride, const void *y, const float *scale, const uint8_t *xc, const uint8_t *xs,
                    const uint8_t *wc, const uint8_t *wsc, int64_t M, int64_t N, int64_t K, void *gx, float *gw, float *gb,
                    const MgPlan &pl, char *ws, hipStream_t st) {
@@ -313,7 +317,7 @@ static void mg_run(const void *gy, int64_t stride, const void *y, const float *s
     const int64_t tm = (M + 63) / 64, tn = (N + 63) / 64, tk = (K + 63) / 64;
     p.split = (unsigned)(tm * tn);
     p.turn_w = gx ? (unsigned)(tk * tn) : 0u;
-    hipLaunchKernelGGL((mx4_grad_prep_kernel<T, P>), dim3(p.split + p.turn_w + (gw ? (unsigned)(tk * tm) : 0u)), dim3(256),
+    hipLaunchKernelGGL((mx4_grad_prep_kernel<T, PX, PW>), dim3(p.split + p.turn_w + (gw ? (unsigned)(tk * tm) : 0u)), dim3(256),
                        0, st, p);
     const MgProduct jx = mg_job(ws + pl.z_rows, M, ws + pl.wt, K, N, pl.gx_cuts, pl.gx_large, nullptr, gx,
                                 ws + pl.slab_x);
@@ -321,15 +325,15 @@ static void mg_run(const void *gy, int64_t stride, const void *y, const float *s
                                 ws + pl.slab_w);
     const MgProduct none = {};
     auto launch = [&](const MgProduct &x, const MgProduct &w, bool large, float *bias) {
-        const unsigned threads = MgSmall<P>::THREADS;
-        static_assert(MgSmall<P>::THREADS == MgLarge<P>::THREADS, "one launch shape");
+        const unsigned threads = MgSmall<PX>::THREADS;
+        static_assert(MgSmall<PX>::THREADS == MgLarge<PX>::THREADS, "one launch shape");
         const dim3 grid(x.tiles + w.tiles + (bias ? (unsigned)(N + threads - 1) / threads : 0u));
         if (grid.x == 0) return;
         if (large)
-            hipLaunchKernelGGL((mx4_grad_product_kernel<T, MgLarge<P>>), grid, dim3(threads), 0, st, x, w, p.bias_part,
+            hipLaunchKernelGGL((mx4_grad_product_kernel<T, MgLarge<PX>, MgLarge<PW>>), grid, dim3(threads), 0, st, x, w, p.bias_part,
                                (int)tm, (int)N, bias);
         else
-            hipLaunchKernelGGL((mx4_grad_product_kernel<T, MgSmall<P>>), grid, dim3(threads), 0, st, x, w, p.bias_part,
+            hipLaunchKernelGGL((mx4_grad_product_kernel<T, MgSmall<PX>, MgSmall<PW>>), grid, dim3(threads), 0, st, x, w, p.bias_part,
                                (int)tm, (int)N, bias);
     };
     if (!gx || !gw || pl.gx_large == pl.gw_large) {
@@ -356,18 +360,20 @@ extern "C" int sln_mx4_linear_bwd(const void *gy, int dtype, int64_t gy_stride, 
     if ((gx && (!w_codes || !w_scales)) || (gw && (!x_codes || !x_scales))) return SLN_ERR_INVALID_ARG;
     if ((gx && ((uintptr_t)w_codes & 15)) || (gw && ((uintptr_t)x_codes & 15))) return SLN_ERR_INVALID_ARG;
     MgPlan pl;
-    mg_plan(M, N, K, mg_parts(dtype), gx, gw, gb, pl);
+    mg_plan(M, N, K, mg_parts(dtype, scale != nullptr), mg_parts(dtype, false), gx, gw, gb, pl);
     if (pl.bytes && (!workspace || ((uintptr_t)workspace & 255))) return SLN_ERR_INVALID_ARG;
     if (workspace_bytes < (size_t)pl.bytes) return SLN_ERR_WORKSPACE;
     if (!gx && !gw && !gb) return SLN_OK;
     sln_enter();
     char *ws = (char *)workspace;
     hipStream_t st = (hipStream_t)stream;
-    if (dtype == SLN_DTYPE_F32)
-        mg_run<float, 3>(gy, gy_stride, y, scale, x_codes, x_scales, w_codes, w_scales, M, N, K, gx, gw, gb, pl, ws, st);
-    else if (dtype == SLN_DTYPE_BF16)
-        mg_run<__bf16, 2>(gy, gy_stride, y, scale, x_codes, x_scales, w_codes, w_scales, M, N, K, gx, gw, gb, pl, ws, st);
-    else
-        mg_run<_Float16, 2>(gy, gy_stride, y, scale, x_codes, x_scales, w_codes, w_scales, M, N, K, gx, gw, gb, pl, ws, st);
+#define MG_GO(T, PX, PW)                                                                                               \
+    mg_run<T, PX, PW>(gy, gy_stride, y, scale, x_codes, x_scales, w_codes, w_scales, M, N, K, gx, gw, gb, pl, ws, st)
+    if (dtype == SLN_DTYPE_F32) MG_GO(float, 3, 3);
+    else if (dtype == SLN_DTYPE_BF16 && scale) MG_GO(__bf16, 3, 2);
+    else if (dtype == SLN_DTYPE_BF16) MG_GO(__bf16, 2, 2);
+    else if (scale) MG_GO(_Float16, 3, 2);
+    else MG_GO(_Float16, 2, 2);
+#undef MG_GO
     return sln_launch_status();
 }
