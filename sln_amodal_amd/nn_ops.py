@@ -83,13 +83,14 @@ def _mx4_rows(x, weight, w2, bias, scale, relu):
     """act((x w2^T) * scale + bias) on microscaled 4-bit operands; w2() makes the [N, K] rows of `weight`.  In evaluation
     the weight's codes are kept on the parameter until its version counter moves (edits through `.data` do not move it:
     delete `weight._sln_mx4_codes` after one) or the stream changes; a captured graph rounds the weight itself, so that
-    its replays follow the weight and read no memory that is given back when the weight changes."""
+    its replays follow the weight and read no memory that is given back when the weight changes.  A weight that a captured
+    optimiser step updates (`_sln_captured`) is rounded in every call: replays move it, but not its version."""
     from . import mx4
     if not x.is_cuda:
         raise RuntimeError("4-bit layers run on the GPU only (no CPU fallback in sln_amodal_amd)")
     if torch.is_grad_enabled() and weight.requires_grad:
         return mx4.mx4_linear(x, w2(), bias, scale=scale, relu=relu)
-    if torch.cuda.is_current_stream_capturing():
+    if torch.cuda.is_current_stream_capturing() or getattr(weight, "_sln_captured", False):
         with torch.no_grad():
             codes = mx4.mx4_quantize(w2())
         return mx4.mx4_linear(x, codes, bias, scale=scale, relu=relu)

@@ -105,6 +105,14 @@ class ClippedSGD(object):
                 elif p.grad is not None:
                     p.grad.zero_()
 
+    def replayed(self):
+        """To be called when graphs that captured step() were replayed, before anything else reads the weights: what layers
+        keep of a weight (its 16-bit parts, folded biases) goes by the weight's version counter, and a replay writes weights
+        without moving it."""
+        ps = list({id(p): p for _, ps in self._captured for p in ps}.values())
+        if ps:
+            torch._C._autograd._unsafe_set_version_counter(ps, [p._version + 1 for p in ps])
+
     def _active(self):
         out = []
         for g in self.param_groups:
@@ -134,7 +142,10 @@ class ClippedSGD(object):
         """veto: float32 [1] device tensor or None; > 0 = do not apply this step (conv_hip.clamp_veto(), or the
         all-reduced one of parallel.GradientAllReducer): the update is skipped on the device through the same guard
         as a non-finite gradient norm and counted in `skipped` and `skipped_clamped`; `last_norm` stays the real
-        norm.  No host sync either way."""
+        norm.  No host sync either way.
+
+        A step may be captured into a graph, with an eager step over the same parameters before it.  Its replays use the
+        hyper-parameters of the capture and the gradient tensors that were there: keep those, and call replayed()."""
         act = self._active()
         if not act:
             return None
@@ -201,7 +212,9 @@ class ClippedSGD(object):
             if self._spare is None or self._spare.shape[1] != n:
                 raise RuntimeError("take an eager step over the same parameters before each captured one")
             stage, self._spare = [self._spare, None], None
-            self._captured.append(stage[0])
+            self._captured.append((stage[0], ps))
+            for p in ps:                       # (its replays write p without moving p's version: nothing made from p is kept)
+                p._sln_captured = True
         elif self._spare is None or self._spare.shape[1] != n:
             self._spare = torch.empty((3, n), dtype=torch.int64, pin_memory=True)
         host = [[t.data_ptr() for t in ts] for ts in (ps, gs, bs)]

@@ -1,0 +1,120 @@
+"""GPU tests of optimiser steps that are captured into graphs beside what goes on eagerly: what layers keep of the weights, what
+the graphs' launches read, and what the optimiser's state does meanwhile.  Every comparison is for equal bits: a captured
+step is the same launches over the same values."""
+import gc
+import weakref
+
+import pytest
+import torch
+from torch import nn
+
+pytestmark = pytest.mark.gpu
+KINDS = ["ClippedSGD", "ClippedMuon"]
+
+
+def _make(kind, shapes, seed=8):
+    from sln_amodal_amd import optim
+    gen = torch.Generator().manual_seed(seed)
+    ps = [nn.Parameter((torch.randn(s, generator=gen) * 0.1).cuda()) for s in shapes]
+    return ps, _optimiser(kind, ps)
+
+
+def _optimiser(kind, ps, lr=0.1):
+    from sln_amodal_amd import optim
+    if kind == "ClippedSGD":
+        return optim.ClippedSGD([{"params": ps, "weight_decay": 1e-3}], lr=lr, momentum=0.8)
+    mats, rest = [p for p in ps if p.dim() > 1], [p for p in ps if p.dim() < 2]
+    return optim.ClippedMuon([{"params": mats, "orthogonal": True}, {"params": rest}], lr=lr, momentum=0.8)
+
+
+def _grads(ps, seed):
+    gen = torch.Generator().manual_seed(seed)
+    return [torch.randn(p.shape, generator=gen).cuda() for p in ps]
+
+
+def _set(ps, gs):
+    for p, g in zip(ps, gs):
+        p.grad = g
+
+
+def _capture(opt, **kw):
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(s):
+        with torch.cuda.graph(graph, stream=s):
+            opt.step(5.0, **kw)
+    torch.cuda.current_stream().wait_stream(s)
+    return graph
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_a_4_bit_layer_sees_the_weights_that_replays_wrote(kind):
+    """Evaluate (the weight's codes are kept), replay a captured step, evaluate again: the codes of the new weight."""
+    from sln_amodal_amd import nn_ops, ops
+    lin = nn.Linear(96, 40).cuda()
+    lin.weight._sln_mx4 = True
+    ps = [lin.weight, lin.bias]
+    opt = _optimiser(kind, ps)
+    x = _grads([torch.empty(30, 96)], 1)[0]
+    static = _grads(ps, 2)
+    _set(ps, static)
+    fresh = lambda: ops.mx4_linear(x, lin.weight.detach().clone(), lin.bias.detach().clone())
+    with torch.no_grad():
+        first = nn_ops.linear(x, lin)
+        opt.step(5.0)
+        assert torch.equal(nn_ops.linear(x, lin), fresh())
+        graph = _capture(opt)
+        assert torch.equal(nn_ops.linear(x, lin), fresh())       # (kept here, were the weight not in a captured step)
+        for r in range(3):
+            for g, v in zip(static, _grads(ps, 10 + r)):
+                g.copy_(v)
+            graph.replay()
+            y = nn_ops.linear(x, lin)
+            assert torch.equal(y, fresh()) and not torch.equal(y, first), r
+            first = y
+
+
+def test_other_layers_see_them_after_replayed():
+    from sln_amodal_amd import nn_ops
+    conv = nn.Conv2d(64, 64, 3, padding=1).cuda()
+    ps = list(conv.parameters())
+    opt = _optimiser("ClippedSGD", ps)
+    x = _grads([torch.empty(1, 64, 16, 16)], 1)[0].contiguous(memory_format=torch.channels_last)
+    static = _grads(ps, 2)
+    _set(ps, static)
+
+    def fresh():                                                 # the same layer as a new module: nothing kept
+        other = nn.Conv2d(64, 64, 3, padding=1).cuda()
+        other.load_state_dict(conv.state_dict())
+        return nn_ops.conv_bn_act(x, other)
+
+    with torch.no_grad():
+        first = nn_ops.conv_bn_act(x, conv)
+        opt.step(5.0)
+        graph = _capture(opt)
+        nn_ops.conv_bn_act(x, conv)
+        for r in range(3):
+            for g, v in zip(static, _grads(ps, 10 + r)):
+                g.copy_(v)
+            graph.replay()
+            opt.replayed()
+            y, want = nn_ops.conv_bn_act(x, conv), fresh()
+            # (operand scales are kept per layer: equal up to their choice, 2^-20 of the largest; stale weights are O(1) off)
+            assert (y - want).abs().max() <= 1e-4 * want.abs().max() and (y - first).abs().max() > 1e-2 * want.abs().max(), r
+            first = y
+
+
+def test_replayed_moves_the_versions_of_captured_weights_only():
+    ps, opt = _make("ClippedSGD", [(20, 30), (30,)])
+    other = nn.Parameter(torch.ones(3, device="cuda"))
+    opt.param_groups[0]["params"].append(other)
+    versions = [p._version for p in ps + [other]]
+    opt.replayed()
+    assert versions == [p._version for p in ps + [other]]
+    _set(ps, _grads(ps, 3))
+    opt.step(5.0)
+    _capture(opt)
+    versions = [p._version for p in ps + [other]]
+    opt.replayed()
+    assert [p._version for p in ps + [other]] == [versions[0] + 1, versions[1] + 1, versions[2]]
