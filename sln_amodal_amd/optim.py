@@ -9,6 +9,7 @@ import torch
 from . import _lib
 
 CHUNK = 1 << 16
+_EAGER_FIRST = "take an eager step over the same parameters before each captured one"
 
 
 class ClippedSGD(object):
@@ -30,7 +31,7 @@ class ClippedSGD(object):
         self.skipped_clamped = None          # device int32: of those, the steps vetoed for clamped operand blocks
         self._plan_key, self._plan = None, None
         self._ring, self._turn = [], 0       # pinned staging buffers of the pointer tables
-        self._spare, self._captured = None, []        # the next captured step's, those of captured steps
+        self._spare, self._captured = None, []        # the next captured step's table; what captured steps read and write
         self.capturing = False               # inside a HIP-graph capture: no event waits (the tables are static)
         self.last_norm = None
 
@@ -109,7 +110,7 @@ class ClippedSGD(object):
         """To be called when graphs that captured step() were replayed, before anything else reads the weights: what layers
         keep of a weight (its 16-bit parts, folded biases) goes by the weight's version counter, and a replay writes weights
         without moving it."""
-        ps = list({id(p): p for _, ps in self._captured for p in ps}.values())
+        ps = list({id(p): p for c in self._captured for p in c[0]}.values())
         if ps:
             torch._C._autograd._unsafe_set_version_counter(ps, [p._version + 1 for p in ps])
 
@@ -124,6 +125,8 @@ class ClippedSGD(object):
     def _chunks(self, numels, wds, device):
         key = (tuple(numels), tuple(wds))
         if key != self._plan_key:
+            if self._capturing():
+                raise RuntimeError(_EAGER_FIRST)
             ct, co = [], []
             for i, n in enumerate(numels):
                 for off in range(0, n, CHUNK):
@@ -194,6 +197,9 @@ class ClippedSGD(object):
             ps.append(p); gs.append(g); bs.append(b)
         return ps, gs, bs
 
+    def _capturing(self):
+        return self.capturing or torch.cuda.is_current_stream_capturing()
+
     def _upload(self, ps, gs, bs, dev):
         """Pointer tables [3, n] (weights, gradients, momentum), as lists and on the device: gradients are fresh
         allocations every step, so the tables are re-sent each time -- from pinned staging buffers and asynchronously, so
@@ -201,22 +207,25 @@ class ClippedSGD(object):
         is reused only after the copy that read it has completed (4 in flight); one that a captured graph copies from is
         never written again (its replays read it)."""
         n = len(ps)
-        if not self._ring or self._ring[0][0].shape[1] != n:
-            self._ring = [[torch.empty((3, n), dtype=torch.int64, pin_memory=True), None] for _ in range(4)]
-        capturing = self.capturing or torch.cuda.is_current_stream_capturing()
-        stage = self._ring[self._turn % len(self._ring)]
-        self._turn += 1
-        if stage[1] is not None and not capturing:
-            stage[1].synchronize()
+        capturing = self._capturing()
         if capturing:
             if self._spare is None or self._spare.shape[1] != n:
-                raise RuntimeError("take an eager step over the same parameters before each captured one")
+                raise RuntimeError(_EAGER_FIRST)
             stage, self._spare = [self._spare, None], None
-            self._captured.append((stage[0], ps))
+            # everything of the optimiser's own that the replays touch lives as long as the optimiser, whatever later eager
+            # steps put in its place: tables, chunk plan, momentum, and the memory that the weights had
+            self._captured.append((ps, bs, stage[0], self._plan, [p.detach() for p in ps]))
             for p in ps:                       # (its replays write p without moving p's version: nothing made from p is kept)
                 p._sln_captured = True
-        elif self._spare is None or self._spare.shape[1] != n:
-            self._spare = torch.empty((3, n), dtype=torch.int64, pin_memory=True)
+        else:
+            if not self._ring or self._ring[0][0].shape[1] != n:
+                self._ring = [[torch.empty((3, n), dtype=torch.int64, pin_memory=True), None] for _ in range(4)]
+            if self._spare is None or self._spare.shape[1] != n:
+                self._spare = torch.empty((3, n), dtype=torch.int64, pin_memory=True)
+            stage = self._ring[self._turn % len(self._ring)]
+            self._turn += 1
+            if stage[1] is not None:
+                stage[1].synchronize()
         host = [[t.data_ptr() for t in ts] for ts in (ps, gs, bs)]
         stage[0].numpy()[:] = host
         tab = torch.empty((3, n), dtype=torch.int64, device=dev)

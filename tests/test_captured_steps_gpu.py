@@ -118,3 +118,58 @@ def test_replayed_moves_the_versions_of_captured_weights_only():
     versions = [p._version for p in ps + [other]]
     opt.replayed()
     assert [p._version for p in ps + [other]] == [versions[0] + 1, versions[1] + 1, versions[2]]
+
+
+SHAPES = [(20, 30), (100, 130), (30,)]
+
+
+def _twins(kind):
+    (a, oa), (b, ob) = _make(kind, SHAPES), _make(kind, SHAPES)
+    first = _grads(a, 9)
+    for ps, opt in ((a, oa), (b, ob)):
+        _set(ps, [g.clone() for g in first])
+        opt.step(5.0)
+    return a, oa, b, ob
+
+
+def _same(a, oa, b, ob):
+    torch.cuda.synchronize()
+    return all(torch.equal(p, q) for p, q in zip(a, b)) and \
+        all(torch.equal(oa.state[p], ob.state[q]) for p, q in zip(a, b))
+
+
+def _churn():
+    """Takes over what the allocator got back: small blocks full of ones."""
+    return [torch.full((n,), -1, dtype=torch.int64, device="cuda") for n in (1, 2, 3, 4, 6, 8, 9, 16, 32, 64) for _ in range(20)]
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_what_a_captured_step_reads_outlives_eager_steps_of_another_set(kind):
+    """An eager step without one of the gradients, and one with another weight decay, make new plans: the graph keeps its own."""
+    a, oa, b, ob = _twins(kind)
+    static = _grads(a, 20)
+    _set(a, static)
+    graph = _capture(oa)
+    kept = [weakref.ref(t) for t in oa._plan] + [weakref.ref(t) for t in oa.state.values()]
+    for change in ("set", "decay"):
+        for ps, opt in ((a, oa), (b, ob)):
+            _set(ps, [g.clone() for g in _grads(ps, 30)])
+            if change == "set":
+                ps[0].grad = None
+            else:
+                opt.param_groups[-1]["weight_decay"] = 0.25
+            opt.step(5.0)
+            opt.param_groups[-1]["weight_decay"] = 1e-3 if kind == "ClippedSGD" else 0.0
+    gc.collect()
+    assert all(r() is not None for r in kept)                     # (from the host, before any replay)
+    assert _same(a, oa, b, ob)
+    ones = _churn()
+    for r in range(3):
+        new = _grads(a, 40 + r)
+        for g, v in zip(static, new):
+            g.copy_(v)
+        graph.replay()
+        _set(b, [v.clone() for v in new])
+        ob.step(5.0)
+        assert _same(a, oa, b, ob), r
+    assert all((t == -1).all() for t in ones)
