@@ -89,6 +89,7 @@ class ClippedSGD(object):
             if len(d["params"]) != len(g["params"]):
                 raise ValueError("loaded state dict contains a parameter group of a different size")
             g.update({key: v for key, v in d.items() if key != "params"})
+        held = self._held()
         self.state = {}
         self._skipped_loaded = int(sd.get("skipped_steps", 0))     # (added to the device counter's value)
         with torch.no_grad():
@@ -96,7 +97,11 @@ class ClippedSGD(object):
                 p = flat[int(i)]
                 b = st.get("momentum_buffer")
                 if b is not None:
-                    self.state[p] = torch.zeros_like(p, memory_format=torch.preserve_format).copy_(b)
+                    own = held.pop(id(p), (p, None))[1]            # (a captured step's is loaded in place: its replays go on from it)
+                    own = torch.zeros_like(p, memory_format=torch.preserve_format) if own is None else own
+                    self.state[p] = own.copy_(b)
+            for p, own in held.values():
+                self.state[p] = own.zero_()
 
     def zero_grad(self, set_to_none=True):
         for g in self.param_groups:
@@ -113,6 +118,10 @@ class ClippedSGD(object):
         ps = list({id(p): p for c in self._captured for p in c[0]}.values())
         if ps:
             torch._C._autograd._unsafe_set_version_counter(ps, [p._version + 1 for p in ps])
+
+    def _held(self):
+        """id(weight) -> (weight, momentum buffer) of captured steps."""
+        return {id(p): (p, b) for c in self._captured for p, b in zip(c[0], c[1])}
 
     def _active(self):
         out = []
@@ -181,6 +190,7 @@ class ClippedSGD(object):
     def _buffers(self, act):
         """Parameters, gradients (element i of the gradient is element i of the weight) and momentum buffers."""
         ps, gs, bs = [], [], []
+        capturing, held = self._capturing(), self._held()
         for p, _ in act:
             g = p.grad
             if p.dtype != torch.float32 or g.dtype != torch.float32:
@@ -191,8 +201,12 @@ class ClippedSGD(object):
                 g = torch.empty_like(p).copy_(g)
             b = self.state.get(p)
             if b is None:
+                if capturing:                  # (its clearing would be part of every replay)
+                    raise RuntimeError(_EAGER_FIRST)
                 b = self.state[p] = torch.zeros_like(p, memory_format=torch.preserve_format)
             elif b.stride() != p.stride():     # (and of the momentum: the weight may have changed its memory format)
+                if capturing or id(p) in held:
+                    raise RuntimeError("a weight of a captured step cannot change its memory format")
                 b = self.state[p] = torch.empty_like(p).copy_(b)
             ps.append(p); gs.append(g); bs.append(b)
         return ps, gs, bs

@@ -173,3 +173,65 @@ def test_what_a_captured_step_reads_outlives_eager_steps_of_another_set(kind):
         ob.step(5.0)
         assert _same(a, oa, b, ob), r
     assert all((t == -1).all() for t in ones)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_loaded_momentum_reaches_a_captured_step(kind):
+    a, oa, b, ob = _twins(kind)
+    static = _grads(a, 20)
+    _set(a, static)
+    graph = _capture(oa)
+    addresses = [oa.state[p].data_ptr() for p in a]
+    saved = [p.detach().clone() for p in a]
+    sd = oa.state_dict()
+    sd["state"] = {i: {"momentum_buffer": s["momentum_buffer"].clone()} for i, s in sd["state"].items()}
+    for without in (None, 2):                                     # the whole state; one without a buffer: zeros
+        if without is not None:
+            sd["state"].pop(without)
+        graph.replay()
+        for ps, opt in ((a, oa), (b, ob)):
+            with torch.no_grad():
+                for p, v in zip(ps, saved):
+                    p.copy_(v)
+            opt.load_state_dict(sd)
+        if without is not None:
+            ob.state[b[without]] = torch.zeros_like(b[without])
+        assert [oa.state[p].data_ptr() for p in a] == addresses and _same(a, oa, b, ob)
+        new = _grads(a, 50)
+        for g, v in zip(static, new):
+            g.copy_(v)
+        graph.replay()
+        _set(b, [v.clone() for v in new])
+        ob.step(5.0)
+        assert _same(a, oa, b, ob)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_captures_that_would_take_memory_of_the_capture_are_refused(kind):
+    ps, opt = _make(kind, [(6, 5, 3, 3), (20, 30), (20, 30)])
+    _set(ps, _grads(ps, 3))
+    before = [p.detach().clone() for p in ps]
+
+    def refused():
+        opt.capturing = True                                      # (what a capture sets; nothing is being captured here)
+        with pytest.raises(RuntimeError):
+            opt.step(5.0)
+        opt.capturing = False
+
+    refused()                                                     # no eager step yet
+    ps[2].grad = None
+    opt.step(5.0)
+    before = [p.detach().clone() for p in ps]
+    _set(ps, _grads(ps, 4))
+    ps[1].grad = None
+    refused()                                                     # as many weights of the same sizes, but not the same ones
+    _set(ps, _grads(ps, 4))
+    refused()                                                     # more of them
+    assert all(torch.equal(p, q) for p, q in zip(ps, before))
+    opt.step(5.0)
+    graph = _capture(opt)
+    ps[0].data = ps[0].data.contiguous(memory_format=torch.channels_last)
+    _set(ps, _grads(ps, 5))
+    with pytest.raises(RuntimeError):                             # the graph writes this weight's momentum
+        opt.step(5.0)
+    del graph
