@@ -168,8 +168,6 @@ class ClippedSGD(object):
         ct, co, numel, partial, wd = self._chunks([p.numel() for p in ps], [w for _, w in act], dev)
         tab = self._upload(ps, gs, bs, dev)[1]
         sq = torch.empty(1, dtype=torch.float64, device=dev)
-        if self.skipped is None:
-            self.skipped = torch.zeros(1, dtype=torch.int32, device=dev)
         lr, momentum = self._hyper()
         st = C.c_void_p(torch.cuda.current_stream().cuda_stream)
         L = _lib.lib()
@@ -191,6 +189,10 @@ class ClippedSGD(object):
         """Parameters, gradients (element i of the gradient is element i of the weight) and momentum buffers."""
         ps, gs, bs = [], [], []
         capturing, held = self._capturing(), self._held()
+        if self.skipped is None:
+            if capturing:
+                raise RuntimeError(_EAGER_FIRST)
+            self.skipped, self.skipped_clamped = (torch.zeros(1, dtype=torch.int32, device=act[0][0].device) for _ in range(2))
         for p, _ in act:
             g = p.grad
             if p.dtype != torch.float32 or g.dtype != torch.float32:
@@ -228,7 +230,7 @@ class ClippedSGD(object):
             stage, self._spare = [self._spare, None], None
             # everything of the optimiser's own that the replays touch lives as long as the optimiser, whatever later eager
             # steps put in its place: tables, chunk plan, momentum, and the memory that the weights had
-            self._captured.append((ps, bs, stage[0], self._plan, [p.detach() for p in ps]))
+            self._captured.append((ps, bs, stage[0], self._plan, [p.detach() for p in ps], self.skipped, self.skipped_clamped))
             for p in ps:                       # (its replays write p without moving p's version: nothing made from p is kept)
                 p._sln_captured = True
         else:
@@ -253,8 +255,6 @@ class ClippedSGD(object):
         """The guard's input: +inf instead of the squared norm when the step is vetoed (two 5-us elementwise ops)."""
         if veto is None:
             return sq
-        if self.skipped_clamped is None:
-            self.skipped_clamped = torch.zeros(1, dtype=torch.int32, device=sq.device)
         hit = veto.reshape(1) > 0
         # (a step that is non-finite anyway is counted as that, not as clamped)
         self.skipped_clamped += (hit & torch.isfinite(sq)).to(torch.int32)
@@ -352,8 +352,6 @@ class ClippedMuon(ClippedSGD):
             row = 8 * len(ps)
             at = tab.data_ptr()
             sq = torch.empty(1, dtype=torch.float64, device=dev)
-            if self.skipped is None:
-                self.skipped = torch.zeros(1, dtype=torch.int32, device=dev)
             st = _lib.stream_of(dev)
             L = _lib.lib()
             # (the workspace before the first launch: nothing is written if there is no memory for it)

@@ -235,3 +235,20 @@ def test_captures_that_would_take_memory_of_the_capture_are_refused(kind):
     with pytest.raises(RuntimeError):                             # the graph writes this weight's momentum
         opt.step(5.0)
     del graph
+
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_replays_count_their_vetoes(kind):
+    """The first veto of all comes inside of the capture: its counter was there before."""
+    a, oa, _, _ = _twins(kind)
+    _set(a, _grads(a, 20))
+    veto = torch.zeros(1, device="cuda")
+    graph = _capture(oa, veto=veto)
+    for hit in (1, 0, 1, 1):
+        veto.fill_(hit)
+        before = [p.detach().clone() for p in a]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(a, before)) == bool(hit)
+    assert oa.skipped_clamped_steps() == 3 and oa.skipped_steps() == 3
