@@ -9,7 +9,8 @@ import torch
 from . import _lib
 
 CHUNK = 1 << 16
-_EAGER_FIRST = "take an eager step over the same parameters before each captured one"
+CAPTURES = 16          # steps that can be captured after an eager one (their tables cannot be made inside of a capture)
+_EAGER_FIRST = "take an eager step over the same parameters before captured ones (at least %d may follow it)" % (CAPTURES // 2)
 
 
 class ClippedSGD(object):
@@ -31,7 +32,7 @@ class ClippedSGD(object):
         self.skipped_clamped = None          # device int32: of those, the steps vetoed for clamped operand blocks
         self._plan_key, self._plan = None, None
         self._ring, self._turn = [], 0       # pinned staging buffers of the pointer tables
-        self._spare, self._captured = None, []        # the next captured step's table; what captured steps read and write
+        self._spares, self._captured = [], []         # tables for captured steps; what those read and write
         self.capturing = False               # inside a HIP-graph capture: no event waits (the tables are static)
         self.last_norm = None
 
@@ -156,7 +157,7 @@ class ClippedSGD(object):
         as a non-finite gradient norm and counted in `skipped` and `skipped_clamped`; `last_norm` stays the real
         norm.  No host sync either way.
 
-        A step may be captured into a graph, with an eager step over the same parameters before it.  Its replays use the
+        Steps may be captured into graphs, after an eager step over the same parameters (eight or more in a row).  Replays use the
         hyper-parameters of the capture and the gradient tensors that were there: keep those, and call replayed()."""
         act = self._active()
         if not act:
@@ -225,9 +226,11 @@ class ClippedSGD(object):
         n = len(ps)
         capturing = self._capturing()
         if capturing:
-            if self._spare is None or self._spare.shape[1] != n:
+            if not torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("`capturing` is set, but nothing is being captured on this stream")
+            if not self._spares or self._spares[0].shape[1] != n:
                 raise RuntimeError(_EAGER_FIRST)
-            stage, self._spare = [self._spare, None], None
+            stage = [self._spares.pop(), None]
             # everything of the optimiser's own that the replays touch lives as long as the optimiser, whatever later eager
             # steps put in its place: tables, chunk plan, momentum, and the memory that the weights had
             self._captured.append((ps, bs, stage[0], self._plan, [p.detach() for p in ps], self.skipped, self.skipped_clamped))
@@ -236,8 +239,8 @@ class ClippedSGD(object):
         else:
             if not self._ring or self._ring[0][0].shape[1] != n:
                 self._ring = [[torch.empty((3, n), dtype=torch.int64, pin_memory=True), None] for _ in range(4)]
-            if self._spare is None or self._spare.shape[1] != n:
-                self._spare = torch.empty((3, n), dtype=torch.int64, pin_memory=True)
+            if len(self._spares) < CAPTURES // 2 or self._spares[0].shape[1] != n:
+                self._spares = list(torch.empty((CAPTURES, 3, n), dtype=torch.int64, pin_memory=True))
             stage = self._ring[self._turn % len(self._ring)]
             self._turn += 1
             if stage[1] is not None:

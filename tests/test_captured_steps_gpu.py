@@ -214,7 +214,7 @@ def test_captures_that_would_take_memory_of_the_capture_are_refused(kind):
 
     def refused():
         opt.capturing = True                                      # (what a capture sets; nothing is being captured here)
-        with pytest.raises(RuntimeError):
+        with pytest.raises(RuntimeError, match="eager step"):
             opt.step(5.0)
         opt.capturing = False
 
@@ -232,7 +232,7 @@ def test_captures_that_would_take_memory_of_the_capture_are_refused(kind):
     graph = _capture(opt)
     ps[0].data = ps[0].data.contiguous(memory_format=torch.channels_last)
     _set(ps, _grads(ps, 5))
-    with pytest.raises(RuntimeError):                             # the graph writes this weight's momentum
+    with pytest.raises(RuntimeError, match="memory format"):      # the graph writes this weight's momentum
         opt.step(5.0)
     del graph
 
@@ -252,3 +252,26 @@ def test_replays_count_their_vetoes(kind):
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(a, before)) == bool(hit)
     assert oa.skipped_clamped_steps() == 3 and oa.skipped_steps() == 3
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_captures_in_a_row(kind):
+    """Several steps captured after one eager step, each with gradients of its own, replayed out of order."""
+    a, oa, b, ob = _twins(kind)
+    statics, graphs = [], []
+    for i in range(8):
+        statics.append(_grads(a, 20 + i))
+        _set(a, statics[-1])
+        graphs.append(_capture(oa))
+    for r, i in enumerate((3, 0, 7, 3, 5, 1)):
+        new = _grads(a, 60 + r)
+        for g, v in zip(statics[i], new):
+            g.copy_(v)
+        graphs[i].replay()
+        _set(b, [v.clone() for v in new])
+        ob.step(5.0)
+        assert _same(a, oa, b, ob), (r, i)
+    _set(a, _grads(a, 90))
+    oa.capturing = True
+    with pytest.raises(RuntimeError, match="nothing is being captured"):
+        oa.step(5.0)
