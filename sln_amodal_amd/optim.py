@@ -279,8 +279,9 @@ class ClippedMuon(ClippedSGD):
         p <- p (1 - lr weight_decay) - lr sqrt(max(1, rows / cols)) orthogonalize(u, steps, eps)
 
     Orthogonal groups have an lr, momentum, weight_decay of their own (one momentum for all of them); the other groups
-    agree on one lr and momentum, like ClippedSGD's.  The same guard: a step with a non-finite gradient norm or a veto
-    writes nothing and is counted.  Hyper-parameters are read when step() is called; a captured step keeps them."""
+    agree on one lr and momentum, like ClippedSGD's; setting `lr` sets theirs and scales the orthogonal ones'.  The same
+    guard: a step with a non-finite gradient norm or a veto writes nothing and is counted.  Hyper-parameters are read when
+    step() is called; a captured step keeps them."""
 
     def __init__(self, param_groups, lr, momentum=0.95, nesterov=True, steps=5, eps=1e-7):
         super(ClippedMuon, self).__init__(param_groups, lr, momentum)
@@ -313,6 +314,26 @@ class ClippedMuon(ClippedSGD):
             raise ValueError("ClippedMuon applies one lr / momentum to its non-orthogonal groups (got lr %s, "
                              "momentum %s)" % (sorted(lrs), sorted(moms)))
         return (min(lrs) if lrs else 0.0), (min(moms) if moms else 0.0)
+
+    @property
+    def lr(self):
+        return self._hyper()[0]
+
+    @lr.setter
+    def lr(self, value):
+        """The rate that the getter reads; the orthogonal groups' rates keep their ratio to it.  (Where it is zero, the ratio
+        that they had when it was set to that.)"""
+        rest, ortho = self._split()
+        live = [float(g["lr"]) for g in (rest if any(g["params"] for g in rest) else ortho) if g["params"]]
+        value, old = float(value), min(live, default=0.0)
+        ratios = [g["lr"] / old if old else g.get("lr_ratio") for g in ortho]
+        if None in ratios:
+            raise ValueError("lr is 0: the ratio of the orthogonal groups' rates to it is not known, set them in param_groups")
+        for g in rest:
+            g["lr"] = value
+        for g, ratio in zip(ortho, ratios):
+            g["lr"] = value if ratio == 1.0 else value * ratio
+            g["lr_ratio"] = ratio
 
     def load_state_dict(self, sd):
         if len(sd["param_groups"]) == len(self.param_groups):
