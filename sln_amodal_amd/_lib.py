@@ -156,6 +156,15 @@ class on_device(object):
             self.guard.__exit__(*exc)
 
 
+def need_no_tangent(what, *tensors):
+    """Refuses dual tensors of forward-mode differentiation: a kernel reads the values and would drop the tangent."""
+    import torch.autograd.forward_ad as fw
+    if getattr(fw, "_current_level", 0) >= 0:
+        for t in tensors:
+            if t is not None and fw.unpack_dual(t).tangent is not None:
+                raise RuntimeError("%s has no forward-mode derivative" % what)
+
+
 def stream_of(dev):
     """torch's current stream on `dev` as the C entries take it."""
     import torch

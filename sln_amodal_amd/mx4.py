@@ -184,8 +184,8 @@ def mx4_linear(x, weight, bias=None, scale=None, relu=False):
 
     weight: an Mx4Tensor (rounded once and kept: serving; it gets no gradient) or a float32 [N, K] tensor that is rounded
     in every call (training).  bias, scale: float32 [N] or None; scale (a frozen normalisation's) gets no gradient.
-    Backward (straight through the rounding): x, a float32 weight and bias.  Up to 16 rows take one pass over the weight
-    without a separate rounding of x.  Deterministic."""
+    Backward (straight through the rounding): x, a float32 weight and bias; no second derivative, no forward mode.  Up to 16
+    rows take one pass over the weight without a separate rounding of x.  Deterministic."""
     _need_float(x, "x")
     wq = weight if isinstance(weight, Mx4Tensor) else None
     if wq is None:
@@ -207,6 +207,7 @@ def mx4_linear(x, weight, bias=None, scale=None, relu=False):
             raise ValueError("%s must be [%d], got %s" % (name, N, tuple(t.shape)))
         if t.device != dev:
             raise ValueError("%s is on %s, x on %s" % (name, t.device, dev))
+    _lib.need_no_tangent("mx4_linear", x, weight if wq is None else None, bias, scale)
     grad = torch.is_grad_enabled()
     if scale is not None:
         if grad and scale.requires_grad:

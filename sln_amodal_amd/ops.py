@@ -411,6 +411,7 @@ def orthogonalize(x, steps=5, eps=1e-7):
             raise ValueError("the matrices of one call share a type and a device")
         if grad and t.requires_grad:
             raise RuntimeError("orthogonalize has no gradient: detach x or call it under torch.no_grad()")
+        _lib.need_no_tangent("orthogonalize", t)
         r, c = shape[-2], shape[-1]
         if min(r, c) > 65535 or max(r, c) > 1 << 22:
             raise ValueError("orthogonalize: at most 65535 x 2^22, got %s" % (tuple(shape),))
