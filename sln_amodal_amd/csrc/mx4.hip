@@ -118,9 +118,13 @@ struct MxGemm {
     int relu;
 };
 
-// One rounding for scale, one for bias (no fused multiply-add), so that every kernel of this file ends alike.
+// One rounding for scale, one for bias, one to the type, so that every kernel of this file, with and without ReLU, ends
+// alike.  (The file is built with contraction on: without the pragma these are fused multiply-adds, in float16 without a
+// rounding between the sum and the type.)
 __device__ __forceinline__ float mx_act(float v, float scale, float bias, int relu) {
-    v = __fadd_rn(__fmul_rn(v, scale), bias);
+#pragma clang fp contract(off)
+    v = v * scale;
+    v = v + bias;
     return relu && v < 0.f ? 0.f : v;              // (a NaN stays)
 }
 template <typename T>
