@@ -107,15 +107,18 @@ static int64_t ortho_operand_bytes(const OrthoProb &p, bool pairs) {
 __device__ __forceinline__ float ortho_shift(int shift, int step, int sign) {
     return ldexpf(1.f, sign * max(0, shift - 2 * step));
 }
-// 1 / (norm + eps) and h
-__device__ __forceinline__ float ortho_inverse(double sum, float eps, int &shift) {
+// h, and X = G up inv = G 2^h / (norm + eps), |G| up <= norm + eps.  (From 2^126 on 1 / (norm + eps) is no normal float32
+// number and would hold too few bits: 2^64 of it goes into up.)
+__device__ __forceinline__ float ortho_inverse(double sum, float eps, int &shift, float &up) {
     const double norm = sqrt(sum), r = norm / (norm + (double)eps);
     shift = 0;
     if (r > 0.0 && r < 1.0) {
         frexp(r, &shift);                          // r < 2^shift
         shift = min(max(-shift, 0), 126);
     }
-    return (float)(1.0 / (norm + (double)eps));
+    const int down = norm + (double)eps > 0x1p100 ? 64 : 0;
+    up = ldexpf(1.f, shift - down);
+    return (float)(ldexp(1.0, down) / (norm + (double)eps));
 }
 
 template <typename T>
@@ -288,9 +291,9 @@ __global__ __launch_bounds__(256) void ortho_split_kernel(OrthoTable tab, OrthoR
     double acc = 0.0;
     for (int i = t; i < p.nparts; i += 256) acc += tab.part[p.part0 + i];
     int shift;
-    const float inv = ortho_inverse(ortho_block_sum(acc, s_red), eps, shift);
+    float up;
+    const float inv = ortho_inverse(ortho_block_sum(acc, s_red), eps, shift, up);
     if (w.ij == 0 && t == 0) tab.prob[w.prob].shift = shift;
-    const float up = ldexpf(1.f, shift);           // |g| up <= norm + eps
     float cf = 1.f;
     if (p.buf) ortho_clip(rule, cf);
     const bool tall = p.rows > p.cols;
@@ -785,8 +788,8 @@ __global__ __launch_bounds__(512) void ortho_small_kernel(OrthoBatch batch, Orth
 #pragma unroll
         for (int q = 0; q < 8; ++q) sum += (double)u[s][q] * u[s][q];
     int shift;
-    const float inv = ortho_inverse(ortho_block_sum(sum, (double *)ls), eps, shift);
-    const float up = ldexpf(1.f, shift);
+    float up;
+    const float inv = ortho_inverse(ortho_block_sum(sum, (double *)ls), eps, shift, up);
     // ---- X
     each([&](int s, int i, int k8) {
         if (t + 512 * s >= MP * groups * 4) return;
