@@ -1,10 +1,11 @@
 // Newton-Schulz orthogonalisation of many matrices at once, and the optimiser step built on it (gfx950).
 //
 //   X <- G / (|G|_F + eps), on the transpose where G is taller than wide (so X is m x n, m <= n)
-//   `steps` times:  A = X X^T,  P = a I + b A + c A^2,  X <- P X        (a, b, c) = (3.4445, -4.7750, 2.0315)
+//   `steps` times:  A = X X^T,  P = a I + b A + c A^2,  X <- P X        (a, b, c) = (3.4445, -4.7750, 2.0315), the
+//   coefficients published with the Muon optimiser
 //
 // maps every singular value s of X to p(s) = a s + b s^3 + c s^5, again and again: in five steps all of (0.005, 1] come
-// into 0.68 ... 1.14, so X ends near the orthogonal factor U V^T of G.  p keeps [0, 1.21] inside [0, 1.21], hence
+// into 0.68 ... 1.16, so X ends near the orthogonal factor U V^T of G.  p keeps [0, 1.21] inside [0, 1.21], hence
 // |X|_2 <= 1.21, |A|_2 <= 1.47, |P|_2 <= 3.45 throughout and a FIXED power-of-two scale (2^14) puts every operand into
 // fp16's range: an operand is two fp16 parts of value * 2^14 (22 ... 23 bits for values above 2^-17, an absolute floor of
 // 2^-39 below), a product of two is three matrix instructions into an fp32 accumulator.  No pass looks for a maximum.
