@@ -601,8 +601,8 @@ int sln_mx4_linear_fwd(const void *x, int dtype, int64_t M, int64_t K, int64_t s
                        const float *scale, const float *bias, int relu, void *y, void *workspace, size_t workspace_bytes,
                        sln_stream_t stream);
 /* Straight-through gradients of y = act((x^ w^T) * scale + bias): gy [M][N] in dtype (row stride gy_stride), y [M][N] in
- * dtype: the output, gy counts where it is > 0 (NULL: everywhere); gx [M][K] in dtype, gw [N][K] f32, gb [N] f32, each
- * NULL if not wanted.  Workspace (256-byte boundary): sln_mx4_linear_bwd_workspace_bytes.  Bit-reproducible. */
+ * dtype: the output, gy counts where it is > 0, not where it is a NaN (NULL: everywhere); gx [M][K] in dtype, gw [N][K]
+ * f32, gb [N] f32, each NULL if not wanted.  Workspace (256-byte boundary): sln_mx4_linear_bwd_workspace_bytes.  Bit-reproducible. */
 size_t sln_mx4_linear_bwd_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype, int want_gx, int want_gw,
                                           int want_gb);
 int sln_mx4_linear_bwd(const void *gy, int dtype, int64_t gy_stride, const void *y, const float *scale,

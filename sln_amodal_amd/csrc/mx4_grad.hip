@@ -2,6 +2,8 @@
 //
 //   z = gy [y > 0],   gx = (z scale) w^,   gw = scale (z^T x^),   gb = sum over the rows of z
 //
+// (z is 0 where y is a NaN, as under the convolutions' masks; x^ or w^ holds that NaN, so gw or gx does not hide it.)
+//
 // The rounding passes its gradient through unchanged, saturated values included.  w^ and x^ are what the forward
 // multiplied: e2m1 values times powers of two have two significant bits, so ONE bf16 part holds them exactly, and a
 // float32 gradient is exactly the sum of three bf16 parts (8 bits of its significand each, cut, not rounded).

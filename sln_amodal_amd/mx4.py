@@ -184,8 +184,9 @@ def mx4_linear(x, weight, bias=None, scale=None, relu=False):
 
     weight: an Mx4Tensor (rounded once and kept: serving; it gets no gradient) or a float32 [N, K] tensor that is rounded
     in every call (training).  bias, scale: float32 [N] or None; scale (a frozen normalisation's) gets no gradient.
-    Backward (straight through the rounding): x, a float32 weight and bias; no second derivative, no forward mode.  Up to 16
-    rows take one pass over the weight without a separate rounding of x.  Deterministic."""
+    Backward (straight through the rounding): x, a float32 weight and bias; no second derivative, no forward mode; a ReLU lets
+    the gradient through where the output is > 0, not where it is a NaN, like the framework's convolutions.  Up to 16 rows take
+    one pass over the weight without a separate rounding of x.  Deterministic."""
     _need_float(x, "x")
     wq = weight if isinstance(weight, Mx4Tensor) else None
     if wq is None:

@@ -52,3 +52,20 @@ def test_scaled_16_bit_gradients_are_as_near_as_float32_ones(dtype):
     slack = (3 * N + 3) * 2.0 ** -23 * (zs.abs() @ wv.abs())
     lo, hi = (want - slack).to(dtype), (want + slack).to(dtype)
     assert ((gx == lo) | (gx == hi) | ((gx > lo) & (gx < hi))).all()
+
+
+@pytest.mark.parametrize("rows", [12, 40])
+def test_relu_stops_the_gradient_where_the_output_is_nan(rows):
+    """y > 0 is false for a NaN, as in the framework's convolutions (torch's relu lets the gradient through there): the bias
+    counts the other rows only.  The NaN is not hidden: the weight's gradient meets it in x."""
+    from sln_amodal_amd import ops
+    g = torch.Generator().manual_seed(rows)
+    x, w, b = torch.rand(rows, 64, generator=g), torch.rand(20, 64, generator=g), torch.zeros(20)
+    x[3, 7] = float("nan")
+    xd, wd, bd = (t.cuda().requires_grad_() for t in (x, w, b))
+    y = ops.mx4_linear(xd, wd, bd, relu=True)
+    assert torch.isnan(y[3]).all() and (y[:3] > 0).all() and (y[4:] > 0).all()
+    gx, gw, gb = torch.autograd.grad(y, (xd, wd, bd), torch.ones_like(y))
+    assert torch.equal(gb.cpu(), torch.full((20,), float(rows - 1)))
+    assert not gx[3].any() and torch.isfinite(gx).all()
+    assert torch.isnan(gw[:, :32]).all() and torch.isfinite(gw[:, 32:]).all()
