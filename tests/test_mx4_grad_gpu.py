@@ -54,6 +54,42 @@ def test_scaled_16_bit_gradients_are_as_near_as_float32_ones(dtype):
     assert ((gx == lo) | (gx == hi) | ((gx > lo) & (gx < hi))).all()
 
 
+def _large(rows, cols):
+    """csrc/mx4_grad.hip (mg_large): 128 x 256 tiles from 384 of them on."""
+    return (-(-rows // 128)) * (-(-cols // 256)) >= 384
+
+
+@pytest.mark.parametrize("M,N,K,gx_large,gw_large", [(130, 1025, 11010, False, True), (1100, 1030, 10900, True, True),
+                                                     (1100, 130, 10900, True, False)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gradients_on_the_large_tiles(M, N, K, gx_large, gw_large, dtype):
+    from sln_amodal_amd import ops
+    assert (_large(M, K), _large(N, K)) == (gx_large, gw_large)
+    g = torch.Generator().manual_seed(M + N)
+    x = (torch.randn(M, K, generator=g) * torch.exp(torch.randn(K, generator=g))).to(dtype)
+    w = torch.randn(N, K, generator=g) / K ** 0.5
+    scale, bias = torch.exp(0.3 * torch.randn(N, generator=g)), 0.1 * torch.randn(N, generator=g)
+    gy = (torch.randn(M, N, generator=g) * torch.exp(torch.randn(M, 1, generator=g))).to(dtype)
+    xd, wd, bd = x.cuda().requires_grad_(), w.cuda().requires_grad_(), bias.cuda().requires_grad_()
+    y = ops.mx4_linear(xd, wd, bd, scale=scale.cuda(), relu=True)
+    gx, gw, gb = torch.autograd.grad(y, (xd, wd, bd), gy.cuda())
+    # (the reference's products in 64 bits on the device: plain matrices, no batches)
+    xv, wv, s = ref.values(x).cuda(), ref.values(w).cuda(), scale.double().cuda()
+    z = torch.where(y.detach() > 0, gy.cuda().double(), torch.zeros((), dtype=torch.float64, device="cuda"))
+    zs = z * s
+    want_x, mag_x = zs @ wv, zs.abs() @ wv.abs()
+    zt = zs.t().contiguous()
+    want_w, mag_w = zt @ xv, zt.abs() @ xv.abs()
+    bx = ((3 * N + 2) * 2.0 ** -23 + 2.0 ** -24) * mag_x + torch.finfo(dtype).eps / 2 * (1 + 2.0 ** -6) * want_x.abs() + 2.0 ** -25
+    assert ((gx.double() - want_x).abs() <= bx).all()
+    assert ((gw.double() - want_w).abs() <= (3 * M + 3) * 2.0 ** -23 * mag_w + 1e-30).all()
+    assert ((gb.double() - z.sum(0)).abs() <= (M + 2) * 2.0 ** -23 * z.abs().sum(0) + 1e-30).all()
+    for i, want in enumerate((gx, gw, gb)):                        # one at a time: the same bits
+        args = [t if j == i else t.detach() for j, t in enumerate((xd, wd, bd))]
+        y1 = ops.mx4_linear(args[0], args[1], args[2], scale=scale.cuda(), relu=True)
+        assert torch.equal(y1, y) and torch.equal(torch.autograd.grad(y1, (xd, wd, bd)[i], gy.cuda())[0], want)
+
+
 @pytest.mark.parametrize("rows", [12, 40])
 def test_relu_stops_the_gradient_where_the_output_is_nan(rows):
     """y > 0 is false for a NaN, as in the framework's convolutions (torch's relu lets the gradient through there): the bias
