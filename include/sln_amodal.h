@@ -583,7 +583,8 @@ int sln_mx4_round(const void *x, int dtype, int64_t R, int64_t K, int64_t stride
 int sln_mx4_values(const uint8_t *codes, const uint8_t *scales, int64_t R, int64_t K, void *out, int dtype,
                    sln_stream_t stream);
 /* y [M][N] = act((a b^T) * scale[n] + bias[n]), a [M][K] and b [N][K] rounded; scale / bias f32 [N] or NULL; relu: act =
- * max(0, .) (a NaN stays).  Workspace: sln_mx4_product_workspace_bytes(M, N, K, 1) (0: none needed).  Bit-reproducible. */
+ * max(0, .) (a NaN stays).  M, N <= 2^28.  Workspace: sln_mx4_product_workspace_bytes(M, N, K, 1) (0: none needed).
+ * Bit-reproducible. */
 size_t sln_mx4_product_workspace_bytes(int64_t M, int64_t N, int64_t K, int rounded);
 int sln_mx4_product(const uint8_t *a_codes, const uint8_t *a_scales, const uint8_t *b_codes, const uint8_t *b_scales,
                     int64_t M, int64_t N, int64_t K, const float *scale, const float *bias, int relu, void *y, int dtype,
@@ -602,7 +603,8 @@ int sln_mx4_linear_fwd(const void *x, int dtype, int64_t M, int64_t K, int64_t s
                        sln_stream_t stream);
 /* Straight-through gradients of y = act((x^ w^T) * scale + bias): gy [M][N] in dtype (row stride gy_stride), y [M][N] in
  * dtype: the output, gy counts where it is > 0, not where it is a NaN (NULL: everywhere); gx [M][K] in dtype, gw [N][K]
- * f32, gb [N] f32, each NULL if not wanted.  Workspace (256-byte boundary): sln_mx4_linear_bwd_workspace_bytes.  Bit-reproducible. */
+ * f32, gb [N] f32, each NULL if not wanted.  M, N <= 2^21.  Workspace (256-byte boundary):
+ * sln_mx4_linear_bwd_workspace_bytes.  Bit-reproducible. */
 size_t sln_mx4_linear_bwd_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype, int want_gx, int want_gw,
                                           int want_gb);
 int sln_mx4_linear_bwd(const void *gy, int dtype, int64_t gy_stride, const void *y, const float *scale,

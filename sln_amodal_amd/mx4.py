@@ -12,6 +12,7 @@ from . import _lib
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 FEW_ROWS = 16          # rows that sln_mx4_rows_product takes: rounded inside the product, no launch in front of it
 MAX_K = 1 << 22
+MAX_GRAD = 1 << 21     # rows and outputs that sln_mx4_linear_bwd takes
 
 
 def _need_float(t, name):
@@ -217,6 +218,9 @@ def mx4_linear(x, weight, bias=None, scale=None, relu=False):
     if bias is not None and not bias.is_contiguous():
         bias = bias.contiguous()
     if grad and (x.requires_grad or (wq is None and weight.requires_grad) or (bias is not None and bias.requires_grad)):
+        if max(x.numel() // wshape[1], N) > MAX_GRAD:
+            raise ValueError("mx4_linear: at most 2^21 rows and outputs with gradients, got %s for a weight %s" %
+                             (tuple(x.shape), tuple(wshape)))
         return _Mx4LinearFn.apply(x, None if wq is not None else weight, bias, scale, bool(relu), wq)
     y = _forward(x, weight, wq, bias, scale, bool(relu), False)[0]
     return y if x.dim() == 2 else y.view(x.shape[:-1] + (N,))

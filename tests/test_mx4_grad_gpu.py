@@ -105,3 +105,17 @@ def test_relu_stops_the_gradient_where_the_output_is_nan(rows):
     assert torch.equal(gb.cpu(), torch.full((20,), float(rows - 1)))
     assert not gx[3].any() and torch.isfinite(gx).all()
     assert torch.isnan(gw[:, :32]).all() and torch.isfinite(gw[:, 32:]).all()
+
+
+def test_more_rows_than_the_gradients_take_are_refused_before_the_forward():
+    from sln_amodal_amd import ops
+    w = torch.ones(3, 32, device="cuda")
+    x = torch.ones(1, 32, device="cuda").expand((1 << 21) + 1, 32)
+    assert torch.equal(ops.mx4_linear(x, w)[-1], torch.full((3,), 32.0, device="cuda"))
+    with pytest.raises(ValueError):
+        ops.mx4_linear(x, w.requires_grad_())
+    with pytest.raises(ValueError):
+        ops.mx4_linear(torch.ones(2, 1, device="cuda", requires_grad=True), torch.ones(1, 1, device="cuda").expand((1 << 21) + 1, 1))
+    x = x[:-1]
+    gx, gw = torch.autograd.grad(ops.mx4_linear(x.requires_grad_(), w).sum(), (x, w))
+    assert (gx == 3).all() and (gw == 2.0 ** 21).all()
