@@ -2,7 +2,7 @@
 //
 //   z = gy [y > 0],   gx = (z scale) w^,   gw = scale (z^T x^),   gb = sum over the rows of z
 //
-// (z is 0 where y is a NaN, as under the convolutions' masks; x^ or w^ holds that NaN, so gw or gx does not hide it.)
+// (z is 0 where y is a NaN, as under the convolutions' masks; a NaN of x^ or w^ still reaches gw or gx.)
 //
 // The rounding passes its gradient through unchanged, saturated values included.  w^ and x^ are what the forward
 // multiplied: e2m1 values times powers of two have two significant bits, so ONE bf16 part holds them exactly, and a
@@ -11,7 +11,8 @@
 // nothing is rounded before the sum but z * scale, to float32.  (Parts below bf16's smallest normal, 2^-126, may be lost.)
 // Three parts for float32 gradients and for z * scale of any type, two where a 16-bit z is taken as it is.  (z * scale cut
 // to two parts, 16 bits, costs the sums of gx up to 2^-15 of their terms, all in one direction: of 1501 x 1024 bfloat16
-// results over 324 outputs 0.6 % were not the nearest; with three parts 0.014 %, a float32 product's 0.023 %.)
+// results over 324 outputs 0.6 % were not the nearest; with three parts 0.014 %, a float32 product's 0.023 %.  The third part
+// takes 1600 x 12544 x 1024 in bfloat16, forward and both gradients in a graph, from 229 us to 269; without scale 224.)
 //
 // Both products contract along rows (mfma_nt.h): gx over the outputs, so w^ is laid out [K][N]; gw over the rows of the
 // batch, so z is laid out [N][M] and x^ [K][M].
@@ -154,7 +155,8 @@ __global__ __launch_bounds__(256) void mx4_grad_prep_kernel(const MgPrep p) {
 // loads and stores (1600 x 12544 x 1024, three parts, both gradients: 230 us; 128 x 128 tiles of four waves 285, 256 x 256
 // tiles, one workgroup per CU, 281, though their k-loop alone is the fastest): 247 GFLOP of products, 1.07 PFLOP/s of the
 // 1.30 that the library's bf16 product reaches.
-// (Small ones: eight waves too; 1501 x 1024 x 324 bf16, both directions: 49 us, with four 52.)
+// (Small ones: eight waves too; 1501 x 1024 x 324 bf16, both directions: 49 us without scale, with it, three parts, 52; two
+// parts with four waves took 52.)
 template <int P> struct MgSmall : NtShape<P, 1, 128, 128, 2, 4, 2> {};
 template <int P> struct MgLarge : NtShape<P, 1, 128, 256, 2, 4, 2> {};
 

@@ -384,8 +384,9 @@ def orthogonalize(x, steps=5, eps=1e-7):
 
     x: a tensor [..., rows, cols] (a matrix or a stack of them) or a list / tuple of matrices of any shapes; float32,
     bfloat16 or float16, one type and device for all.  Returns the same structure, the same types; a matrix of zeros stays
-    zero, one with an infinity or a NaN becomes NaN.  All matrices share every launch.  Products are float32-accurate
-    whatever the type, rounded once at the end; the same call gives the same bits.  No gradient."""
+    zero, one with an infinity or a NaN becomes NaN.  All matrices share every launch.  Whatever the type, operands hold 22 to
+    23 bits and sums are float32 (errors 0.4 ... 3 times those of a float32 evaluation, 1e-6 of the result), rounded once at the
+    end; the same call gives the same bits.  No gradient, no forward mode."""
     many = isinstance(x, (list, tuple))
     mats = x if many else (x,)
     steps, eps = int(steps), float(eps)
