@@ -189,7 +189,7 @@ class ClippedSGD(object):
     def _buffers(self, act):
         """Parameters, gradients (element i of the gradient is element i of the weight) and momentum buffers."""
         ps, gs, bs = [], [], []
-        capturing, held = self._capturing(), self._held()
+        capturing = self._capturing()
         if self.skipped is None:
             if capturing:
                 raise RuntimeError(_EAGER_FIRST)
@@ -208,7 +208,7 @@ class ClippedSGD(object):
                     raise RuntimeError(_EAGER_FIRST)
                 b = self.state[p] = torch.zeros_like(p, memory_format=torch.preserve_format)
             elif b.stride() != p.stride():     # (and of the momentum: the weight may have changed its memory format)
-                if capturing or id(p) in held:
+                if capturing or id(p) in self._held():
                     raise RuntimeError("a weight of a captured step cannot change its memory format")
                 b = self.state[p] = torch.empty_like(p).copy_(b)
             ps.append(p); gs.append(g); bs.append(b)
