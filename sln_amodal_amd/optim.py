@@ -13,6 +13,13 @@ CAPTURES = 16          # steps that can be captured after an eager one (their ta
 _EAGER_FIRST = "take an eager step over the same parameters before captured ones (at least %d may follow it)" % (CAPTURES // 2)
 
 
+class _Captured(list):
+    """What captured steps over a weight hold, on the weight.  Copies and pickles of the weight start without."""
+
+    def __reduce__(self):
+        return _Captured, ()
+
+
 class ClippedSGD(object):
     """param_groups like torch.optim.SGD's ([{'params': [...], 'weight_decay': w}, ...]).  step(max_norm)
     clips over every parameter that holds a gradient and applies momentum SGD; the total gradient norm
@@ -231,11 +238,14 @@ class ClippedSGD(object):
             if not self._spares or self._spares[0].shape[1] != n:
                 raise RuntimeError(_EAGER_FIRST)
             stage = [self._spares.pop(), None]
-            # everything of the optimiser's own that the replays touch lives as long as the optimiser, whatever later eager
-            # steps put in its place: tables, chunk plan, momentum, and the memory that the weights had
-            self._captured.append((ps, bs, stage[0], self._plan, [p.detach() for p in ps], self.skipped, self.skipped_clamped))
+            # everything of the optimiser's own that the replays touch lives as long as the optimiser or one of the weights,
+            # whatever later eager steps put in its place: tables, chunk plan, momentum, and the memory that the weights had
+            step = (ps, bs, stage[0], self._plan, [p.detach() for p in ps], self.skipped, self.skipped_clamped)
+            self._captured.append(step)
             for p in ps:                       # (its replays write p without moving p's version: nothing made from p is kept)
-                p._sln_captured = True
+                if not getattr(p, "_sln_captured", None):
+                    p._sln_captured = _Captured()
+                p._sln_captured.append(step)
         else:
             if not self._ring or self._ring[0][0].shape[1] != n:
                 self._ring = [[torch.empty((3, n), dtype=torch.int64, pin_memory=True), None] for _ in range(4)]

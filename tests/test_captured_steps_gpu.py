@@ -1,7 +1,9 @@
 """GPU tests of optimiser steps that are captured into graphs beside what goes on eagerly: what layers keep of the weights, what
 the graphs' launches read, and what the optimiser's state does meanwhile.  Every comparison is for equal bits: a captured
 step is the same launches over the same values."""
+import copy
 import gc
+import pickle
 import weakref
 
 import pytest
@@ -275,3 +277,31 @@ def test_captures_in_a_row(kind):
     oa.capturing = True
     with pytest.raises(RuntimeError, match="nothing is being captured"):
         oa.step(5.0)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_a_captured_step_outlives_its_optimiser(kind):
+    """The graph is replayed after the optimiser went: what it reads hangs on the weights."""
+    a, oa, b, ob = _twins(kind)
+    static = _grads(a, 20)
+    _set(a, static)
+    graph = _capture(oa)
+    kept = [weakref.ref(t) for t in oa._plan] + [weakref.ref(t) for t in oa.state.values()]
+    for clone in (pickle.loads(pickle.dumps(a[0])), copy.deepcopy(a[0])):
+        assert not getattr(clone, "_sln_captured", None) and torch.equal(clone, a[0])
+    momentum = [oa.state[p] for p in a]
+    del oa
+    gc.collect()
+    assert all(r() is not None for r in kept)                     # (from the host, before any replay)
+    ones = _churn()
+    for r in range(3):
+        new = _grads(a, 40 + r)
+        for g, v in zip(static, new):
+            g.copy_(v)
+        graph.replay()
+        _set(b, [v.clone() for v in new])
+        ob.step(5.0)
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(a, b)) and \
+            all(torch.equal(m, ob.state[q]) for m, q in zip(momentum, b)), r
+    assert all((t == -1).all() for t in ones)
